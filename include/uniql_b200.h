@@ -42,7 +42,9 @@ enum {
   UNIQL_STATUS_BAD_TOKEN_ID = 1,  /* an embedding id was outside [0, vocab); row written as zeros */
   UNIQL_STATUS_WAIT_TIMEOUT = 2,  /* a bounded wait (asynchronous copy, or words another GPU has to write) gave up;
                                      the output is invalid */
-  UNIQL_STATUS_BAD_INDEX = 4      /* a slicing index pointed outside the source layer; that column / row was written as zeros */
+  UNIQL_STATUS_BAD_INDEX = 4,     /* a slicing index pointed outside the source layer; that column / row was written as zeros.
+                                     KV cache: a slot or page number outside the cache; that token was skipped / read as absent */
+  UNIQL_STATUS_NO_PAGE = 8        /* uniql_kv_page_plan: the free stack or a row of the block table was too short */
 };
 
 int uniql_abi_version(void);
@@ -328,6 +330,81 @@ int uniql_w4a16_gemv_plan_check(int64_t m, int64_t k, const int64_t* n, int npro
  * and a k-split, also when UNIQL_B200_TC_SPLIT asks for one that is too large.  Returns 0, or the row-tile size whose plan
  * breaks a rule the kernel relies on, or 1000 + the scale groups of a launch that gets no shape. */
 int uniql_w4a16_swap_plan_check(void);
+
+/*
+ * Attention around a paged KV cache held in 4 bits.  No counterpart in the reference, which keeps fp16 keys and values: these
+ * are the operators that a decoder block runs between its q/k/v linears and its o_proj.
+ *
+ * Cache (one per layer), both arrays 16-byte aligned and caller-owned:
+ *   codes   int32 [num_pages, 2, kv_heads, page_size, dp / 8]   index 0 of axis 1 is K, 1 is V; channel d of a row sits in
+ *           bits 4 (d % 8) .. 4 (d % 8) + 3 of word d / 8
+ *   scales  fp16 [num_pages, 2, kv_heads, page_size, 2]         (scale, zero) of each row: value = zero + scale * code
+ *   dp      stored row length, 64 or 128 channels; head sizes are multiples of 8 up to dp (K and V may differ), the channels
+ *           behind them hold code 0
+ *   page_size  16, 32, 64, 128 or 256 tokens.  Token t of a request sits in row t % page_size of page block_table[request][t /
+ *           page_size]; its slot is page * page_size + t % page_size.
+ * dtype is UNIQL_F16 or UNIQL_BF16; strides are in elements; softmax_scale is positive.  Integers on the device are never trusted with an address: lengths
+ * are clamped, pages and slots outside the cache are skipped (UNIQL_STATUS_BAD_INDEX).
+ *
+ * uniql_kv_page_plan: what a step's new tokens need, from the requests' lengths alone, without the host seeing any of it.
+ *   lens, new_lens   int32 [batch]: tokens cached before the step, tokens the step adds (negative counts as 0)
+ *   block_table      int32 [batch, max_blocks], row stride ld_table; entries ceil(len / page_size) .. ceil((len + new) /
+ *                    page_size) - 1 are written, the others left alone
+ *   free_pages       int32 [free_cap]: stack of free pages, of which free_count[0] are left.  Requests take theirs in order from
+ *                    the top.  Where it runs out the entry is -1, and so are the slots in it; tokens past max_blocks pages get
+ *                    slot -1 as well; either raises UNIQL_STATUS_NO_PAGE.
+ *   slots, positions int64 [total_new]: slot and position (len + j) of every new token, request after request; places
+ *                    behind the last token get -1 and 0, and tokens past total_new are not written
+ *   cu_new           int32 [batch + 1]: where each request's new tokens begin
+ *   lens_out         int32 [batch] = len + new, free_count_out int32 [1] = what is left; either may be its input
+ *   batch up to UNIQL_KV_MAX_BATCH.
+ *
+ * uniql_kv4_append: quantises the rows k[t], v[t] (t < tokens; [kv_heads, head] each, unit channel stride) and stores them at slots[t].
+ *   zero = fp16(min), scale = fp16((max - min) / 15) but at least 2^-24, code = the nearest to (x - zero) / scale, ties to even,
+ *   within 0..15.  Values beyond +-65504 are clamped to them first; a row that holds a NaN reads back as NaN.  A slot of -1
+ *   is skipped (padding); other slots of one call must differ.
+ *
+ * uniql_kv4_gather: rows of tokens starts[i] .. starts[i] + (cu[i + 1] - cu[i]) - 1 of every request i (starts NULL: from 0),
+ *   packed: k_out [total, kv_heads, dk], v_out [total, kv_heads, dv], each value rounded once.  Places that no request
+ *   covers, and tokens on a page outside the cache, are zeros.
+ *
+ * uniql_kv4_attention: one query token per request over its first lens[i] cached tokens (grouped heads: query head h reads kv head
+ *   h / (heads / kv_heads)): out[i, h] = softmax(softmax_scale * q k^T) v in fp32, rounded once.  Length 0, or no token on a page of
+ *   the cache, gives zeros.  The tokens are split evenly over the GPU whatever the lengths are, and the parts of a request are
+ *   joined in a fixed order.
+ *   scratch  uniql_kv4_attention_scratch_bytes(...) bytes, rules as for uniql_w4a16_linear
+ *
+ * uniql_prompt_attention: packed prompts.  Request i owns rows cu_q[i] .. cu_q[i + 1] - 1 of q [total_q, heads, dk] and out
+ *   [total_q, heads, dv] and rows cu_k[i] .. of k, v [total_k, kv_heads, dk / dv].  causal: query j sees the keys up to j + (keys -
+ *   queries), so that the last query sees them all; a query that sees none gives zeros, and so do rows of `out` that no
+ *   request owns.  k and v of tokens that other requests own never reach a request, whatever they hold; within a request a
+ *   non-finite v may reach queries in front of it that share its 128-row tile.
+ *   Rows must be 16-byte aligned (strides multiples of 8).  P is rounded to the input type in front of the second product.
+ */
+#define UNIQL_KV_MAX_BATCH 16384
+int uniql_kv_page_plan(const int32_t* lens, const int32_t* new_lens, int64_t batch, int32_t* block_table, int64_t ld_table,
+                       int64_t max_blocks, const int32_t* free_pages, int64_t free_cap, const int32_t* free_count,
+                       int64_t page_size, int64_t total_new, int64_t* slots, int64_t* positions, int32_t* cu_new,
+                       int32_t* lens_out, int32_t* free_count_out, int* status_word, void* stream);
+int uniql_kv4_append(const void* k, int64_t k_token_stride, int64_t k_head_stride, const void* v, int64_t v_token_stride,
+                     int64_t v_head_stride, int dtype, int64_t tokens, int64_t kv_heads, int64_t dk, int64_t dv,
+                     const int64_t* slots, void* codes, void* scales, int64_t num_pages, int64_t page_size, int64_t dp,
+                     int* status_word, void* stream);
+int uniql_kv4_gather(const void* codes, const void* scales, int64_t num_pages, int64_t page_size, int64_t dp, int64_t kv_heads,
+                     const int32_t* block_table, int64_t ld_table, int64_t max_blocks, int64_t batch, const int32_t* starts,
+                     const int32_t* cu, int64_t total, int64_t dk, int64_t dv, int dtype, void* k_out, void* v_out,
+                     int* status_word, void* stream);
+int uniql_kv4_attention(const void* q, int64_t q_batch_stride, int64_t q_head_stride, const void* codes, const void* scales,
+                        int64_t num_pages, int64_t page_size, int64_t dp, const int32_t* block_table, int64_t ld_table,
+                        int64_t max_blocks, const int32_t* lens, int64_t batch, int64_t heads, int64_t kv_heads, int64_t dk,
+                        int64_t dv, float softmax_scale, int dtype, void* out, void* scratch, size_t scratch_bytes,
+                        int* status_word, void* stream);
+size_t uniql_kv4_attention_scratch_bytes(int64_t batch, int64_t heads, int64_t kv_heads, int64_t dp);
+int uniql_prompt_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k, int64_t k_token_stride,
+                           int64_t k_head_stride, const void* v, int64_t v_token_stride, int64_t v_head_stride,
+                           const int32_t* cu_q, const int32_t* cu_k, int64_t batch, int64_t total_q, int64_t total_k,
+                           int64_t heads, int64_t kv_heads, int64_t dk, int64_t dv, float softmax_scale, int causal, int dtype,
+                           void* out, int* status_word, void* stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,563 @@
+// Attention of one query token per request over a paged KV cache held in 4 bits.  Layout and rules: include/uniql_b200.h.
+//
+// Mathematics.  With a cached row k_t = z + s c and m = z + 8 s the score is  x_t = f (s (q . (c - 8)) + m sum(q)),  f =
+// softmax_scale log2(e): the products run over the exact centred codes on the tensor cores (mma.sync m16n8k16, fp32 sums),
+// scale and zero enter once per token in fp32.  The value side folds its scale into the exponent: with y_t = x_t + log2 s'_t,
+// M a running bound of y and w_t = 2^(y_t - M),
+//     out = (sum w_t (c'_t - 8) + sum (w_t / s'_t) m'_t) / sum (w_t / s'_t),
+// so that w is the one operand that is rounded (fp16, 2^-12 relative above 6e-5; it is at most 2^8, see below), next to exact
+// codes, whatever the magnitude of the values.  M is raised, and the sums rescaled, only when some y exceeds it by more than 8.
+// Queries are taken to fp16 after a division by the power of two below their largest channel: exact, but for channels under 2^-14
+// of the largest.
+//
+// Layout of the products.  Tokens are the 16-row operand of the first product (a lane's packed words of two tokens are its
+// fragment; which channel sits at which k index is free, so long as the query fragments follow), query heads its eight
+// columns.  The weights w cross to the second product by two 8 x 8 transposes (movmatrix); there channels are the rows and the
+// tokens of a lane meet pairwise: two byte permutes join the same nibbles of two tokens.  So the 4-bit words go from shared
+// memory to the tensor cores with one LOP3 and one HSUB2 / HFMA2 per two codes.
+//
+// Bound: HBM, (dk + dv) / 2 + 8 bytes per token and kv head.  Each warp keeps a ring of kStages steps of 16 tokens in flight
+// with cp.async.  Split: the 64-token tiles of all requests form one list (a tile: one request, one kv head), cut into equal
+// ranges, one per CTA; lengths are read on the device.  A CTA whose range covers only a part of a request's list stores an
+// fp32 partial (sums, M), and the last CTA of that request to arrive joins the parts in order: deterministic.
+#include "common.cuh"
+#include "kv_cache.cuh"
+#include "tma.cuh"
+
+namespace uniql {
+
+namespace kva {
+constexpr int kWarps = 4, kThreads = kWarps * 32;
+constexpr int kStages = 4;
+constexpr int kTile = 16 * kWarps;              // tokens of a tile
+constexpr float kFloor = -1e30f;                // M before the first token
+constexpr int kMaxCtas = 2048;
+}  // namespace kva
+
+struct KvaParams {
+  const unsigned char* q;
+  int64_t q_bs, q_hs;                           // elements
+  const unsigned char* codes;
+  const unsigned char* scales;
+  const int32_t* table;
+  int64_t ld_table;
+  const int32_t* lens;
+  unsigned char* out;
+  float* part;                                  // [2 * ctas][8 NT][DP + 2]
+  int* tickets;                                 // [ctas], zero
+  int* status_word;
+  int batch, heads, kv_heads, group, hgroups;   // group: query heads of a kv head; hgroups: launches of 8 NT of them
+  int max_blocks, num_pages, page_shift, dk, dv, bf16;
+  float scale_log2;
+};
+
+__device__ __forceinline__ void kva_cp16(uint32_t dst, const void* src, bool real) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(real ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ uint32_t kva_lds32(uint32_t a) {
+  uint32_t v;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
+  return v;
+}
+__device__ __forceinline__ float kva_exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t kva_transpose(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+__device__ __forceinline__ float kva_load(const unsigned char* p, int64_t i, int bf16) {
+  return bf16 ? __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(p)[i]) : __half2float(reinterpret_cast<const __half*>(p)[i]);
+}
+__device__ __forceinline__ void kva_store(unsigned char* p, int64_t i, int bf16, float v) {
+  if (bf16) reinterpret_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
+  else reinterpret_cast<__half*>(p)[i] = __float2half_rn(v);
+}
+
+// The token (of a step's 16) that sits at row / k index r of the products: k = 2c, 2c + 1, 2c + 8, 2c + 9 are tokens c, 7 - c, 8 + c
+// and 15 - c.  With it, and the 16-byte chunks of 64-byte rows swapped in pairs by bit 1 of the token, both the rows (four lanes
+// a row) and the columns (eight lanes a row, four tokens) are read from shared memory without bank conflicts.
+__device__ __forceinline__ int kva_token(int r) { return (r & 8) + ((r & 1) ? 7 - ((r & 7) >> 1) : ((r & 7) >> 1)); }
+
+template <int DP, int NT>
+__global__ void __launch_bounds__(kva::kThreads, NT == 1 ? 4 : 2) kv4_attention_kernel(const __grid_constant__ KvaParams p) {
+  using namespace kva;
+  constexpr int ROWB = DP / 2;                  // bytes of a packed row
+  constexpr int CODEB = 16 * ROWB;              // one step's packed rows, K or V
+  constexpr int STAGEB = 2 * CODEB + 128;       // K codes, V codes, K scales, V scales
+  constexpr int RINGB = kStages * STAGEB;
+  constexpr int H = 8 * NT, MT = DP / 16, QK = DP / 16;
+  constexpr int PSTR = DP + 2;                  // floats of one head's partial
+  extern __shared__ __align__(16) unsigned char smem[];
+  __shared__ long long s_wide[kWarps];
+  __shared__ float s_m[kWarps][H], s_l[kWarps][H], s_z[kWarps][H];
+  __shared__ int s_find[2];
+  __shared__ long long s_before;
+  __shared__ int s_last;
+  pdl_wait();
+  pdl_launch_dependents();
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
+  const int cap = min((int64_t)p.max_blocks << p.page_shift, (int64_t)kMaxTokens);
+  const int lists = p.kv_heads * p.hgroups;     // tile lists of a request
+  auto length = [&](int b) { return min(max(p.lens[b], 0), cap); };
+
+  // ---- this CTA's range of the list of all tiles
+  const int per = (p.batch + kThreads - 1) / kThreads;
+  long long mine = 0;
+  for (int b = tid * per; b < min((tid + 1) * per, p.batch); ++b) mine += (length(b) + kTile - 1) / kTile;
+  long long incl = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long v = __shfl_up_sync(~0u, incl, o);
+    if (lane >= o) incl += v;
+  }
+  if (lane == 31) s_wide[warp] = incl;
+  __syncthreads();
+  long long total = 0, before = incl - mine;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) {
+    if (w < warp) before += s_wide[w];
+    total += s_wide[w];
+  }
+  const long long N = total * lists;            // at most 2^28 / 64 * 2^14 * 2^10 < 2^47; times the CTAs below 2^58
+  const long long ctas = min((long long)gridDim.x, N);
+  const long long begin = blockIdx.x < ctas ? N * blockIdx.x / ctas : 0;
+  const long long end = blockIdx.x < ctas ? N * (blockIdx.x + 1) / ctas : 0;
+  // idle rows of the batch
+  for (int b = blockIdx.x; b < p.batch; b += gridDim.x)
+    if (length(b) == 0)
+      for (int i = tid; i < p.heads * p.dv; i += kThreads) kva_store(p.out, (int64_t)b * p.heads * p.dv + i, p.bf16, 0.f);
+  if (begin == end) return;
+  if (mine && before * lists <= begin && begin < (before + mine) * lists) {
+    long long at = before;
+    for (int b = tid * per; b < min((tid + 1) * per, p.batch); ++b) {
+      const int t = (length(b) + kTile - 1) / kTile;
+      if (begin < (at + t) * lists) {
+        s_find[0] = b;
+        s_before = at * lists;
+        break;
+      }
+      at += t;
+    }
+  }
+  __syncthreads();
+  int b = s_find[0];
+  long long req_begin = s_before;
+
+  const uint32_t ring = smem_addr(smem) + warp * RINGB;
+  const int tok_a = kva_token(g);               // rows g and g + 8 of the first product: tokens tok_a and 8 + tok_a
+  bool bad_page = false;
+
+  for (long long cur = begin; cur < end;) {
+    int len = length(b);
+    int tiles = (len + kTile - 1) / kTile;
+    while (cur >= req_begin + (long long)tiles * lists) {       // next request that has tokens
+      req_begin += (long long)tiles * lists;
+      ++b;
+      len = length(b);
+      tiles = (len + kTile - 1) / kTile;
+    }
+    const int list = (int)((cur - req_begin) / tiles);
+    const long long list_begin = req_begin + (long long)list * tiles;
+    const int t0 = (int)(cur - list_begin);
+    const int t1 = (int)min((long long)tiles, t0 + (end - cur));
+    const int kvh = list / p.hgroups, hg = list - kvh * p.hgroups;
+    const int head0 = kvh * p.group + hg * H;                   // first query head of this list
+    const int nh = min(H, p.group - hg * H);
+    cur += t1 - t0;
+
+    // ---- producer: step `st` (16 tokens) of this warp into ring slot st / kWarps % kStages
+    const int first = t0 * kWarps + warp, last = min(t1 * kWarps, (len + 15) / 16);   // steps first, first + kWarps, .. < last
+    const int32_t* trow = p.table + (size_t)b * p.ld_table;
+    const int pmask = (1 << p.page_shift) - 1;
+    uint32_t absent = 0;                        // bit i: ring slot i holds a step whose page is outside the cache
+    int next_page = first < last ? trow[first * 16 >> p.page_shift] : 0;
+    auto produce = [&](int st, int slot) {
+      if (st < last) {
+        const int page = next_page;
+        if (st + kWarps < last) next_page = trow[(st + kWarps) * 16 >> p.page_shift];
+        const bool ok = (unsigned)page < (unsigned)p.num_pages;
+        bad_page |= !ok;
+        absent = (absent & ~(1u << slot)) | ((ok ? 0u : 1u) << slot);
+        const size_t row = (((size_t)(ok ? page : 0) * 2 * p.kv_heads + kvh) << p.page_shift) + (st * 16 & pmask);
+        const size_t vrow = row + ((size_t)p.kv_heads << p.page_shift);
+        const uint32_t dst = ring + slot * STAGEB;
+#pragma unroll
+        for (int i = 0; i < CODEB / 512; ++i) {
+          const int ch = lane + 32 * i;         // 16-byte chunk of the step
+          uint32_t d = ch * 16;
+          if (DP == 128) d ^= ((ch >> 3) & 1) << 5;             // chunk of token t = ch / 4 moves to chunk ^ (t & 2)
+          // an absent page copies nothing, from an address that exists
+          kva_cp16(dst + d, ok ? p.codes + row * ROWB + ch * 16 : (const unsigned char*)p.part, ok);
+          kva_cp16(dst + CODEB + d, ok ? p.codes + vrow * ROWB + ch * 16 : (const unsigned char*)p.part, ok);
+        }
+        if (lane < 8)
+          kva_cp16(dst + 2 * CODEB + lane * 16, ok ? p.scales + (lane < 4 ? row : vrow) * 4 + (lane & 3) * 16 : (const unsigned char*)p.part, ok);
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+#pragma unroll
+    for (int i = 0; i < kStages - 1; ++i) produce(first + i * kWarps, i);
+
+    // ---- query fragments
+    uint32_t qf[NT][2 * QK];
+    float f[NT][2], fq[NT][2];                  // per head 8 nt + 2c + e: f 2^e_h, f sum(q)
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int h = nt * 8 + g;
+      const int64_t base = (int64_t)b * p.q_bs + (int64_t)(head0 + h) * p.q_hs;
+      float v[DP / 4];
+      float top = 0.f, sum = 0.f;
+#pragma unroll
+      for (int i = 0; i < DP / 4; ++i) {
+        const int d = c * (DP / 4) + i;
+        v[i] = (h < nh && d < p.dk) ? kva_load(p.q, base + d, p.bf16) : 0.f;
+        top = fmaxf(top, fabsf(v[i]));
+        sum += v[i];
+      }
+#pragma unroll
+      for (int o = 1; o < 4; o <<= 1) {
+        top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
+        sum += __shfl_xor_sync(~0u, sum, o);
+      }
+      // 2^-e with 2^e <= top < 2^(e + 1), kept where both powers are normal numbers; 1 for zeros and infinities
+      const int eb = (__float_as_int(top) >> 23) & 255;
+      const bool scaled = eb >= 1 && eb <= 253;
+      const float down = scaled ? __int_as_float((254 - eb) << 23) : 1.f, up = scaled ? __int_as_float(eb << 23) : 1.f;
+#pragma unroll
+      for (int i = 0; i < DP / 32; ++i)
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+          const __half2 h2 = __floats2half2_rn(v[8 * i + n] * down, v[8 * i + n + 4] * down);
+          qf[nt][4 * i + n] = *reinterpret_cast<const uint32_t*>(&h2);
+        }
+      const float fh = p.scale_log2 * up, fs = p.scale_log2 * sum;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {             // heads 2c and 2c + 1 are lanes' g = 2c, 2c + 1
+        f[nt][e] = __shfl_sync(~0u, fh, (2 * c + e) * 4);
+        fq[nt][e] = __shfl_sync(~0u, fs, (2 * c + e) * 4);
+      }
+    }
+
+    float o[NT][MT][4], M[NT][2], L[NT][2], Z[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+      for (int i = 0; i < MT; ++i) o[nt][i][0] = o[nt][i][1] = o[nt][i][2] = o[nt][i][3] = 0.f;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) { M[nt][e] = kFloor; L[nt][e] = Z[nt][e] = 0.f; }
+    }
+
+    int slot = 0;
+    for (int st = first; st < last; st += kWarps) {
+      const int fill = slot == 0 ? kStages - 1 : slot - 1;
+      produce(st + (kStages - 1) * kWarps, fill);
+      asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
+      __syncwarp();
+      const uint32_t sk = ring + slot * STAGEB, sv = sk + CODEB, ss = sv + CODEB;
+      // ---- scores of 16 tokens
+      float x[NT][4];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) x[nt][0] = x[nt][1] = x[nt][2] = x[nt][3] = 0.f;
+      {
+        uint32_t wa[DP / 32], wb[DP / 32];
+        if (DP == 128) {
+          const uint32_t ad = sk + tok_a * ROWB + ((c * 16) ^ ((tok_a & 2) << 4));
+          const uint4 a = lds128(ad), e = lds128(ad + 8 * ROWB);
+          wa[0] = a.x; wa[1] = a.y; wa[DP / 32 - 2] = a.z; wa[DP / 32 - 1] = a.w;
+          wb[0] = e.x; wb[1] = e.y; wb[DP / 32 - 2] = e.z; wb[DP / 32 - 1] = e.w;
+        } else {
+          const uint32_t ad = sk + tok_a * ROWB + c * 8;
+          const uint2 a = lds64(ad), e = lds64(ad + 8 * ROWB);
+          wa[0] = a.x; wa[1] = a.y;
+          wb[0] = e.x; wb[1] = e.y;
+        }
+#pragma unroll
+        for (int i = 0; i < DP / 32; ++i) {
+          const uint32_t a8 = wa[i] >> 8, b8 = wb[i] >> 8;
+          const uint32_t lo[4] = {kv4_pair(wa[i], 0x64086408u), kv4_pair(wb[i], 0x64086408u),
+                                  kv4_pair_hi(wa[i], 0xd480d480u), kv4_pair_hi(wb[i], 0xd480d480u)};
+          const uint32_t hi[4] = {kv4_pair(a8, 0x64086408u), kv4_pair(b8, 0x64086408u),
+                                  kv4_pair_hi(a8, 0xd480d480u), kv4_pair_hi(b8, 0xd480d480u)};
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            mma_m16n8k16(x[nt], lo, qf[nt][4 * i], qf[nt][4 * i + 1]);
+            mma_m16n8k16(x[nt], hi, qf[nt][4 * i + 2], qf[nt][4 * i + 3]);
+          }
+        }
+      }
+      // ---- weights
+      const int limit = ((absent >> slot) & 1) ? 0 : len - st * 16;    // tokens of this step that exist
+      float ls[2], rs[2], zc[2];
+      bool over = false;
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const int t = tok_a + 8 * r;
+        const uint32_t km = kva_lds32(ss + t * 4), vm = kva_lds32(ss + 64 + t * 4);
+        const float2 kf = __half22float2(*reinterpret_cast<const __half2*>(&km));
+        const float2 vf = __half22float2(*reinterpret_cast<const __half2*>(&vm));
+        const bool real = t < limit;
+        const float m = fmaf(8.f, kf.x, kf.y);
+        const float vs = real ? fmaxf(vf.x, 5.9604645e-8f) : 1.f;
+        ls[r] = real ? __log2f(vs) : -INFINITY;
+        rs[r] = __fdividef(1.f, vs);
+        zc[r] = real ? fmaf(8.f, vf.x, vf.y) : 0.f;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float y = fmaf(x[nt][2 * r + e] * kf.x, f[nt][e], m * fq[nt][e]) + ls[r];
+            y = real ? y : -INFINITY;
+            x[nt][2 * r + e] = y;
+            over |= y > M[nt][e] + 8.f;
+          }
+      }
+      if (__any_sync(~0u, over)) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float top = fmaxf(x[nt][e], x[nt][2 + e]);
+#pragma unroll
+            for (int s = 4; s < 32; s <<= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, s));
+            top = fmaxf(top, M[nt][e]);
+            const float k = kva_exp2(M[nt][e] - top);
+            M[nt][e] = top;
+            L[nt][e] *= k;
+            Z[nt][e] *= k;
+#pragma unroll
+            for (int i = 0; i < MT; ++i) { o[nt][i][e] *= k; o[nt][i][2 + e] *= k; }
+          }
+      }
+      uint32_t pb[NT][2];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          float w[2];
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            w[e] = kva_exp2(x[nt][2 * r + e] - M[nt][e]);
+            const float l = w[e] * rs[r];
+            L[nt][e] += l;
+            Z[nt][e] = fmaf(l, zc[r], Z[nt][e]);
+          }
+          const __half2 h2 = __floats2half2_rn(w[0], w[1]);
+          pb[nt][r] = kva_transpose(*reinterpret_cast<const uint32_t*>(&h2));
+        }
+      // ---- weighted sums of the codes
+      {
+        uint32_t u[4][DP / 64];                 // tokens c, 7 - c, 8 + c, 15 - c: this lane's words
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int t = (j & 2) * 4 + ((j & 1) ? 7 - c : c);
+          if (DP == 128) {
+            const uint2 v = lds64(sv + t * ROWB + ((g * 8) ^ ((t & 2) << 4)));
+            u[j][0] = v.x; u[j][DP / 64 - 1] = v.y;
+          } else {
+            u[j][0] = kva_lds32(sv + t * ROWB + g * 4);
+          }
+        }
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {  // nibbles 0-3, 4-7 of the words
+          const uint32_t sel = half ? 0x7632 : 0x5410;
+          uint32_t w[2][DP / 64];
+#pragma unroll
+          for (int k = 0; k < DP / 64; ++k) {
+            w[0][k] = __byte_perm(u[0][k], u[1][k], sel);
+            w[1][k] = __byte_perm(u[2][k], u[3][k], sel);
+          }
+          if (DP == 128) {
+            // row g: channel 16 g + n of word 2g, row g + 8: channel 16 g + 8 + n of word 2g + 1
+            constexpr int k1 = DP / 64 - 1;
+            const uint32_t s00 = w[0][0] >> 8, s01 = w[0][k1] >> 8, s10 = w[1][0] >> 8, s11 = w[1][k1] >> 8;
+            const uint32_t a[4][4] = {
+                {kv4_pair(w[0][0], 0x64086408u), kv4_pair(w[0][k1], 0x64086408u), kv4_pair(w[1][0], 0x64086408u), kv4_pair(w[1][k1], 0x64086408u)},
+                {kv4_pair_hi(w[0][0], 0xd480d480u), kv4_pair_hi(w[0][k1], 0xd480d480u), kv4_pair_hi(w[1][0], 0xd480d480u), kv4_pair_hi(w[1][k1], 0xd480d480u)},
+                {kv4_pair(s00, 0x64086408u), kv4_pair(s01, 0x64086408u), kv4_pair(s10, 0x64086408u), kv4_pair(s11, 0x64086408u)},
+                {kv4_pair_hi(s00, 0xd480d480u), kv4_pair_hi(s01, 0xd480d480u), kv4_pair_hi(s10, 0xd480d480u), kv4_pair_hi(s11, 0xd480d480u)}};
+#pragma unroll
+            for (int n = 0; n < 4; ++n)
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) mma_m16n8k16(o[nt][4 * half % MT + n], a[n], pb[nt][0], pb[nt][1]);
+          } else if (half == 0) {
+            // row g: channel 8 g + n, row g + 8: channel 8 g + 4 + n of word g
+            const uint32_t h0 = __byte_perm(u[0][0], u[1][0], 0x7632), h1 = __byte_perm(u[2][0], u[3][0], 0x7632);
+            const uint32_t l0 = w[0][0], l1 = w[1][0];
+            const uint32_t l08 = l0 >> 8, l18 = l1 >> 8, h08 = h0 >> 8, h18 = h1 >> 8;
+            const uint32_t a[4][4] = {
+                {kv4_pair(l0, 0x64086408u), kv4_pair(h0, 0x64086408u), kv4_pair(l1, 0x64086408u), kv4_pair(h1, 0x64086408u)},
+                {kv4_pair_hi(l0, 0xd480d480u), kv4_pair_hi(h0, 0xd480d480u), kv4_pair_hi(l1, 0xd480d480u), kv4_pair_hi(h1, 0xd480d480u)},
+                {kv4_pair(l08, 0x64086408u), kv4_pair(h08, 0x64086408u), kv4_pair(l18, 0x64086408u), kv4_pair(h18, 0x64086408u)},
+                {kv4_pair_hi(l08, 0xd480d480u), kv4_pair_hi(h08, 0xd480d480u), kv4_pair_hi(l18, 0xd480d480u), kv4_pair_hi(h18, 0xd480d480u)}};
+#pragma unroll
+            for (int n = 0; n < 4; ++n)
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) mma_m16n8k16(o[nt][n], a[n], pb[nt][0], pb[nt][1]);
+          }
+        }
+      }
+      __syncwarp();                             // the slot's words are in registers of the whole warp before it is refilled
+      slot = slot + 1 == kStages ? 0 : slot + 1;
+    }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+
+    // ---- join the warps: sums over the lanes that share a head, then over the warps through shared memory
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+#pragma unroll
+        for (int s = 4; s < 32; s <<= 1) {
+          L[nt][e] += __shfl_xor_sync(~0u, L[nt][e], s);
+          Z[nt][e] += __shfl_xor_sync(~0u, Z[nt][e], s);
+        }
+        if (g == 0) {
+          const int h = nt * 8 + 2 * c + e;
+          s_m[warp][h] = M[nt][e];
+          s_l[warp][h] = L[nt][e];
+          s_z[warp][h] = Z[nt][e];
+        }
+      }
+    __syncthreads();                            // every warp has read its ring: it becomes the exchange area
+    float* ex = reinterpret_cast<float*>(smem);   // [warp][head][DP]
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int h = nt * 8 + 2 * c + (e & 1);
+          // DP 128: tile i = nibble i, rows 16 g + i and 16 g + 8 + i; DP 64: rows 8 g + i and 8 g + 4 + i
+          const int d = DP == 128 ? 16 * g + i + ((e & 2) ? 8 : 0) : 8 * g + i + ((e & 2) ? 4 : 0);
+          ex[(warp * H + h) * DP + d] = o[nt][i][e];
+        }
+    __syncthreads();
+    const bool whole = t0 == 0 && t1 == tiles;
+    // parts of a list sit in the slots of their CTAs: 2 cta + 1 if the list begins in the CTA's range, else 2 cta
+    const int my_slot = 2 * (int)blockIdx.x + (t0 == 0 ? 1 : 0);
+    for (int i = tid; i < nh * DP; i += kThreads) {
+      const int h = i / DP, d = i - h * DP;
+      float top = s_m[0][h];
+#pragma unroll
+      for (int w = 1; w < kWarps; ++w) top = fmaxf(top, s_m[w][h]);
+      float acc = 0.f, l = 0.f;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        const float k = kva_exp2(s_m[w][h] - top);
+        acc = fmaf(k, ex[(w * H + h) * DP + d] + s_z[w][h], acc);
+        l = fmaf(k, s_l[w][h], l);
+      }
+      if (whole) {
+        if (d < p.dv) kva_store(p.out, ((int64_t)b * p.heads + head0 + h) * p.dv + d, p.bf16, l == 0.f ? 0.f : acc / l);
+      } else {
+        float* dst = p.part + ((size_t)my_slot * H + h) * PSTR;
+        dst[d] = acc;
+        if (d == 0) { dst[DP] = top; dst[DP + 1] = l; }
+      }
+    }
+    if (!whole) {
+      // CTAs of this list: the ones whose ranges hold its first and its last tile
+      const long long last_tile = list_begin + tiles - 1;
+      const int c0 = (int)(((list_begin + 1) * ctas - 1) / N), c1 = (int)(((last_tile + 1) * ctas - 1) / N);
+      __threadfence();
+      __syncthreads();
+      if (tid == 0) s_last = atomicAdd(p.tickets + c0, 1) == c1 - c0;
+      __syncthreads();
+      if (s_last) {
+        __threadfence();
+        for (int i = tid; i < nh * DP; i += kThreads) {
+          const int h = i / DP, d = i - h * DP;
+          if (d >= p.dv) continue;
+          float top = kFloor;
+          for (int k = c0; k <= c1; ++k) top = fmaxf(top, __ldcg(p.part + ((size_t)(2 * k + (k == c0)) * H + h) * PSTR + DP));
+          float acc = 0.f, l = 0.f;
+          for (int k = c0; k <= c1; ++k) {
+            const float* src = p.part + ((size_t)(2 * k + (k == c0)) * H + h) * PSTR;
+            const float w = kva_exp2(__ldcg(src + DP) - top);
+            acc = fmaf(w, __ldcg(src + d), acc);
+            l = fmaf(w, __ldcg(src + DP + 1), l);
+          }
+          kva_store(p.out, ((int64_t)b * p.heads + head0 + h) * p.dv + d, p.bf16, l == 0.f ? 0.f : acc / l);
+        }
+        if (tid == 0) p.tickets[c0] = 0;
+      }
+    }
+    __syncthreads();                            // the exchange area becomes the ring again
+  }
+  if (bad_page && p.status_word) atomicOr(p.status_word, UNIQL_STATUS_BAD_INDEX);
+}
+
+template <int DP, int NT>
+static constexpr size_t kva_smem() {
+  const size_t ring = (size_t)kva::kWarps * kva::kStages * (16 * DP + 128);
+  const size_t ex = (size_t)kva::kWarps * 8 * NT * DP * 4;
+  return ring > ex ? ring : ex;
+}
+
+static int kva_ctas(int nt) {
+  const int n = device_info().sm_count * (nt == 1 ? 4 : 2);
+  return n < kva::kMaxCtas ? n : kva::kMaxCtas;
+}
+static int kva_nt(int64_t heads, int64_t kv_heads) { return heads / kv_heads > 8 ? 2 : 1; }
+
+template <int DP, int NT>
+static int kva_launch(KvaParams& p, cudaStream_t stream) {
+  static thread_local bool attr_set[64] = {};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= 64 || !attr_set[dev]) {
+    UNIQL_CUDA_TRY(cudaFuncSetAttribute(kv4_attention_kernel<DP, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                        (int)kva_smem<DP, NT>()));
+    if (dev >= 0 && dev < 64) attr_set[dev] = true;
+  }
+  return launch_pdl(kv4_attention_kernel<DP, NT>, (unsigned)kva_ctas(NT), kva::kThreads, kva_smem<DP, NT>(), stream, p);
+}
+
+}  // namespace uniql
+
+extern "C" size_t uniql_kv4_attention_scratch_bytes(int64_t batch, int64_t heads, int64_t kv_heads, int64_t dp) {
+  using namespace uniql;
+  if (batch <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || (dp != 64 && dp != 128)) return 0;
+  const int nt = kva_nt(heads, kv_heads);
+  return UNIQL_SCRATCH_COUNTER_BYTES + (size_t)2 * kva_ctas(nt) * 8 * nt * (dp + 2) * sizeof(float);
+}
+
+extern "C" int uniql_kv4_attention(const void* q, int64_t q_batch_stride, int64_t q_head_stride, const void* codes,
+                                   const void* scales, int64_t num_pages, int64_t page_size, int64_t dp,
+                                   const int32_t* block_table, int64_t ld_table, int64_t max_blocks, const int32_t* lens,
+                                   int64_t batch, int64_t heads, int64_t kv_heads, int64_t dk, int64_t dv, float softmax_scale,
+                                   int dtype, void* out, void* scratch, size_t scratch_bytes, int* status_word, void* stream) {
+  using namespace uniql;
+  static_assert(kva::kMaxCtas * sizeof(int) <= UNIQL_SCRATCH_COUNTER_BYTES, "a ticket per CTA");
+  if (batch < 0 || heads <= 0 || kv_heads <= 0 || num_pages < 0 || dk <= 0 || dv <= 0 || max_blocks < 0 || ld_table < max_blocks)
+    return UNIQL_EINVAL;
+  if (dtype != UNIQL_F16 && dtype != UNIQL_BF16) return UNIQL_EDTYPE;
+  int st = kv4_check(num_pages, page_size, dp, kv_heads, dk, dv);
+  if (st != UNIQL_OK) return st;
+  if (heads % kv_heads || heads > 16384 || batch > UNIQL_KV_MAX_BATCH || max_blocks > kMaxTokens) return UNIQL_ESHAPE;
+  if (!(softmax_scale > 0.f) || softmax_scale > 1e30f) return UNIQL_EINVAL;
+  if (batch == 0) return UNIQL_OK;
+  if (!q || !lens || !out || (max_blocks > 0 && !block_table)) return UNIQL_EINVAL;
+  if (num_pages > 0 && (!codes || !scales || !aligned16(codes) || !aligned16(scales))) return UNIQL_EINVAL;
+  if (!scratch || (reinterpret_cast<uintptr_t>(scratch) & 255u) ||
+      scratch_bytes < uniql_kv4_attention_scratch_bytes(batch, heads, kv_heads, dp))
+    return UNIQL_ESCRATCH;
+  KvaParams p;
+  p.q = (const unsigned char*)q; p.q_bs = q_batch_stride; p.q_hs = q_head_stride;
+  p.codes = (const unsigned char*)codes; p.scales = (const unsigned char*)scales;
+  p.table = block_table; p.ld_table = ld_table; p.lens = lens; p.out = (unsigned char*)out;
+  p.tickets = (int*)scratch; p.part = (float*)((char*)scratch + UNIQL_SCRATCH_COUNTER_BYTES); p.status_word = status_word;
+  const int nt = kva_nt(heads, kv_heads);
+  p.batch = (int)batch; p.heads = (int)heads; p.kv_heads = (int)kv_heads; p.group = (int)(heads / kv_heads);
+  p.hgroups = (p.group + 8 * nt - 1) / (8 * nt);
+  p.max_blocks = (int)max_blocks; p.num_pages = (int)num_pages; p.page_shift = page_shift_of(page_size);
+  p.dk = (int)dk; p.dv = (int)dv; p.bf16 = dtype == UNIQL_BF16;
+  p.scale_log2 = softmax_scale * 1.44269504088896340736f;
+  cudaStream_t s = (cudaStream_t)stream;
+  if (dp == 128) return nt == 1 ? kva_launch<128, 1>(p, s) : kva_launch<128, 2>(p, s);
+  return nt == 1 ? kva_launch<64, 1>(p, s) : kva_launch<64, 2>(p, s);
+}

@@ -1,0 +1,451 @@
+// The paged 4-bit KV cache: planning of its pages, the quantising write and the dequantising read.  Layout and rules:
+// include/uniql_b200.h.  No counterpart in UniQL.
+#include "common.cuh"
+#include "kv_cache.cuh"
+
+namespace uniql {
+
+// ------------------------------------------------------------------------------------------------ page plan
+// need_i = ceil((len_i + new_i) / P) - ceil(len_i / P), cut at the width of the table; the exclusive sums of need and new
+// say which entries of the free stack and which places of the packed tokens a request owns.  Every CTA of one cluster
+// computes both sums for the whole batch (8 bytes a request from L2) and keeps them in shared memory; the new pages and
+// the new tokens are then flat lists that all threads walk, each finding its request by bisection, so that one prompt of
+// thousands of tokens costs no more than thousands of single ones.  lens and free_count may be overwritten in place: that
+// is done behind a cluster barrier, when every CTA has read them.
+constexpr int kPlanThreads = 1024, kPlanCap = 1 << 30;
+
+struct PlanParams {
+  const int32_t* lens;
+  const int32_t* new_lens;
+  int32_t* table;
+  int64_t ld_table;
+  const int32_t* free_pages;
+  const int32_t* free_count;
+  int64_t* slots;
+  int64_t* positions;
+  int32_t* cu_new;
+  int32_t* lens_out;
+  int32_t* free_count_out;
+  int* status_word;
+  int64_t total_new;
+  int batch, max_blocks, free_cap, page_shift;
+};
+
+// largest i with start[i] <= x, for start[0] = 0 <= x
+__device__ __forceinline__ int plan_find(const int* start, int n, int x) {
+  int lo = 0, hi = n;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (start[mid] <= x) lo = mid; else hi = mid;
+  }
+  return lo;
+}
+
+__global__ void __launch_bounds__(kPlanThreads) kv_page_plan_kernel(const __grid_constant__ PlanParams p) {
+  extern __shared__ int plan_smem[];
+  int* s_len = plan_smem;                       // [batch]
+  int* s_cu = s_len + p.batch;                  // [batch + 1]
+  int* s_first = s_cu + p.batch + 1;            // [batch + 1]
+  __shared__ long long warp_new[32], warp_need[32];
+  __shared__ long long carry_new, carry_need;
+  __shared__ int s_count;
+  pdl_wait();
+  pdl_launch_dependents();
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int pmask = (1 << p.page_shift) - 1;
+  if (tid == 0) {
+    carry_new = carry_need = 0;
+    s_cu[0] = s_first[0] = 0;                   // all there is of them when the batch is empty
+    s_count = min(max(p.free_count[0], 0), p.free_cap);
+  }
+  bool short_table = false;
+  __syncthreads();
+  for (int i0 = 0; i0 < p.batch; i0 += kPlanThreads) {
+    const int i = i0 + tid;
+    int len = 0, add = 0, need = 0;
+    if (i < p.batch) {
+      len = min(max(p.lens[i], 0), kMaxTokens);
+      add = min(max(p.new_lens[i], 0), kMaxTokens);
+      const int had = (len + pmask) >> p.page_shift, has = (len + add + pmask) >> p.page_shift;
+      need = max(min(has, p.max_blocks) - had, 0);
+      short_table |= has > p.max_blocks && add > 0;
+      s_len[i] = len;
+    }
+    long long xn = add, xb = need;              // inclusive sums over the warp, then over the block
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long a = __shfl_up_sync(~0u, xn, o), b = __shfl_up_sync(~0u, xb, o);
+      if (lane >= o) { xn += a; xb += b; }
+    }
+    if (lane == 31) { warp_new[warp] = xn; warp_need[warp] = xb; }
+    __syncthreads();
+    if (warp == 0) {
+      long long a = warp_new[lane], b = warp_need[lane];
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const long long c = __shfl_up_sync(~0u, a, o), d = __shfl_up_sync(~0u, b, o);
+        if (lane >= o) { a += c; b += d; }
+      }
+      warp_new[lane] = a;
+      warp_need[lane] = b;
+    }
+    __syncthreads();
+    const long long bn = carry_new + (warp ? warp_new[warp - 1] : 0), bb = carry_need + (warp ? warp_need[warp - 1] : 0);
+    // sums of lengths that nobody can mean stop at kPlanCap: the lists below stay sorted, and places under it are exact
+    if (i < p.batch) {
+      s_cu[i] = (int)min(bn + xn - add, (long long)kPlanCap);
+      s_first[i] = (int)min(bb + xb - need, (long long)kPlanCap);
+    }
+    __syncthreads();
+    if (tid == kPlanThreads - 1) {
+      carry_new = bn + xn;
+      carry_need = bb + xb;
+      s_cu[min(i0 + kPlanThreads, p.batch)] = (int)min(carry_new, (long long)kPlanCap);      // the next round writes the same value
+      s_first[min(i0 + kPlanThreads, p.batch)] = (int)min(carry_need, (long long)kPlanCap);
+    }
+    __syncthreads();
+  }
+  const int tokens = s_cu[p.batch], pages = s_first[p.batch], count = s_count;
+  const int rank = blockIdx.x, ranks = gridDim.x, step = ranks * kPlanThreads;
+  for (int x = rank * kPlanThreads + tid; x < pages; x += step) {
+    const int i = plan_find(s_first, p.batch, x);
+    const int had = (s_len[i] + pmask) >> p.page_shift;
+    p.table[(size_t)i * p.ld_table + had + (x - s_first[i])] = x < count ? p.free_pages[count - 1 - x] : -1;
+  }
+  for (int64_t x = (int64_t)rank * kPlanThreads + tid; x < p.total_new; x += step) {
+    int64_t slot = -1, pos = 0;
+    if (x < tokens) {
+      const int i = plan_find(s_cu, p.batch, (int)x);
+      const int len = s_len[i], at = len + ((int)x - s_cu[i]), had = (len + pmask) >> p.page_shift;
+      const int block = at >> p.page_shift;
+      int page = -1;
+      if (block < p.max_blocks) {
+        const int r = s_first[i] + block - had;
+        if (block < had) page = p.table[(size_t)i * p.ld_table + block];
+        else if (r < count) page = p.free_pages[count - 1 - r];
+      }
+      pos = at;
+      if (page >= 0) slot = ((int64_t)page << p.page_shift) + (at & pmask);
+    }
+    p.slots[x] = slot;
+    p.positions[x] = pos;
+  }
+  if ((short_table || (rank == 0 && tid == 0 && (pages > count || tokens > p.total_new))) && p.status_word)
+    atomicOr(p.status_word, UNIQL_STATUS_NO_PAGE);
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  if (rank == 0) {
+    for (int i = tid; i <= p.batch; i += kPlanThreads) {
+      p.cu_new[i] = s_cu[i];
+      if (i < p.batch) p.lens_out[i] = s_len[i] + min(max(p.new_lens[i], 0), kMaxTokens);
+    }
+    if (tid == 0) p.free_count_out[0] = max(count - pages, 0);
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ append
+// A row (one token, one head, K or V) is DP / 8 lanes with eight channels each: one 16-byte load, four shuffles for the
+// extremes, one packed word stored.  HBM-bound by the reads: 4 bytes a channel against 0.5 written.
+__device__ __forceinline__ void kv4_load8(const void* src, int bf16, float (&x)[8]) {
+  const uint4 w = *reinterpret_cast<const uint4*>(src);
+  const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    float2 f;
+    if (bf16) f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&u[e]));
+    else f = __half22float2(*reinterpret_cast<const __half2*>(&u[e]));
+    x[2 * e] = f.x;
+    x[2 * e + 1] = f.y;
+  }
+}
+
+// Nearest code to (x - z) / s, ties to even.  The product with 1 / s is within 3 * 2^-24 of the quotient (relative); where
+// that leaves the side of a half-way point open the two sides are compared exactly: x - z spans at most 41 bits and
+// (k + 1/2) * s sixteen, both exact in fp64.
+__device__ __forceinline__ uint32_t kv4_code(float x, float z, float s, float inv) {
+  const float y = fminf(fmaxf((x - z) * inv, 0.f), 15.f);
+  const float k = floorf(y);
+  const float frac = y - k;
+  if (fabsf(frac - 0.5f) < 1e-4f) {
+    const double d = (double)x - (double)z, mid = ((double)k + 0.5) * (double)s;
+    const int ki = (int)k;
+    return (uint32_t)(d > mid || (d == mid && (ki & 1)) ? ki + 1 : ki);
+  }
+  return (uint32_t)__float2int_rn(y);
+}
+
+struct AppendParams {
+  const unsigned char* src[2];
+  int64_t token_stride[2], head_stride[2];      // elements
+  const int64_t* slots;
+  uint32_t* codes;
+  __half2* scales;
+  int* status_word;
+  int64_t tokens, num_slots;
+  int heads, d[2], bf16, page_shift;
+};
+
+constexpr int kAppendThreads = 256;
+
+template <int DP>
+__global__ void __launch_bounds__(kAppendThreads) kv4_append_kernel(const __grid_constant__ AppendParams p) {
+  constexpr int W = DP / 8;                     // lanes of a row
+  pdl_wait();
+  pdl_launch_dependents();
+  const int sub = threadIdx.x % W;
+  const int64_t rows = p.tokens * 2 * p.heads;
+  const int64_t step = (int64_t)gridDim.x * (kAppendThreads / W);
+  const int pmask = (1 << p.page_shift) - 1;
+  // all lanes of a warp stay in the loop together: the shuffles below name the whole warp
+  const int64_t first = (int64_t)blockIdx.x * (kAppendThreads / W) + threadIdx.x / W;
+  const int64_t warp_first = first - (threadIdx.x % 32) / W;
+  for (int64_t r = first, wr = warp_first; wr < rows; r += step, wr += step) {
+    const bool live = r < rows;
+    const int64_t pair = live ? r / p.heads : 0;
+    const int h = live ? (int)(r - pair * p.heads) : 0, kv = (int)(pair & 1);
+    const int64_t t = pair >> 1;
+    const int64_t slot = live ? p.slots[t] : -1;
+    const bool stored = slot >= 0 && slot < p.num_slots;
+    const bool mine = stored && sub * 8 < p.d[kv];
+    float x[8];
+    if (mine)
+      kv4_load8(p.src[kv] + 2 * (t * p.token_stride[kv] + h * p.head_stride[kv] + sub * 8), p.bf16, x);
+    float lo = 65504.f, hi = -65504.f;
+    bool nan = false;
+    if (mine) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        nan |= x[e] != x[e];
+        x[e] = fminf(fmaxf(x[e], -65504.f), 65504.f);
+        lo = fminf(lo, x[e]);
+        hi = fmaxf(hi, x[e]);
+      }
+    }
+    unsigned bad = nan;
+#pragma unroll
+    for (int o = W / 2; o; o >>= 1) {
+      lo = fminf(lo, __shfl_xor_sync(~0u, lo, o));
+      hi = fmaxf(hi, __shfl_xor_sync(~0u, hi, o));
+      bad |= __shfl_xor_sync(~0u, bad, o);
+    }
+    __half sh = __float2half_rn(__fdiv_rn(hi - lo, 15.f));
+    if (__half2float(sh) < 5.9604645e-8f) sh = __ushort_as_half(1);      // 2^-24: a scale is never zero
+    __half zh = __float2half_rn(lo);
+    const float s = __half2float(sh), z = __half2float(zh), inv = __frcp_rn(s);
+    uint32_t word = 0;
+    if (mine && !bad) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) word |= kv4_code(x[e], z, s, inv) << (4 * e);
+    }
+    if (stored) {
+      const int64_t page = slot >> p.page_shift;
+      const int64_t row = ((page * 2 + kv) * p.heads + h) * (pmask + 1) + (slot & pmask);
+      p.codes[row * W + sub] = word;
+      if (sub == 0) {
+        if (bad) sh = zh = __ushort_as_half(0x7fff);
+        p.scales[row] = __halves2half2(sh, zh);
+      }
+    } else if (live && slot != -1 && sub == 0 && p.status_word) {
+      atomicOr(p.status_word, UNIQL_STATUS_BAD_INDEX);
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ gather
+// zero + scale * code, fused so that it is rounded once, from the packed rows of a token range.  HBM-bound by the writes.
+// A CTA owns kGatherTokens packed places: one thread per place finds request, page and row (bisection over cu), then all
+// walk the places' rows, DP / 8 lanes a row, one word in and 16 bytes out each.
+constexpr int kGatherThreads = 256, kGatherTokens = 16;
+
+struct GatherParams {
+  const uint32_t* codes;
+  const __half2* scales;
+  const int32_t* table;
+  const int32_t* starts;
+  const int32_t* cu;
+  unsigned char* out[2];
+  int* status_word;
+  int64_t ld_table, num_pages, total;
+  int batch, max_blocks, heads, d[2], bf16, page_shift;
+};
+
+template <int DP>
+__global__ void __launch_bounds__(kGatherThreads) kv4_gather_kernel(const __grid_constant__ GatherParams p) {
+  constexpr int W = DP / 8, ROWS = kGatherThreads / W;
+  __shared__ int64_t s_row[kGatherTokens];      // row of head 0 of K on the token's page, or -1
+  pdl_wait();
+  pdl_launch_dependents();
+  const int64_t t0 = (int64_t)blockIdx.x * kGatherTokens;
+  const int P = 1 << p.page_shift;
+  if (threadIdx.x < kGatherTokens) {
+    const int64_t t = t0 + threadIdx.x;
+    int64_t row = -1;
+    if (t < p.total && p.batch > 0 && t >= p.cu[0] && t < p.cu[p.batch]) {
+      int lo = 0, hi = p.batch;
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (p.cu[mid] <= t) lo = mid; else hi = mid;
+      }
+      const int64_t at = t - p.cu[lo] + (p.starts ? max(p.starts[lo], 0) : 0);
+      const int64_t block = at >> p.page_shift;
+      int page = -1;
+      if (block < p.max_blocks) page = p.table[(size_t)lo * p.ld_table + block];
+      if (page >= 0 && page < p.num_pages) row = (int64_t)page * 2 * p.heads * P + (at & (P - 1));
+      else if (p.status_word) atomicOr(p.status_word, UNIQL_STATUS_BAD_INDEX);
+    }
+    s_row[threadIdx.x] = row;
+  }
+  __syncthreads();
+  const int n = (int)(p.total - t0 < kGatherTokens ? p.total - t0 : kGatherTokens);
+  const int sub = threadIdx.x % W;
+  const int per_kv = n * p.heads;
+  for (int r = threadIdx.x / W; r < 2 * per_kv; r += ROWS) {
+    const int kv = r >= per_kv, rr = r - kv * per_kv;
+    const int i = rr / p.heads, h = rr - i * p.heads;
+    if (sub * 8 >= p.d[kv]) continue;
+    const int64_t row0 = s_row[i];
+    uint4 o = make_uint4(0, 0, 0, 0);
+    if (row0 >= 0) {
+      const int64_t row = row0 + ((int64_t)kv * p.heads + h) * P;
+      const uint32_t w = p.codes[row * W + sub];
+      const __half2 sz = p.scales[row];
+      uint32_t c[4];
+      kv4_codes(w, c);                          // (d, d + 4) pairs
+      if (!p.bf16) {
+        const __half2 s2 = __low2half2(sz), z2 = __high2half2(sz);
+        uint32_t v[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const __half2 f = __hfma2(*reinterpret_cast<const __half2*>(&c[e]), s2, z2);
+          v[e] = *reinterpret_cast<const uint32_t*>(&f);
+        }
+        o = make_uint4(__byte_perm(v[0], v[1], 0x5410), __byte_perm(v[2], v[3], 0x5410), __byte_perm(v[0], v[1], 0x7632),
+                       __byte_perm(v[2], v[3], 0x7632));
+      } else {
+        const float s = __low2float(sz), z = __high2float(sz);
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&c[e]));
+          v[e] = fmaf(f.x, s, z);
+          v[e + 4] = fmaf(f.y, s, z);
+        }
+        uint32_t u[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const __nv_bfloat162 b = __floats2bfloat162_rn(v[2 * e], v[2 * e + 1]);
+          u[e] = *reinterpret_cast<const uint32_t*>(&b);
+        }
+        o = make_uint4(u[0], u[1], u[2], u[3]);
+      }
+    }
+    *reinterpret_cast<uint4*>(p.out[kv] + 2 * (((t0 + i) * p.heads + h) * (int64_t)p.d[kv] + sub * 8)) = o;
+  }
+}
+
+}  // namespace uniql
+
+// ------------------------------------------------------------------------------------------------ C ABI
+extern "C" int uniql_kv_page_plan(const int32_t* lens, const int32_t* new_lens, int64_t batch, int32_t* block_table,
+                                  int64_t ld_table, int64_t max_blocks, const int32_t* free_pages, int64_t free_cap,
+                                  const int32_t* free_count, int64_t page_size, int64_t total_new, int64_t* slots,
+                                  int64_t* positions, int32_t* cu_new, int32_t* lens_out, int32_t* free_count_out,
+                                  int* status_word, void* stream) {
+  using namespace uniql;
+  if (batch < 0 || total_new < 0 || max_blocks < 0 || free_cap < 0 || ld_table < max_blocks) return UNIQL_EINVAL;
+  const int shift = page_shift_of(page_size);
+  if (shift < 0 || batch > UNIQL_KV_MAX_BATCH || total_new > kMaxTokens || max_blocks > kMaxTokens || free_cap > kMaxTokens)
+    return UNIQL_ESHAPE;
+  if (!cu_new || !free_count || !free_count_out) return UNIQL_EINVAL;
+  if (batch > 0 && (!lens || !new_lens || !lens_out || (max_blocks > 0 && !block_table))) return UNIQL_EINVAL;
+  if ((total_new > 0 && (!slots || !positions)) || (free_cap > 0 && !free_pages)) return UNIQL_EINVAL;
+  PlanParams p;
+  p.lens = lens; p.new_lens = new_lens; p.table = block_table; p.ld_table = ld_table;
+  p.free_pages = free_pages; p.free_count = free_count; p.slots = slots; p.positions = positions;
+  p.cu_new = cu_new; p.lens_out = lens_out; p.free_count_out = free_count_out; p.status_word = status_word;
+  p.total_new = total_new; p.batch = (int)batch; p.max_blocks = (int)max_blocks; p.free_cap = (int)free_cap; p.page_shift = shift;
+  const size_t smem = (3 * (size_t)batch + 2) * sizeof(int);
+  if (smem > 48 * 1024) {
+    static thread_local bool attr_set[64] = {};
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (dev < 0 || dev >= 64 || !attr_set[dev]) {
+      UNIQL_CUDA_TRY(cudaFuncSetAttribute(kv_page_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                          (3 * UNIQL_KV_MAX_BATCH + 2) * (int)sizeof(int)));
+      if (dev >= 0 && dev < 64) attr_set[dev] = true;
+    }
+  }
+  // one thread per token up to the eight CTAs of a portable cluster
+  int ctas = (int)((total_new + kPlanThreads - 1) / kPlanThreads);
+  ctas = ctas < 1 ? 1 : ctas > 8 ? 8 : ctas;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)ctas);
+  cfg.blockDim = dim3(kPlanThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = (cudaStream_t)stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = (unsigned)ctas;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  UNIQL_CUDA_TRY(cudaLaunchKernelEx(&cfg, kv_page_plan_kernel, p));
+  return UNIQL_OK;
+}
+
+extern "C" int uniql_kv4_append(const void* k, int64_t k_token_stride, int64_t k_head_stride, const void* v,
+                                int64_t v_token_stride, int64_t v_head_stride, int dtype, int64_t tokens, int64_t kv_heads,
+                                int64_t dk, int64_t dv, const int64_t* slots, void* codes, void* scales, int64_t num_pages,
+                                int64_t page_size, int64_t dp, int* status_word, void* stream) {
+  using namespace uniql;
+  if (tokens < 0 || kv_heads <= 0 || num_pages < 0 || dk <= 0 || dv <= 0) return UNIQL_EINVAL;
+  if (dtype != UNIQL_F16 && dtype != UNIQL_BF16) return UNIQL_EDTYPE;
+  const int st = kv4_check(num_pages, page_size, dp, kv_heads, dk, dv);
+  if (st != UNIQL_OK) return st;
+  if (tokens > kMaxTokens) return UNIQL_ESHAPE;
+  if ((k_token_stride | k_head_stride | v_token_stride | v_head_stride) & 7) return UNIQL_EINVAL;
+  if (tokens == 0) return UNIQL_OK;
+  if (!k || !v || !slots || !aligned16(k) || !aligned16(v)) return UNIQL_EINVAL;
+  if (num_pages > 0 && (!codes || !scales || !aligned16(codes) || !aligned16(scales))) return UNIQL_EINVAL;
+  AppendParams p;
+  p.src[0] = (const unsigned char*)k; p.src[1] = (const unsigned char*)v;
+  p.token_stride[0] = k_token_stride; p.token_stride[1] = v_token_stride;
+  p.head_stride[0] = k_head_stride; p.head_stride[1] = v_head_stride;
+  p.slots = slots; p.codes = (uint32_t*)codes; p.scales = (__half2*)scales; p.status_word = status_word;
+  p.tokens = tokens; p.num_slots = num_pages * page_size; p.heads = (int)kv_heads; p.d[0] = (int)dk; p.d[1] = (int)dv;
+  p.bf16 = dtype == UNIQL_BF16; p.page_shift = page_shift_of(page_size);
+  const int64_t rows = tokens * 2 * kv_heads, per = kAppendThreads / (dp / 8);
+  int64_t ctas = (rows + per - 1) / per;
+  const int64_t cap = 8 * (int64_t)device_info().sm_count;
+  if (ctas > cap) ctas = cap;
+  return dp == 128 ? launch_pdl(kv4_append_kernel<128>, (unsigned)ctas, kAppendThreads, 0, (cudaStream_t)stream, p)
+                   : launch_pdl(kv4_append_kernel<64>, (unsigned)ctas, kAppendThreads, 0, (cudaStream_t)stream, p);
+}
+
+extern "C" int uniql_kv4_gather(const void* codes, const void* scales, int64_t num_pages, int64_t page_size, int64_t dp,
+                                int64_t kv_heads, const int32_t* block_table, int64_t ld_table, int64_t max_blocks,
+                                int64_t batch, const int32_t* starts, const int32_t* cu, int64_t total, int64_t dk, int64_t dv,
+                                int dtype, void* k_out, void* v_out, int* status_word, void* stream) {
+  using namespace uniql;
+  if (total < 0 || batch < 0 || kv_heads <= 0 || num_pages < 0 || dk <= 0 || dv <= 0 || max_blocks < 0 || ld_table < max_blocks)
+    return UNIQL_EINVAL;
+  if (dtype != UNIQL_F16 && dtype != UNIQL_BF16) return UNIQL_EDTYPE;
+  const int st = kv4_check(num_pages, page_size, dp, kv_heads, dk, dv);
+  if (st != UNIQL_OK) return st;
+  if (total > kMaxTokens || batch > kMaxTokens || max_blocks > kMaxTokens) return UNIQL_ESHAPE;
+  if (total == 0) return UNIQL_OK;
+  if (!k_out || !v_out || !aligned16(k_out) || !aligned16(v_out)) return UNIQL_EINVAL;
+  if (batch > 0 && (!cu || (max_blocks > 0 && !block_table))) return UNIQL_EINVAL;
+  if (num_pages > 0 && (!codes || !scales || !aligned16(codes) || !aligned16(scales))) return UNIQL_EINVAL;
+  GatherParams p;
+  p.codes = (const uint32_t*)codes; p.scales = (const __half2*)scales; p.table = block_table; p.starts = starts; p.cu = cu;
+  p.out[0] = (unsigned char*)k_out; p.out[1] = (unsigned char*)v_out; p.status_word = status_word;
+  p.ld_table = ld_table; p.num_pages = num_pages; p.total = total; p.batch = (int)batch; p.max_blocks = (int)max_blocks;
+  p.heads = (int)kv_heads; p.d[0] = (int)dk; p.d[1] = (int)dv; p.bf16 = dtype == UNIQL_BF16;
+  p.page_shift = page_shift_of(page_size);
+  const unsigned ctas = (unsigned)((total + kGatherTokens - 1) / kGatherTokens);
+  return dp == 128 ? launch_pdl(kv4_gather_kernel<128>, ctas, kGatherThreads, 0, (cudaStream_t)stream, p)
+                   : launch_pdl(kv4_gather_kernel<64>, ctas, kGatherThreads, 0, (cudaStream_t)stream, p);
+}

@@ -1,0 +1,500 @@
+// Attention of packed prompts on the tcgen05 tensor cores.  Rules: include/uniql_b200.h.
+//
+// Mathematics: one pass over the keys with a running bound m of the row's scores (in units of log2): with S = Q K^T and f =
+// softmax_scale log2(e), P = 2^(f S - m), l = sum P, O = sum P V, and O / l at the end.  m is raised, and l and O rescaled, only
+// when a score exceeds it by more than 8 (P stays below 2^8, far from fp16's limit), which after the first tiles is rare.
+//
+// A CTA owns two units, a unit being 128 query rows of one query head; units of a request and kv head are numbered row block
+// first, head of the group second, so that the two share their keys and values.  Per 128 keys and unit:
+//   S (tensor memory, 128 fp32 columns) = Q (shared memory) K^T (shared memory)
+//   P (16-bit, on the first 64 of S's columns) -- four softmax warps, one row a thread
+//   O (tensor memory) += P V, P read from tensor memory, V as an MN-major operand straight from its row-major tile
+// While the softmax of one unit runs the tensor cores work on the other:  warps 0-3 and 4-7 softmax of unit 0 and 1 (they also
+// rescale and store O), warp 8 issues the MMAs, warp 9 the TMA loads (no multicast).
+//
+// Masked places: keys behind a request's last are set to -inf in S, and the rows of V behind it in its last tile, which belong
+// to another request, are cleared in shared memory before they are multiplied by the zeros of P.
+// Bound: tensor pipe and the exponentials, 4 * 128 * 128 * d flops against 128 * 128 exponentials (16 a clock and SM) per tile.
+// Every wait is bounded; a wait that gives up sets UNIQL_STATUS_WAIT_TIMEOUT and the kernel drains.
+#include "common.cuh"
+#include "kv_cache.cuh"
+#include "tc.cuh"
+
+namespace uniql {
+
+namespace pa {
+constexpr int kMmaWarp = 8, kLoadWarp = 9;   // warps 0-7: softmax
+constexpr int kThreads = 320;
+constexpr int kRows = 128, kKeys = 128;
+constexpr int kTmemCols = 512;                  // S0, S1, O0, O1: 128 columns each
+template <int DP>
+struct Cfg {
+  static constexpr int kTileBytes = 128 * DP * 2;
+  static constexpr int kStages = 5;
+  static constexpr int kOffKv = 2 * kTileBytes;
+  static constexpr int kOffBar = kOffKv + kStages * kTileBytes;
+  static constexpr int kBars = 1 + 2 * kStages + 6 + 1;
+  static constexpr int kSmem = kOffBar + kBars * 8 + 16 + 1024;
+  static_assert(kSmem <= 227 * 1024, "shared memory");
+};
+}  // namespace pa
+
+struct PaParams {
+  const int32_t* cu_q;
+  const int32_t* cu_k;
+  unsigned char* out;
+  int* status_word;
+  int batch, total_q, total_k, heads, kv_heads, group, dk, dv, causal;
+  float scale_log2;
+};
+
+__device__ __forceinline__ void pa_tma_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+      ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar)
+      : "memory");
+}
+__device__ __forceinline__ void pa_ld32(uint32_t taddr, float* r) {
+  uint32_t* u = reinterpret_cast<uint32_t*>(r);
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7]),
+        "=r"(u[8]), "=r"(u[9]), "=r"(u[10]), "=r"(u[11]), "=r"(u[12]), "=r"(u[13]), "=r"(u[14]), "=r"(u[15]),
+        "=r"(u[16]), "=r"(u[17]), "=r"(u[18]), "=r"(u[19]), "=r"(u[20]), "=r"(u[21]), "=r"(u[22]), "=r"(u[23]),
+        "=r"(u[24]), "=r"(u[25]), "=r"(u[26]), "=r"(u[27]), "=r"(u[28]), "=r"(u[29]), "=r"(u[30]), "=r"(u[31])
+      : "r"(taddr));
+}
+__device__ __forceinline__ void pa_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void pa_st32(uint32_t taddr, const uint32_t* u) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};"
+      ::"r"(taddr), "r"(u[0]), "r"(u[1]), "r"(u[2]), "r"(u[3]), "r"(u[4]), "r"(u[5]), "r"(u[6]), "r"(u[7]), "r"(u[8]),
+        "r"(u[9]), "r"(u[10]), "r"(u[11]), "r"(u[12]), "r"(u[13]), "r"(u[14]), "r"(u[15]), "r"(u[16]), "r"(u[17]),
+        "r"(u[18]), "r"(u[19]), "r"(u[20]), "r"(u[21]), "r"(u[22]), "r"(u[23]), "r"(u[24]), "r"(u[25]), "r"(u[26]),
+        "r"(u[27]), "r"(u[28]), "r"(u[29]), "r"(u[30]), "r"(u[31])
+      : "memory");
+}
+__device__ __forceinline__ void pa_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ float pa_exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ void pa_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+      ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc)
+      : "memory");
+}
+__device__ __forceinline__ void pa_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+      ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(acc)
+      : "memory");
+}
+template <bool BF16>
+__device__ __forceinline__ uint32_t pa_pack(float a, float b) {
+  if (BF16) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+template <int DP, bool BF16>
+__global__ void __launch_bounds__(pa::kThreads, 1)
+prompt_attention_kernel(const __grid_constant__ PaParams p, const __grid_constant__ CUtensorMap qmap,
+                        const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
+  using namespace pa;
+  using C = Cfg<DP>;
+  constexpr int SUB = 128 * 128;                // bytes of a sub-tile of 128 rows x 64 channels
+  extern __shared__ uint8_t smem_unaligned[];
+  __shared__ int s_work[4];                     // request, pair, valid
+  __shared__ long long s_wide[kThreads / 32];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_unaligned) + 1023) & ~(uintptr_t)1023);
+  const uint32_t sbase = tc_smem_addr(smem);
+  const uint32_t bar_q = sbase + C::kOffBar, bar_full = bar_q + 8, bar_empty = bar_full + 8 * C::kStages;
+  const uint32_t bar_s = bar_empty + 8 * C::kStages, bar_p = bar_s + 16, bar_o = bar_p + 16, bar_clean = bar_o + 16;
+  volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(smem + C::kOffBar + C::kBars * 8);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+
+  if (warp == kMmaWarp) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tc_smem_addr((const void*)tmem_slot)),
+                 "r"(kTmemCols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  if (warp == kLoadWarp && tc_elect()) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&qmap) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&kmap) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&vmap) : "memory");
+    tc_mbar_init(bar_q, 1);
+    for (int s = 0; s < C::kStages; ++s) {
+      tc_mbar_init(bar_full + 8 * s, 1);
+      tc_mbar_init(bar_empty + 8 * s, 1);
+    }
+    for (int t = 0; t < 2; ++t) {
+      tc_mbar_init(bar_s + 8 * t, 1);
+      tc_mbar_init(bar_p + 8 * t, 4);
+      tc_mbar_init(bar_o + 8 * t, 1);
+    }
+    tc_mbar_init(bar_clean, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
+  pdl_wait();
+  pdl_launch_dependents();
+
+  // ---- which request and which two units: pairs of units of all requests in order, kv head fastest, the last row blocks (the
+  // ones with the most keys) of a request first
+  const int pair = blockIdx.x / p.kv_heads, kvh = blockIdx.x - pair * p.kv_heads;
+  auto begin_q = [&](int b) { return min(max(p.cu_q[b], 0), p.total_q); };
+  auto begin_k = [&](int b) { return min(max(p.cu_k[b], 0), p.total_k); };
+  auto pairs_of = [&](int b) {
+    const int n = max(begin_q(b + 1) - begin_q(b), 0);
+    return (long long)(((n + kRows - 1) / kRows) * (long long)p.group + 1) / 2;
+  };
+  {
+    const int per = (p.batch + kThreads - 1) / kThreads;
+    const int b0 = min(tid * per, p.batch), b1 = min(b0 + per, p.batch);
+    long long mine = 0;
+    for (int b = b0; b < b1; ++b) mine += pairs_of(b);
+    long long incl = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long v = __shfl_up_sync(~0u, incl, o);
+      if (lane >= o) incl += v;
+    }
+    if (lane == 31) s_wide[warp] = incl;
+    if (tid == 0) s_work[0] = -1;
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    long long before = incl - mine;
+    for (int w = 0; w < warp; ++w) before += s_wide[w];
+    if (before <= pair && pair < before + mine) {
+      for (int b = b0; b < b1; ++b) {
+        const long long n = pairs_of(b);
+        if (pair < before + n) {
+          s_work[0] = b;
+          s_work[1] = (int)(n - 1 - (pair - before));
+          break;
+        }
+        before += n;
+      }
+    }
+    __syncthreads();
+  }
+  // rows that no request owns
+  {
+    const int lo = p.batch > 0 ? begin_q(0) : p.total_q, hi = p.batch > 0 ? begin_q(p.batch) : p.total_q;
+    const size_t rowb = (size_t)p.heads * p.dv * 2;
+    for (int r = blockIdx.x; r < lo + p.total_q - hi; r += gridDim.x) {
+      uint4* dst = reinterpret_cast<uint4*>(p.out + (size_t)(r < lo ? r : r - lo + hi) * rowb);
+      for (int i = tid; i < (int)(rowb / 16); i += kThreads) dst[i] = make_uint4(0, 0, 0, 0);
+    }
+  }
+  const uint32_t tmem = *tmem_slot;
+  const int req = s_work[0];
+  bool timed_out = false;
+  if (req >= 0) {
+    const int q0 = begin_q(req), nq = begin_q(req + 1) - q0;
+    const int k0 = begin_k(req), nk = max(begin_k(req + 1) - k0, 0);
+    const int units = ((nq + kRows - 1) / kRows) * p.group, u0 = 2 * s_work[1];
+    const int shift = p.causal ? nk - nq : 0;   // query i sees the keys below i + 1 + shift
+    int row[2], head[2], n[2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const int u = u0 + t;
+      row[t] = u / p.group * kRows;
+      head[t] = kvh * p.group + u % p.group;
+      int seen = nk;
+      if (p.causal) seen = min(nk, max(min(row[t] + kRows, nq) + shift, 0));
+      n[t] = u < units ? (seen + kKeys - 1) / kKeys : 0;
+    }
+    const int nmax = max(n[0], n[1]);
+    const bool dirty = nmax * kKeys > nk;       // the last tile of V reaches behind the request
+
+    if (warp == kLoadWarp) {
+      // ------------------------------------------------------------------ loads: Q, then K 0, V 0, K 1, V 1, ...
+      if (tc_elect() && nmax > 0) {
+        tc_mbar_expect_tx(bar_q, ((n[0] > 0) + (n[1] > 0)) * C::kTileBytes);
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+          if (n[t] > 0)
+            for (int i = 0; i < DP / 64; ++i)
+              pa_tma_3d(sbase + t * C::kTileBytes + i * SUB, &qmap, 64 * i, head[t], q0 + row[t], bar_q);
+        for (int it = 0; it < 2 * nmax; ++it) {
+          const int s = it % C::kStages;
+          if (!timed_out && !tc_mbar_wait(bar_empty + 8 * s, ((it / C::kStages) & 1) ^ 1)) timed_out = true;
+          if (timed_out) break;
+          tc_mbar_expect_tx(bar_full + 8 * s, C::kTileBytes);
+          for (int i = 0; i < DP / 64; ++i)
+            pa_tma_3d(sbase + C::kOffKv + s * C::kTileBytes + i * SUB, (it & 1) ? &vmap : &kmap, 64 * i, kvh,
+                      k0 + (it >> 1) * kKeys, bar_full + 8 * s);
+        }
+      }
+      timed_out = __shfl_sync(~0u, (int)(__any_sync(~0u, timed_out)), 0);
+      if (dirty && nmax > 0 && !timed_out) {
+        const int it = 2 * nmax - 1, s = it % C::kStages;
+        if (!tc_mbar_wait(bar_full + 8 * s, (it / C::kStages) & 1)) timed_out = true;
+        if (!timed_out) {
+          const int r0 = nk - (nmax - 1) * kKeys;               // first row of another request
+          const uint32_t tile = sbase + C::kOffKv + s * C::kTileBytes;
+          for (int i = lane; i < (kKeys - r0) * 8 * (DP / 64); i += 32) {
+            const int sub = i / ((kKeys - r0) * 8), x = i - sub * ((kKeys - r0) * 8);
+            asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(tile + sub * SUB + r0 * 128 + x * 16), "r"(0) : "memory");
+          }
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        }
+        __syncwarp();
+        if (lane == 0) tc_mbar_arrive(bar_clean);
+      }
+    } else if (warp == kMmaWarp) {
+      // ------------------------------------------------------------------ MMAs
+      if (tc_elect() && nmax > 0) {
+        constexpr uint32_t kType = BF16 ? (1u << 7) | (1u << 10) : 0u;
+        const uint32_t idesc_s = (1u << 4) | kType | ((uint32_t)(kKeys >> 3) << 17) | (8u << 24);
+        const int nv = (p.dv + 15) / 16 * 16, ks = (p.dk + 15) / 16;
+        const uint32_t idesc_o = (1u << 4) | kType | (1u << 16) | ((uint32_t)(nv >> 3) << 17) | (8u << 24);
+        auto wait = [&](uint32_t bar, uint32_t parity) {
+          if (!timed_out && !tc_mbar_wait(bar, parity)) timed_out = true;
+          tc_fence_after();
+        };
+        auto scores = [&](int t, int it) {      // S_t = Q_t K^T with the tile of item it
+          const uint32_t kt = sbase + C::kOffKv + (it % C::kStages) * C::kTileBytes, qt = sbase + t * C::kTileBytes;
+          if (!timed_out)
+            for (int s = 0; s < ks; ++s)
+              pa_mma_ss(tmem + t * 128, tc_smem_desc(qt + (s >> 2) * SUB) + 2 * (s & 3),
+                        tc_smem_desc(kt + (s >> 2) * SUB) + 2 * (s & 3), idesc_s, s > 0);
+          tc_commit(bar_s + 8 * t);
+        };
+        auto values = [&](int t, int it, uint32_t acc) {        // O_t (+)= P_t V
+          const uint32_t vt = sbase + C::kOffKv + (it % C::kStages) * C::kTileBytes;
+          // MN-major, 128-byte swizzle: 64-channel sub-tiles SUB bytes apart, groups of 8 keys 1024 bytes apart
+          const uint64_t vd = (uint64_t)((vt & 0x3FFFFu) >> 4) | ((uint64_t)(SUB >> 4) << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
+          if (!timed_out)
+#pragma unroll
+            for (int s = 0; s < 8; ++s)
+              pa_mma_ts(tmem + 256 + t * 128, tmem + t * 128 + 8 * s, vd + 128 * s, idesc_o, s > 0 ? 1u : acc);
+          tc_commit(bar_o + 8 * t);
+        };
+        wait(bar_q, 0);
+        wait(bar_full, 0);
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+          if (n[t] > 0) scores(t, 0);
+        tc_commit(bar_empty);
+        for (int j = 0; j < nmax; ++j) {
+          const int iv = 2 * j + 1, ik = 2 * j + 2, sv = iv % C::kStages, sk = ik % C::kStages;
+          wait(bar_full + 8 * sv, (iv / C::kStages) & 1);
+          if (j + 1 < nmax) wait(bar_full + 8 * sk, (ik / C::kStages) & 1);
+          else if (dirty) wait(bar_clean, 0);
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            if (j < n[t]) {
+              wait(bar_p + 8 * t, j & 1);
+              values(t, iv, j > 0);
+            }
+            if (t == 1) tc_commit(bar_empty + 8 * sv);
+            if (j + 1 < n[t]) scores(t, ik);
+          }
+          if (j + 1 < nmax) tc_commit(bar_empty + 8 * sk);
+        }
+      }
+    } else {
+      // ------------------------------------------------------------------ softmax, one query row a thread
+      const int t = warp >> 2;
+      const int nt = t ? n[1] : n[0], row0 = t ? row[1] : row[0], i = row0 + (warp & 3) * 32 + lane;
+      const int limit = p.causal ? min(nk, max(i + 1 + shift, 0)) : nk;
+      const int full = p.causal ? min(nk, max(row0 + 1 + shift, 0)) : nk;       // keys that every row of the unit sees
+      const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+      const uint32_t ts = tmem + t * 128 + lanes, to = tmem + 256 + t * 128 + lanes;
+      const float f = p.scale_log2;
+      float m = -INFINITY, l = 0.f;
+      for (int j = 0; j < nt; ++j) {
+        if (!timed_out && !tc_mbar_wait(bar_s + 8 * t, j & 1)) timed_out = true;
+        tc_fence_after();
+        float s[128];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) pa_ld32(ts + 32 * c, s + 32 * c);
+        pa_wait_ld();
+        if ((j + 1) * kKeys > full) {
+          const int left = limit - j * kKeys;
+#pragma unroll
+          for (int c = 0; c < 128; ++c) s[c] = c < left ? s[c] : -INFINITY;
+        }
+        float top = fmaxf(s[0], s[1]);
+#pragma unroll
+        for (int c = 2; c < 128; ++c) top = fmaxf(top, s[c]);
+        top = i < nq ? top * f : -INFINITY;     // rows of another request have no say in when m is raised
+        if (__any_sync(~0u, top > m + 8.f)) {
+          const float mn = fmaxf(m, top);
+          const float k = mn == -INFINITY ? 1.f : pa_exp2(m - mn);
+          m = mn;
+          l *= k;
+          if (j > 0) {
+            if (!timed_out && !tc_mbar_wait(bar_o + 8 * t, (j - 1) & 1)) timed_out = true;
+            tc_fence_after();
+#pragma unroll 1
+            for (int c = 0; c < DP; c += 32) {
+              float o[32];
+              pa_ld32(to + c, o);
+              pa_wait_ld();
+#pragma unroll
+              for (int e = 0; e < 32; ++e) o[e] *= k;
+              pa_st32(to + c, reinterpret_cast<const uint32_t*>(o));
+            }
+          }
+        }
+        const float base = m == -INFINITY ? 0.f : m;
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < 128; ++c) {
+          s[c] = pa_exp2(fmaf(s[c], f, -base));
+          sum[c & 3] += s[c];
+        }
+        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          uint32_t w[32];
+#pragma unroll
+          for (int c = 0; c < 32; ++c) w[c] = pa_pack<BF16>(s[64 * h + 2 * c], s[64 * h + 2 * c + 1]);
+          pa_st32(ts + 32 * h, w);
+        }
+        pa_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) tc_mbar_arrive(bar_p + 8 * t);
+      }
+      // ---- O / l
+      if (u0 + t < units) {
+        if (nt > 0) {
+          if (!timed_out && !tc_mbar_wait(bar_o + 8 * t, (nt - 1) & 1)) timed_out = true;
+          tc_fence_after();
+        }
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        unsigned char* dst = p.out + ((size_t)(q0 + i) * p.heads + (t ? head[1] : head[0])) * p.dv * 2;
+#pragma unroll 1
+        for (int c = 0; c < DP; c += 32) {
+          float o[32];
+          if (nt > 0) {
+            pa_ld32(to + c, o);
+            pa_wait_ld();
+          } else {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = 0.f;
+          }
+          if (i < nq) {
+#pragma unroll
+            for (int v = 0; v < 4; ++v)
+              if (c + 8 * v < p.dv) {
+                uint32_t w[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  const float a = l == 0.f ? 0.f : o[8 * v + 2 * e] * inv, b = l == 0.f ? 0.f : o[8 * v + 2 * e + 1] * inv;
+                  w[e] = pa_pack<BF16>(a, b);
+                }
+                *reinterpret_cast<uint4*>(dst + (c + 8 * v) * 2) = make_uint4(w[0], w[1], w[2], w[3]);
+              }
+          }
+        }
+      }
+    }
+  }
+  if (timed_out && p.status_word) atomicOr(p.status_word, UNIQL_STATUS_WAIT_TIMEOUT);
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kMmaWarp) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
+  }
+}
+
+// rows [tokens, heads, d] as a 3-D tensor, boxes of 64 channels x 1 head x 128 tokens; what lies outside reads as zero
+static int pa_map(CUtensorMap* map, const void* x, int64_t tokens, int64_t heads, int64_t d, int64_t token_stride,
+                  int64_t head_stride, bool bf16) {
+  EncodeTiledFn enc = encode_tiled_fn();
+  if (!enc) return cuda_fail(cudaErrorNotSupported);
+  cuuint64_t dims[3] = {(cuuint64_t)d, (cuuint64_t)heads, (cuuint64_t)tokens};
+  cuuint64_t strides[2] = {(cuuint64_t)head_stride * 2, (cuuint64_t)token_stride * 2};
+  cuuint32_t box[3] = {64, 1, 128}, estr[3] = {1, 1, 1};
+  if (enc(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void*>(x), dims, strides,
+          box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+    return cuda_fail(cudaErrorInvalidValue);
+  return UNIQL_OK;
+}
+
+template <int DP, bool BF16>
+static int pa_launch(const PaParams& p, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, unsigned ctas, cudaStream_t stream) {
+  static thread_local bool attr_set[64] = {};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= 64 || !attr_set[dev]) {
+    UNIQL_CUDA_TRY(cudaFuncSetAttribute(prompt_attention_kernel<DP, BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, pa::Cfg<DP>::kSmem));
+    if (dev >= 0 && dev < 64) attr_set[dev] = true;
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(ctas);
+  cfg.blockDim = dim3(pa::kThreads);
+  cfg.dynamicSmemBytes = pa::Cfg<DP>::kSmem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  UNIQL_CUDA_TRY(cudaLaunchKernelEx(&cfg, prompt_attention_kernel<DP, BF16>, p, q, k, v));
+  return UNIQL_OK;
+}
+
+}  // namespace uniql
+
+extern "C" int uniql_prompt_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k,
+                                      int64_t k_token_stride, int64_t k_head_stride, const void* v, int64_t v_token_stride,
+                                      int64_t v_head_stride, const int32_t* cu_q, const int32_t* cu_k, int64_t batch,
+                                      int64_t total_q, int64_t total_k, int64_t heads, int64_t kv_heads, int64_t dk, int64_t dv,
+                                      float softmax_scale, int causal, int dtype, void* out, int* status_word, void* stream) {
+  using namespace uniql;
+  if (batch < 0 || total_q < 0 || total_k < 0 || heads <= 0 || kv_heads <= 0 || dk <= 0 || dv <= 0) return UNIQL_EINVAL;
+  if (dtype != UNIQL_F16 && dtype != UNIQL_BF16) return UNIQL_EDTYPE;
+  if (dk % 8 || dv % 8 || dk > 128 || dv > 128 || heads % kv_heads || heads > 16384 || kv_heads > 1024) return UNIQL_ESHAPE;
+  if (batch > UNIQL_KV_MAX_BATCH || total_q > kMaxTokens || total_k > kMaxTokens) return UNIQL_ESHAPE;
+  if (!(softmax_scale > 0.f) || softmax_scale > 1e30f) return UNIQL_EINVAL;
+  if ((q_token_stride | q_head_stride | k_token_stride | k_head_stride | v_token_stride | v_head_stride) & 7) return UNIQL_EINVAL;
+  if (q_token_stride < 0 || q_head_stride < 0 || k_token_stride < 0 || k_head_stride < 0 || v_token_stride < 0 || v_head_stride < 0)
+    return UNIQL_EINVAL;
+  if (total_q == 0) return UNIQL_OK;
+  if (!q || !out || !aligned16(q) || !aligned16(out)) return UNIQL_EINVAL;
+  if (total_k > 0 && (!k || !v || !aligned16(k) || !aligned16(v))) return UNIQL_EINVAL;
+  if (batch > 0 && (!cu_q || !cu_k)) return UNIQL_EINVAL;
+  PaParams p;
+  p.cu_q = cu_q; p.cu_k = cu_k; p.out = (unsigned char*)out; p.status_word = status_word;
+  p.batch = (int)batch; p.total_q = (int)total_q; p.total_k = (int)total_k; p.heads = (int)heads; p.kv_heads = (int)kv_heads;
+  p.group = (int)(heads / kv_heads); p.dk = (int)dk; p.dv = (int)dv; p.causal = causal != 0;
+  p.scale_log2 = softmax_scale * 1.44269504088896340736f;
+  const bool bf16 = dtype == UNIQL_BF16;
+  CUtensorMap qm, km, vm;
+  int st = pa_map(&qm, q, total_q, heads, dk, q_token_stride, q_head_stride, bf16);
+  // without keys no tile of K or V is ever loaded: the maps only have to be valid
+  if (st == UNIQL_OK) st = total_k ? pa_map(&km, k, total_k, kv_heads, dk, k_token_stride, k_head_stride, bf16) : (km = qm, UNIQL_OK);
+  if (st == UNIQL_OK) st = total_k ? pa_map(&vm, v, total_k, kv_heads, dv, v_token_stride, v_head_stride, bf16) : (vm = qm, UNIQL_OK);
+  if (st != UNIQL_OK) return st;
+  // at most this many pairs of units: every request rounds its row blocks and its pairs up
+  const int64_t blocks = total_q / pa::kRows + (batch < total_q ? batch : total_q);
+  const int64_t pairs = (blocks * p.group + 1) / 2 + batch;
+  const int64_t ctas = pairs > 0 ? pairs * kv_heads : 1;     // at least one: rows that nobody owns are cleared
+  if (ctas > ((int64_t)1 << 31) - 1) return UNIQL_ESHAPE;
+  cudaStream_t s = (cudaStream_t)stream;
+  if (dk > 64 || dv > 64)
+    return bf16 ? pa_launch<128, true>(p, qm, km, vm, (unsigned)ctas, s) : pa_launch<128, false>(p, qm, km, vm, (unsigned)ctas, s);
+  return bf16 ? pa_launch<64, true>(p, qm, km, vm, (unsigned)ctas, s) : pa_launch<64, false>(p, qm, km, vm, (unsigned)ctas, s);
+}

@@ -48,6 +48,17 @@ at::Tensor scratch_for(int device, cudaStream_t stream, size_t need) {
   return slot;
 }
 
+// Scratch of a call that a graph may replay at any time, on any stream, beside eager calls and other graphs: memory of the graph's
+// own while the stream is captured (its counter region cleared by a captured memset), the stream's scratch otherwise.
+at::Tensor own_scratch(int device, cudaStream_t stream, size_t need) {
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  if (cudaStreamIsCapturing(stream, &status) != cudaSuccess) (void)cudaGetLastError();
+  if (status == cudaStreamCaptureStatusNone) return scratch_for(device, stream, need);
+  at::Tensor t = at::empty({(int64_t)need}, at::TensorOptions().dtype(at::kByte).device(at::Device(at::kCUDA, (c10::DeviceIndex)device)));
+  TORCH_CHECK(cudaMemsetAsync(t.data_ptr(), 0, UNIQL_SCRATCH_COUNTER_BYTES, stream) == cudaSuccess, "clearing captured scratch failed");
+  return t;
+}
+
 // Scratch requirement of the last few shapes (a decode loop repeats a handful of them).
 struct NeedKey {
   int64_t v[8];
@@ -260,6 +271,186 @@ at::Tensor hadamard(const at::Tensor& x, double scale) {
   return y;
 }
 
+// ---- attention around the paged 4-bit KV cache (include/uniql_b200.h): types, devices and shapes are checked here, sizes and
+// alignment by the C ABI.
+int kv_dtype(const at::Tensor& t, const char* name) {
+  if (t.scalar_type() == at::kHalf) return UNIQL_F16;
+  TORCH_CHECK(t.scalar_type() == at::kBFloat16, name, " must be float16 or bfloat16");
+  return UNIQL_BF16;
+}
+
+void check_ints(const at::Tensor& t, const at::Tensor& like, int64_t dim, const char* name) {
+  TORCH_CHECK(t.is_cuda() && t.scalar_type() == at::kInt && t.dim() == dim, name, " must be a ", dim, "-D int32 CUDA tensor");
+  TORCH_CHECK(t.device() == like.device(), name, " is on another device");
+  TORCH_CHECK(t.size(-1) <= 1 || t.stride(-1) == 1, name, " must have unit stride in its last dimension");
+}
+
+// rows [tokens, heads, channels] that a kernel reads with 16-byte loads: unit channel stride, the other strides multiples of 8
+at::Tensor head_rows(const at::Tensor& x) {
+  const bool ok = x.stride(2) == 1 && (x.size(0) <= 1 || (x.stride(0) > 0 && x.stride(0) % 8 == 0)) &&
+                  (x.size(1) <= 1 || (x.stride(1) > 0 && x.stride(1) % 8 == 0)) && ((uintptr_t)x.data_ptr()) % 16 == 0;
+  return ok ? x : x.clone(at::MemoryFormat::Contiguous);
+}
+int64_t stride_of(const at::Tensor& x, int64_t dim) {          // of a dimension with one entry: anything valid
+  return x.size(dim) > 1 ? x.stride(dim) : (dim == 0 ? x.size(1) * x.size(2) : x.size(2));
+}
+
+struct CacheView {
+  int64_t pages, heads, page, dp;
+};
+CacheView check_cache(const at::Tensor& codes, const at::Tensor& scales) {
+  TORCH_CHECK(codes.is_cuda() && scales.is_cuda(), "codes and scales must be CUDA tensors (uniql_b200 has no CPU path)");
+  TORCH_CHECK(codes.scalar_type() == at::kInt && scales.scalar_type() == at::kHalf, "codes must be int32 and scales float16");
+  TORCH_CHECK(codes.dim() == 5 && codes.size(1) == 2 && codes.is_contiguous(),
+              "codes must be a contiguous [pages, 2, kv_heads, page_size, words] tensor");
+  TORCH_CHECK(scales.dim() == 5 && scales.is_contiguous() && scales.size(0) == codes.size(0) && scales.size(1) == 2 &&
+                  scales.size(2) == codes.size(2) && scales.size(3) == codes.size(3) && scales.size(4) == 2,
+              "scales must be a contiguous [pages, 2, kv_heads, page_size, 2] tensor of the same cache");
+  TORCH_CHECK(scales.device() == codes.device(), "codes and scales must be on one device");
+  return {codes.size(0), codes.size(2), codes.size(3), codes.size(4) * 8};
+}
+
+std::vector<at::Tensor> kv_page_plan(const at::Tensor& lens, const at::Tensor& new_lens, const at::Tensor& block_table,
+                                     const at::Tensor& free_pages, const at::Tensor& free_count, int64_t page_size,
+                                     int64_t total_new, bool in_place) {
+  check_ints(lens, lens, 1, "lens");
+  check_ints(new_lens, lens, 1, "new_lens");
+  check_ints(block_table, lens, 2, "block_table");
+  check_ints(free_pages, lens, 1, "free_pages");
+  check_ints(free_count, lens, 1, "free_count");
+  const int64_t batch = lens.size(0), width = block_table.size(1);
+  TORCH_CHECK(new_lens.size(0) == batch && block_table.size(0) == batch, "lens, new_lens and block_table must have one row per request");
+  TORCH_CHECK(free_count.size(0) == 1, "free_count must have one entry");
+  TORCH_CHECK(batch <= 1 || block_table.stride(0) >= width, "rows of block_table must not overlap");
+  TORCH_CHECK(total_new >= 0, "total_new must not be negative");
+  const c10::cuda::CUDAGuard guard(lens.device());
+  const int dev = lens.device().index();
+  const auto i64 = lens.options().dtype(at::kLong);
+  at::Tensor slots = at::empty({total_new}, i64), positions = at::empty({total_new}, i64);
+  at::Tensor cu = at::empty({batch + 1}, lens.options());
+  at::Tensor lens_out = in_place ? lens : at::empty({batch}, lens.options());
+  at::Tensor count_out = in_place ? free_count : at::empty({1}, lens.options());
+  at::Tensor status = status_tensor(dev);
+  const int code = uniql_kv_page_plan(
+      (const int32_t*)lens.data_ptr(), (const int32_t*)new_lens.data_ptr(), batch, (int32_t*)block_table.data_ptr(),
+      batch > 1 ? block_table.stride(0) : width, width, (const int32_t*)free_pages.data_ptr(), free_pages.size(0),
+      (const int32_t*)free_count.data_ptr(), page_size, total_new, (int64_t*)slots.data_ptr(), (int64_t*)positions.data_ptr(),
+      (int32_t*)cu.data_ptr(), (int32_t*)lens_out.data_ptr(), (int32_t*)count_out.data_ptr(), (int*)status.data_ptr(),
+      at::cuda::getCurrentCUDAStream(dev).stream());
+  check_code(code, "uniql_kv_page_plan");
+  return {slots, positions, cu, lens_out, count_out};
+}
+
+void kv4_append(const at::Tensor& k, const at::Tensor& v, const at::Tensor& slots, const at::Tensor& codes, const at::Tensor& scales) {
+  const CacheView cv = check_cache(codes, scales);
+  TORCH_CHECK(k.is_cuda() && v.is_cuda() && k.dim() == 3 && v.dim() == 3, "k and v must be [tokens, kv_heads, channels] CUDA tensors");
+  const int dtype = kv_dtype(k, "k");
+  TORCH_CHECK(v.scalar_type() == k.scalar_type(), "k and v must have the same type");
+  TORCH_CHECK(k.size(0) == v.size(0) && k.size(1) == cv.heads && v.size(1) == cv.heads, "k and v must have one row per token and kv head of the cache");
+  TORCH_CHECK(slots.is_cuda() && slots.scalar_type() == at::kLong && slots.dim() == 1 && slots.size(0) == k.size(0),
+              "slots must be an int64 CUDA tensor with one entry per token");
+  TORCH_CHECK(k.device() == codes.device() && v.device() == codes.device() && slots.device() == codes.device(),
+              "k, v, slots and the cache must be on one device");
+  const c10::cuda::CUDAGuard guard(codes.device());
+  const int dev = codes.device().index();
+  const at::Tensor k3 = head_rows(k), v3 = head_rows(v), sl = slots.contiguous();
+  at::Tensor status = status_tensor(dev);
+  const int code = uniql_kv4_append(k3.data_ptr(), stride_of(k3, 0), stride_of(k3, 1), v3.data_ptr(), stride_of(v3, 0),
+                                    stride_of(v3, 1), dtype, k3.size(0), cv.heads, k3.size(2), v3.size(2),
+                                    (const int64_t*)sl.data_ptr(), codes.data_ptr(), scales.data_ptr(), cv.pages, cv.page, cv.dp,
+                                    (int*)status.data_ptr(), at::cuda::getCurrentCUDAStream(dev).stream());
+  check_code(code, "uniql_kv4_append");
+}
+
+std::vector<at::Tensor> kv4_gather(const at::Tensor& codes, const at::Tensor& scales, const at::Tensor& block_table,
+                                   const at::Tensor& cu, int64_t total, int64_t dk, int64_t dv, bool bf16,
+                                   const std::optional<at::Tensor>& starts) {
+  const CacheView cv = check_cache(codes, scales);
+  check_ints(block_table, codes, 2, "block_table");
+  check_ints(cu, codes, 1, "cu");
+  const int64_t batch = block_table.size(0), width = block_table.size(1);
+  TORCH_CHECK(cu.size(0) == batch + 1, "cu must have one entry more than block_table has rows");
+  TORCH_CHECK(batch <= 1 || block_table.stride(0) >= width, "rows of block_table must not overlap");
+  const bool has_starts = starts.has_value() && starts->defined();
+  if (has_starts) {
+    check_ints(*starts, codes, 1, "starts");
+    TORCH_CHECK(starts->size(0) == batch, "starts must have one entry per request");
+  }
+  TORCH_CHECK(total >= 0 && dk > 0 && dv > 0, "total, head_dim_k and head_dim_v must not be negative");
+  const c10::cuda::CUDAGuard guard(codes.device());
+  const int dev = codes.device().index();
+  const auto opt = scales.options().dtype(bf16 ? at::kBFloat16 : at::kHalf);
+  at::Tensor k = at::empty({total, cv.heads, dk}, opt), v = at::empty({total, cv.heads, dv}, opt);
+  at::Tensor status = status_tensor(dev);
+  const int code = uniql_kv4_gather(codes.data_ptr(), scales.data_ptr(), cv.pages, cv.page, cv.dp, cv.heads,
+                                    (const int32_t*)block_table.data_ptr(), batch > 1 ? block_table.stride(0) : width, width, batch,
+                                    has_starts ? (const int32_t*)starts->data_ptr() : nullptr, (const int32_t*)cu.data_ptr(), total,
+                                    dk, dv, bf16 ? UNIQL_BF16 : UNIQL_F16, k.data_ptr(), v.data_ptr(), (int*)status.data_ptr(),
+                                    at::cuda::getCurrentCUDAStream(dev).stream());
+  check_code(code, "uniql_kv4_gather");
+  return {k, v};
+}
+
+at::Tensor kv4_attention(const at::Tensor& q, const at::Tensor& codes, const at::Tensor& scales, const at::Tensor& block_table,
+                         const at::Tensor& lens, int64_t dv, double softmax_scale) {
+  const CacheView cv = check_cache(codes, scales);
+  TORCH_CHECK(q.is_cuda() && q.dim() == 3, "q must be a [batch, heads, channels] CUDA tensor");
+  const int dtype = kv_dtype(q, "q");
+  check_ints(block_table, codes, 2, "block_table");
+  check_ints(lens, codes, 1, "lens");
+  const int64_t batch = q.size(0), width = block_table.size(1);
+  TORCH_CHECK(block_table.size(0) == batch && lens.size(0) == batch, "q, block_table and lens must have one row per request");
+  TORCH_CHECK(batch <= 1 || block_table.stride(0) >= width, "rows of block_table must not overlap");
+  TORCH_CHECK(q.device() == codes.device(), "q and the cache must be on one device");
+  TORCH_CHECK(dv > 0 && q.size(1) > 0 && q.size(2) > 0, "q and head_dim_v must not be empty");
+  TORCH_CHECK(cv.heads > 0 && q.size(1) % cv.heads == 0, "the query heads must be a multiple of the cache's kv heads");
+  const c10::cuda::CUDAGuard guard(q.device());
+  const int dev = q.device().index();
+  const at::Tensor q3 = q.stride(2) == 1 || q.size(2) == 1 ? q : q.contiguous();
+  at::Tensor out = at::empty({batch, q.size(1), dv}, q.options());
+  if (batch == 0) return out;
+  cudaStream_t stream = at::cuda::getCurrentCUDAStream(dev).stream();
+  const size_t need = uniql_kv4_attention_scratch_bytes(batch, q.size(1), cv.heads, cv.dp);
+  at::Tensor scratch = own_scratch(dev, stream, need);
+  at::Tensor status = status_tensor(dev);
+  const int code = uniql_kv4_attention(q3.data_ptr(), q3.stride(0), q3.stride(1), codes.data_ptr(), scales.data_ptr(), cv.pages,
+                                       cv.page, cv.dp, (const int32_t*)block_table.data_ptr(),
+                                       batch > 1 ? block_table.stride(0) : width, width, (const int32_t*)lens.data_ptr(), batch,
+                                       q.size(1), cv.heads, q.size(2), dv, (float)softmax_scale, dtype, out.data_ptr(),
+                                       scratch.data_ptr(), (size_t)scratch.numel(), (int*)status.data_ptr(), stream);
+  check_code(code, "uniql_kv4_attention");
+  return out;
+}
+
+at::Tensor prompt_attention(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& cu_q,
+                            const std::optional<at::Tensor>& cu_k, bool causal, double softmax_scale) {
+  TORCH_CHECK(q.is_cuda() && k.is_cuda() && v.is_cuda() && q.dim() == 3 && k.dim() == 3 && v.dim() == 3,
+              "q, k and v must be [tokens, heads, channels] CUDA tensors");
+  const int dtype = kv_dtype(q, "q");
+  TORCH_CHECK(k.scalar_type() == q.scalar_type() && v.scalar_type() == q.scalar_type(), "q, k and v must have the same type");
+  TORCH_CHECK(k.device() == q.device() && v.device() == q.device(), "q, k and v must be on one device");
+  TORCH_CHECK(k.size(0) == v.size(0) && k.size(1) == v.size(1) && k.size(2) == q.size(2), "k and v must have the same tokens and heads, q and k the same channels");
+  TORCH_CHECK(k.size(1) > 0 && q.size(1) > 0 && q.size(1) % k.size(1) == 0, "the query heads must be a multiple of the kv heads");
+  TORCH_CHECK(q.size(2) > 0 && v.size(2) > 0, "q, k and v must have channels");
+  check_ints(cu_q, q, 1, "cu_q");
+  const at::Tensor ck = cu_k.has_value() && cu_k->defined() ? *cu_k : cu_q;
+  check_ints(ck, q, 1, "cu_k");
+  TORCH_CHECK(cu_q.size(0) >= 1 && ck.size(0) == cu_q.size(0), "cu_q and cu_k must have one entry more than there are requests");
+  const c10::cuda::CUDAGuard guard(q.device());
+  const int dev = q.device().index();
+  const at::Tensor q3 = head_rows(q), k3 = head_rows(k), v3 = head_rows(v);
+  at::Tensor out = at::empty({q.size(0), q.size(1), v.size(2)}, q.options());
+  at::Tensor status = status_tensor(dev);
+  const int code = uniql_prompt_attention(q3.data_ptr(), stride_of(q3, 0), stride_of(q3, 1), k3.data_ptr(), stride_of(k3, 0),
+                                          stride_of(k3, 1), v3.data_ptr(), stride_of(v3, 0), stride_of(v3, 1),
+                                          (const int32_t*)cu_q.data_ptr(), (const int32_t*)ck.data_ptr(), cu_q.size(0) - 1,
+                                          q.size(0), k.size(0), q.size(1), k.size(1), q.size(2), v.size(2), (float)softmax_scale,
+                                          causal ? 1 : 0, dtype, out.data_ptr(), (int*)status.data_ptr(),
+                                          at::cuda::getCurrentCUDAStream(dev).stream());
+  check_code(code, "uniql_prompt_attention");
+  return out;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -271,4 +462,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("embedding", &embedding, "4-bit embedding gather");
   m.def("hadamard", &hadamard, "Hadamard transform along the last axis");
   m.def("silu_mul", &silu_mul, "silu(gate) * up in one pass");
+  m.def("kv_page_plan", &kv_page_plan, "block tables, slots and positions of a step's new tokens");
+  m.def("kv4_append", &kv4_append, "quantise K/V rows into a paged 4-bit cache");
+  m.def("kv4_gather", &kv4_gather, "rows of a token range of a paged 4-bit cache");
+  m.def("kv4_attention", &kv4_attention, "one query token per request over a paged 4-bit cache");
+  m.def("prompt_attention", &prompt_attention, "causal attention of packed prompts");
 }

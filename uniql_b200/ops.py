@@ -5,9 +5,10 @@ These functions are what the drop-in modules and the `quant_linear_cuda` / `quan
 """
 from __future__ import annotations
 
-import torch
-
 import ctypes
+import math
+
+import torch
 
 from ._lib import Prefetch, Proj, check, lib, torch_ext
 
@@ -34,7 +35,8 @@ def status_word(device: torch.device) -> torch.Tensor:
 
 def read_and_clear_status(device) -> int:
     """Synchronising read of the kernel diagnostics word (bit 0: an embedding id was out of range; bit 1: a bounded
-    wait gave up; bit 2: a slicing index was outside the source layer)."""
+    wait gave up; bit 2: a slicing index was outside the source layer, or a slot or page outside the KV cache; bit 3: a page
+    plan ran out of free pages or of columns of the block table)."""
     t = status_word(torch.device(device))
     v = int(t.item())
     t.zero_()
@@ -398,4 +400,240 @@ def w4a16_dequantize_rows(weight: torch.Tensor, scale: torch.Tensor, row_index: 
                                                  idx.numel(), n_real, out.data_ptr(), idx.numel(),
                                                  status_word(dev).data_ptr(), _stream_handle(dev))
     check(code, "uniql_w4a16_dequantize_rows")
+    return out
+
+
+# ---- attention around a paged KV cache held in 4 bits (layout and rules: include/uniql_b200.h) ---------------------------
+# They go through the torch binding like the modules' forward; with UNIQL_B200_TORCH_EXT=0 the same C calls are made over ctypes.
+
+def _ints(t: torch.Tensor, like: torch.Tensor, dim: int, name: str) -> torch.Tensor:
+    if not t.is_cuda or t.dtype != torch.int32 or t.dim() != dim:
+        raise RuntimeError(f"{name} must be a {dim}-D int32 CUDA tensor")
+    if t.device != like.device:
+        raise RuntimeError(f"{name} is on another device")
+    if t.shape[-1] > 1 and t.stride(-1) != 1:
+        raise RuntimeError(f"{name} must have unit stride in its last dimension")
+    return t
+
+
+def _ld(table: torch.Tensor) -> int:
+    if table.shape[0] > 1 and table.stride(0) < table.shape[1]:
+        raise RuntimeError("rows of block_table must not overlap")
+    return table.stride(0) if table.shape[0] > 1 else table.shape[1]
+
+
+def _cache_shape(codes: torch.Tensor, scales: torch.Tensor):
+    if not codes.is_cuda or not scales.is_cuda:
+        raise RuntimeError("codes and scales must be CUDA tensors (uniql_b200 has no CPU path)")
+    if codes.dtype != torch.int32 or scales.dtype != torch.float16:
+        raise RuntimeError("codes must be int32 and scales float16")
+    if codes.dim() != 5 or codes.shape[1] != 2 or not codes.is_contiguous():
+        raise RuntimeError("codes must be a contiguous [pages, 2, kv_heads, page_size, words] tensor")
+    if scales.shape != (*codes.shape[:4], 2) or not scales.is_contiguous() or scales.device != codes.device:
+        raise RuntimeError("scales must be a contiguous [pages, 2, kv_heads, page_size, 2] tensor of the same cache")
+    pages, _, heads, page, words = codes.shape
+    return pages, heads, page, words * 8
+
+
+def _kv_dtype(t: torch.Tensor, name: str) -> int:
+    if t.dtype not in (torch.float16, torch.bfloat16):
+        raise RuntimeError(f"{name} must be float16 or bfloat16")
+    return _DTYPE_CODE[t.dtype]
+
+
+def _head_rows(x: torch.Tensor) -> torch.Tensor:
+    ok = x.stride(2) == 1 and x.data_ptr() % 16 == 0 and all(x.shape[i] <= 1 or (x.stride(i) > 0 and x.stride(i) % 8 == 0) for i in (0, 1))
+    return x if ok else x.clone(memory_format=torch.contiguous_format)
+
+
+def _row_strides(x: torch.Tensor):
+    return (x.stride(0) if x.shape[0] > 1 else x.shape[1] * x.shape[2]), (x.stride(1) if x.shape[1] > 1 else x.shape[2])
+
+
+def kv4_cache(num_pages: int, kv_heads: int, page_size: int, head_dim: int, device="cuda"):
+    """(codes, scales) of an empty cache of one layer; head_dim: the larger of K's and V's head size."""
+    if page_size not in (16, 32, 64, 128, 256) or not 0 < head_dim <= 128 or head_dim % 8:
+        raise RuntimeError("page_size must be 16, 32, 64, 128 or 256 and head_dim a multiple of 8 up to 128")
+    words = (64 if head_dim <= 64 else 128) // 8
+    return (torch.zeros(num_pages, 2, kv_heads, page_size, words, dtype=torch.int32, device=device),
+            torch.zeros(num_pages, 2, kv_heads, page_size, 2, dtype=torch.float16, device=device))
+
+
+def kv_page_plan(lens: torch.Tensor, new_lens: torch.Tensor, block_table: torch.Tensor, free_pages: torch.Tensor,
+                 free_count: torch.Tensor, page_size: int, total_new: int, in_place: bool = False):
+    """What a step's new tokens need, worked out on the GPU from the requests' lengths: pages from the top of the stack
+    `free_pages` (free_count[0] of them are left) go into `block_table` in place.  Returns (slots int64 [total_new], positions
+    int64 [total_new], cu_new int32 [batch + 1], lens after the step, free_count after the step); with in_place the last two are
+    `lens` and `free_count` themselves.  total_new: places to fill (the rows of the step's tensors; those behind the last
+    token get slot -1).  A shortage of pages or of table columns gives slots of -1 and status bit 3."""
+    ext = torch_ext()
+    if ext is not None:
+        return tuple(ext.kv_page_plan(lens, new_lens, block_table, free_pages, free_count, page_size, total_new, in_place))
+    for t, dim, name in ((lens, 1, "lens"), (new_lens, 1, "new_lens"), (block_table, 2, "block_table"), (free_pages, 1, "free_pages"),
+                         (free_count, 1, "free_count")):
+        _ints(t, lens, dim, name)
+    batch = lens.shape[0]
+    if new_lens.shape[0] != batch or block_table.shape[0] != batch:
+        raise RuntimeError("lens, new_lens and block_table must have one row per request")
+    if free_count.shape[0] != 1 or total_new < 0:
+        raise RuntimeError("free_count must have one entry and total_new must not be negative")
+    ld, dev = _ld(block_table), lens.device
+    slots = torch.empty(total_new, dtype=torch.int64, device=dev)
+    positions = torch.empty(total_new, dtype=torch.int64, device=dev)
+    cu = torch.empty(batch + 1, dtype=torch.int32, device=dev)
+    lens_out = lens if in_place else torch.empty_like(lens)
+    count_out = free_count if in_place else torch.empty_like(free_count)
+    with torch.cuda.device(dev):
+        code = lib().uniql_kv_page_plan(lens.data_ptr(), new_lens.data_ptr(), batch, block_table.data_ptr(), ld, block_table.shape[1],
+                                        free_pages.data_ptr(), free_pages.shape[0], free_count.data_ptr(), page_size, total_new,
+                                        slots.data_ptr(), positions.data_ptr(), cu.data_ptr(), lens_out.data_ptr(),
+                                        count_out.data_ptr(), status_word(dev).data_ptr(), _stream_handle(dev))
+    check(code, "uniql_kv_page_plan")
+    return slots, positions, cu, lens_out, count_out
+
+
+def kv4_append(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor) -> None:
+    """Quantise the rows k, v [tokens, kv_heads, channels] (fp16 or bf16) to 4 bits with one scale and zero per token and head and
+    store them in the cache at `slots` (int64; -1 skips the token; the others must differ)."""
+    ext = torch_ext()
+    if ext is not None:
+        ext.kv4_append(k, v, slots, codes, scales)
+        return
+    pages, heads, page, dp = _cache_shape(codes, scales)
+    if not k.is_cuda or not v.is_cuda or k.dim() != 3 or v.dim() != 3:
+        raise RuntimeError("k and v must be [tokens, kv_heads, channels] CUDA tensors")
+    dtype = _kv_dtype(k, "k")
+    if v.dtype != k.dtype:
+        raise RuntimeError("k and v must have the same type")
+    if k.shape[0] != v.shape[0] or k.shape[1] != heads or v.shape[1] != heads:
+        raise RuntimeError("k and v must have one row per token and kv head of the cache")
+    if not slots.is_cuda or slots.dtype != torch.int64 or slots.dim() != 1 or slots.shape[0] != k.shape[0]:
+        raise RuntimeError("slots must be an int64 CUDA tensor with one entry per token")
+    dev = codes.device
+    if any(t.device != dev for t in (k, v, slots)):
+        raise RuntimeError("k, v, slots and the cache must be on one device")
+    k, v, slots = _head_rows(k), _head_rows(v), slots.contiguous()
+    with torch.cuda.device(dev):
+        code = lib().uniql_kv4_append(k.data_ptr(), *_row_strides(k), v.data_ptr(), *_row_strides(v), dtype, k.shape[0], heads,
+                                      k.shape[2], v.shape[2], slots.data_ptr(), codes.data_ptr(), scales.data_ptr(), pages, page, dp,
+                                      status_word(dev).data_ptr(), _stream_handle(dev))
+    check(code, "uniql_kv4_append")
+
+
+def kv4_gather(codes: torch.Tensor, scales: torch.Tensor, block_table: torch.Tensor, cu: torch.Tensor, total: int, head_dim_k: int,
+               head_dim_v: int | None = None, dtype: torch.dtype = torch.float16, starts: torch.Tensor | None = None):
+    """The cached rows of a token range of every request, dequantised and packed: request i gives cu[i + 1] - cu[i] tokens from
+    starts[i] on (None: from its first).  Returns k [total, kv_heads, head_dim_k] and v [total, kv_heads, head_dim_v]; places behind
+    cu[-1] are zeros."""
+    dv = head_dim_k if head_dim_v is None else head_dim_v
+    if dtype not in (torch.float16, torch.bfloat16):
+        raise RuntimeError("dtype must be float16 or bfloat16")
+    ext = torch_ext()
+    if ext is not None:
+        return tuple(ext.kv4_gather(codes, scales, block_table, cu, total, head_dim_k, dv, dtype == torch.bfloat16, starts))
+    pages, heads, page, dp = _cache_shape(codes, scales)
+    _ints(block_table, codes, 2, "block_table")
+    _ints(cu, codes, 1, "cu")
+    batch = block_table.shape[0]
+    if cu.shape[0] != batch + 1:
+        raise RuntimeError("cu must have one entry more than block_table has rows")
+    if starts is not None and _ints(starts, codes, 1, "starts").shape[0] != batch:
+        raise RuntimeError("starts must have one entry per request")
+    if total < 0 or head_dim_k <= 0 or dv <= 0:
+        raise RuntimeError("total, head_dim_k and head_dim_v must not be negative")
+    ld, dev = _ld(block_table), codes.device
+    k = torch.empty(total, heads, head_dim_k, dtype=dtype, device=dev)
+    v = torch.empty(total, heads, dv, dtype=dtype, device=dev)
+    with torch.cuda.device(dev):
+        code = lib().uniql_kv4_gather(codes.data_ptr(), scales.data_ptr(), pages, page, dp, heads, block_table.data_ptr(), ld,
+                                      block_table.shape[1], batch, starts.data_ptr() if starts is not None else None, cu.data_ptr(),
+                                      total, head_dim_k, dv, _DTYPE_CODE[dtype], k.data_ptr(), v.data_ptr(),
+                                      status_word(dev).data_ptr(), _stream_handle(dev))
+    check(code, "uniql_kv4_gather")
+    return k, v
+
+
+def _own_scratch(device: torch.device, nbytes: int) -> torch.Tensor:
+    """Scratch of a call that a graph may replay beside eager calls and other graphs: the graph's own while the stream is captured."""
+    if torch.cuda.is_current_stream_capturing():
+        return torch.zeros(nbytes, dtype=torch.uint8, device=device)
+    return _scratch_for(device, nbytes)
+
+
+def kv4_attention(q: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, block_table: torch.Tensor, lens: torch.Tensor,
+                  head_dim_v: int | None = None, softmax_scale: float | None = None) -> torch.Tensor:
+    """One query token per request over its first lens[i] cached tokens: q [batch, heads, channels] (fp16 or bf16), grouped heads.
+    Returns [batch, heads, head_dim_v] in q's type; a request of length 0 gives zeros.  softmax_scale: 1 / sqrt(channels)."""
+    if q.dim() != 3:
+        raise RuntimeError("q must be a [batch, heads, channels] CUDA tensor")
+    dk = q.shape[2]
+    dv = dk if head_dim_v is None else head_dim_v
+    scale = 1.0 / math.sqrt(max(dk, 1)) if softmax_scale is None else float(softmax_scale)
+    ext = torch_ext()
+    if ext is not None:
+        return ext.kv4_attention(q, codes, scales, block_table, lens, dv, scale)
+    pages, kv_heads, page, dp = _cache_shape(codes, scales)
+    _require_cuda(q, "q")
+    dtype = _kv_dtype(q, "q")
+    _ints(block_table, codes, 2, "block_table")
+    _ints(lens, codes, 1, "lens")
+    batch, heads = q.shape[:2]
+    if block_table.shape[0] != batch or lens.shape[0] != batch:
+        raise RuntimeError("q, block_table and lens must have one row per request")
+    if q.device != codes.device:
+        raise RuntimeError("q and the cache must be on one device")
+    if dv <= 0 or heads <= 0 or dk <= 0 or kv_heads <= 0 or heads % kv_heads:
+        raise RuntimeError("the query heads must be a multiple of the cache's kv heads, and head sizes positive")
+    ld, dev = _ld(block_table), q.device
+    q = q if q.stride(2) == 1 or dk == 1 else q.contiguous()
+    out = torch.empty(batch, heads, dv, dtype=q.dtype, device=dev)
+    if batch == 0:
+        return out
+    with torch.cuda.device(dev):
+        need = lib().uniql_kv4_attention_scratch_bytes(batch, heads, kv_heads, dp)
+        scratch = _own_scratch(dev, need)
+        code = lib().uniql_kv4_attention(q.data_ptr(), q.stride(0), q.stride(1), codes.data_ptr(), scales.data_ptr(), pages, page, dp,
+                                         block_table.data_ptr(), ld, block_table.shape[1], lens.data_ptr(), batch, heads, kv_heads,
+                                         dk, dv, scale, dtype, out.data_ptr(), scratch.data_ptr(), scratch.numel(),
+                                         status_word(dev).data_ptr(), _stream_handle(dev))
+    check(code, "uniql_kv4_attention")
+    return out
+
+
+def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: torch.Tensor, cu_k: torch.Tensor | None = None,
+                     causal: bool = True, softmax_scale: float | None = None) -> torch.Tensor:
+    """Attention of packed prompts of different lengths: q [tokens, heads, channels], k and v [key tokens, kv_heads, channels] (fp16
+    or bf16; views of a fused q/k/v result are fine), request i owning rows cu_q[i] .. cu_q[i + 1] - 1 of q and cu_k[i] .. of k and
+    v (cu_k None: the same).  With causal the last query of a request sees all its keys, the one before it all but the last.
+    Returns [tokens, heads, channels of v]; queries that see no key, and rows that no request owns, give zeros."""
+    if q.dim() != 3:
+        raise RuntimeError("q must be a [tokens, heads, channels] CUDA tensor")
+    scale = 1.0 / math.sqrt(max(q.shape[2], 1)) if softmax_scale is None else float(softmax_scale)
+    ext = torch_ext()
+    if ext is not None:
+        return ext.prompt_attention(q, k, v, cu_q, cu_k, causal, scale)
+    if not (q.is_cuda and k.is_cuda and v.is_cuda) or k.dim() != 3 or v.dim() != 3:
+        raise RuntimeError("q, k and v must be [tokens, heads, channels] CUDA tensors")
+    dtype = _kv_dtype(q, "q")
+    dev = q.device
+    if k.dtype != q.dtype or v.dtype != q.dtype or k.device != dev or v.device != dev:
+        raise RuntimeError("q, k and v must have the same type and device")
+    if k.shape[:2] != v.shape[:2] or k.shape[2] != q.shape[2]:
+        raise RuntimeError("k and v must have the same tokens and heads, q and k the same channels")
+    heads, kv_heads = q.shape[1], k.shape[1]
+    if heads <= 0 or kv_heads <= 0 or heads % kv_heads or q.shape[2] <= 0 or v.shape[2] <= 0:
+        raise RuntimeError("the query heads must be a multiple of the kv heads, and head sizes positive")
+    ck = cu_q if cu_k is None else cu_k
+    _ints(cu_q, q, 1, "cu_q")
+    _ints(ck, q, 1, "cu_k")
+    if cu_q.shape[0] < 1 or ck.shape[0] != cu_q.shape[0]:
+        raise RuntimeError("cu_q and cu_k must have one entry more than there are requests")
+    q, k, v = _head_rows(q), _head_rows(k), _head_rows(v)
+    out = torch.empty(q.shape[0], heads, v.shape[2], dtype=q.dtype, device=dev)
+    with torch.cuda.device(dev):
+        code = lib().uniql_prompt_attention(q.data_ptr(), *_row_strides(q), k.data_ptr(), *_row_strides(k), v.data_ptr(), *_row_strides(v),
+                                            cu_q.data_ptr(), ck.data_ptr(), cu_q.shape[0] - 1, q.shape[0], k.shape[0], heads, kv_heads,
+                                            q.shape[2], v.shape[2], scale, 1 if causal else 0, dtype, out.data_ptr(),
+                                            status_word(dev).data_ptr(), _stream_handle(dev))
+    check(code, "uniql_prompt_attention")
     return out
