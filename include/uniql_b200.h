@@ -369,8 +369,8 @@ int uniql_w4a16_swap_plan_check(void);
  *   covers, and tokens on a page outside the cache, are zeros.
  *
  * uniql_kv4_attention: one query token per request over its first lens[i] cached tokens (grouped heads: query head h reads kv head
- *   h / (heads / kv_heads)): out[i, h] = softmax(softmax_scale * q k^T) v in fp32, rounded once.  Length 0, or no token on a page of
- *   the cache, gives zeros.  The tokens are split evenly over the GPU whatever the lengths are, and the parts of a request are
+ *   h / (heads / kv_heads)): out[i, h] = softmax(softmax_scale * q k^T) v in fp32, rounded once.  A V scale of 0 (a row that was
+ *   never written) and a page outside the cache are absent tokens; without any token the result is zeros.  The tokens are split evenly over the GPU whatever the lengths are, and the parts of a request are
  *   joined in a fixed order.
  *   scratch  uniql_kv4_attention_scratch_bytes(...) bytes, rules as for uniql_w4a16_linear
  *

@@ -1,23 +1,24 @@
 // Attention of one query token per request over a paged KV cache held in 4 bits.  Layout and rules: include/uniql_b200.h.
 //
 // Mathematics.  With a cached row k_t = z + s c and m = z + 8 s the score is  x_t = f (s (q . (c - 8)) + m sum(q)),  f =
-// softmax_scale log2(e): the products run over the exact centred codes on the tensor cores (mma.sync m16n8k16, fp32 sums),
-// scale and zero enter once per token in fp32.  The value side folds its scale into the exponent: with y_t = x_t + log2 s'_t,
-// M a running bound of y and w_t = 2^(y_t - M),
+// softmax_scale log2(e): the products run over the exact centred codes on the tensor cores (mma.sync m16n8k16, fp32 sums), scale
+// and zero enter once per token in fp32.  (mma.sync on e4m3, where a code needs no conversion, was built and taken out: this part
+// runs it as conversions and fp16 products, 478 instructions per 16 tokens either way.)  Queries are taken to fp16 after a
+// division by the power of two below their largest channel: exact, but for channels under 2^-14 of the largest.
+// The value side folds its scale into the exponent: with y_t = x_t + log2 s'_t, M a running bound of y and w_t = 2^(y_t - M),
 //     out = (sum w_t (c'_t - 8) + sum (w_t / s'_t) m'_t) / sum (w_t / s'_t),
 // so that w is the one operand that is rounded (fp16, 2^-12 relative above 6e-5; it is at most 2^8, see below), next to exact
-// codes, whatever the magnitude of the values.  M is raised, and the sums rescaled, only when some y exceeds it by more than 8.
-// Queries are taken to fp16 after a division by the power of two below their largest channel: exact, but for channels under 2^-14
-// of the largest.
+// fp16 codes, whatever the magnitude of the values.  M is raised, and the sums rescaled, only when some y exceeds it by more
+// than 8.
 //
 // Layout of the products.  Tokens are the 16-row operand of the first product (a lane's packed words of two tokens are its
 // fragment; which channel sits at which k index is free, so long as the query fragments follow), query heads its eight
-// columns.  The weights w cross to the second product by two 8 x 8 transposes (movmatrix); there channels are the rows and the
-// tokens of a lane meet pairwise: two byte permutes join the same nibbles of two tokens.  So the 4-bit words go from shared
-// memory to the tensor cores with one LOP3 and one HSUB2 / HFMA2 per two codes.
+// columns.  The weights w cross to the second product by 8 x 8 transposes (movmatrix); there channels are the rows and the
+// tokens of a lane meet pairwise: byte permutes join the same nibbles of two tokens.  So the 4-bit words go from shared memory
+// to the tensor cores in registers.
 //
-// Bound: HBM, (dk + dv) / 2 + 8 bytes per token and kv head.  Each warp keeps a ring of kStages steps of 16 tokens in flight
-// with cp.async.  Split: the 64-token tiles of all requests form one list (a tile: one request, one kv head), cut into equal
+// Bound: HBM, (dk + dv) / 2 + 8 bytes per token and kv head.  Each warp keeps a ring of kStages steps of 32 tokens in flight
+// with cp.async.  Split: the 32-token steps of all requests form one list (a step: one request, one kv head), cut into equal
 // ranges, one per CTA; lengths are read on the device.  A CTA whose range covers only a part of a request's list stores an
 // fp32 partial (sums, M), and the last CTA of that request to arrive joins the parts in order: deterministic.
 #include "common.cuh"
@@ -28,10 +29,15 @@ namespace uniql {
 
 namespace kva {
 constexpr int kWarps = 4, kThreads = kWarps * 32;
-constexpr int kStages = 4;
-constexpr int kTile = 16 * kWarps;              // tokens of a tile
+constexpr int kStages = 3;
+constexpr int kStep = 32;                       // tokens of a step: one warp, one turn of its ring
+constexpr int kMinSteps = kWarps;               // steps a CTA gets at least, while there are fewer than the GPU could hold
 constexpr float kFloor = -1e30f;                // M before the first token
 constexpr int kMaxCtas = 2048;
+#ifndef KVA_PER
+#define KVA_PER 3
+#endif
+constexpr int per_sm(int nt) { return nt == 1 ? KVA_PER : 2; }        // resident CTAs
 }  // namespace kva
 
 struct KvaParams {
@@ -43,11 +49,11 @@ struct KvaParams {
   int64_t ld_table;
   const int32_t* lens;
   unsigned char* out;
-  float* part;                                  // [2 * ctas][8 NT][DP + 2]
+  float* part;                                  // [2 * ctas][8 NT][DP + 4]
   int* tickets;                                 // [ctas], zero
   int* status_word;
   int batch, heads, kv_heads, group, hgroups;   // group: query heads of a kv head; hgroups: launches of 8 NT of them
-  int max_blocks, num_pages, page_shift, dk, dv, bf16;
+  int max_blocks, num_pages, page_shift, dk, dv, bf16, q_vec;     // q_vec: rows of q are 16-byte aligned
   float scale_log2;
 };
 
@@ -77,37 +83,49 @@ __device__ __forceinline__ void kva_store(unsigned char* p, int64_t i, int bf16,
   else reinterpret_cast<__half*>(p)[i] = __float2half_rn(v);
 }
 
-// The token (of a step's 16) that sits at row / k index r of the products: k = 2c, 2c + 1, 2c + 8, 2c + 9 are tokens c, 7 - c, 8 + c
+__device__ __forceinline__ float kva_log2(float x) {
+  float y;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float kva_rcp(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// The token (of 16) that sits at row / k index r of the products: k = 2c, 2c + 1, 2c + 8, 2c + 9 are tokens c, 7 - c, 8 + c
 // and 15 - c.  With it, and the 16-byte chunks of 64-byte rows swapped in pairs by bit 1 of the token, both the rows (four lanes
 // a row) and the columns (eight lanes a row, four tokens) are read from shared memory without bank conflicts.
 __device__ __forceinline__ int kva_token(int r) { return (r & 8) + ((r & 1) ? 7 - ((r & 7) >> 1) : ((r & 7) >> 1)); }
 
 template <int DP, int NT>
-__global__ void __launch_bounds__(kva::kThreads, NT == 1 ? 4 : 2) kv4_attention_kernel(const __grid_constant__ KvaParams p) {
+__global__ void __launch_bounds__(kva::kThreads, kva::per_sm(NT)) kv4_attention_kernel(const __grid_constant__ KvaParams p) {
   using namespace kva;
   constexpr int ROWB = DP / 2;                  // bytes of a packed row
-  constexpr int CODEB = 16 * ROWB;              // one step's packed rows, K or V
-  constexpr int STAGEB = 2 * CODEB + 128;       // K codes, V codes, K scales, V scales
-  constexpr int RINGB = kStages * STAGEB;
-  constexpr int H = 8 * NT, MT = DP / 16, QK = DP / 16;
-  constexpr int PSTR = DP + 2;                  // floats of one head's partial
+  constexpr int CODEB = 16 * ROWB;              // packed rows of 16 tokens, K or V
+  constexpr int OFF_SC = 4 * CODEB;             // of a stage: K codes (two halves of 16 tokens), V codes, then 128 bytes of scales a half
+  constexpr int STAGEB = OFF_SC + 256;
+  constexpr int RINGB = kStages * STAGEB, WARPB = RINGB + kStep * 20;
+  constexpr int H = 8 * NT, MT = DP / 16, KS = DP / 32;
+  constexpr int PSTR = DP + 4;                  // floats of one head's partial: sums, M, L
   extern __shared__ __align__(16) unsigned char smem[];
   __shared__ long long s_wide[kWarps];
   __shared__ float s_m[kWarps][H], s_l[kWarps][H], s_z[kWarps][H];
-  __shared__ int s_find[2];
+  __shared__ int s_find;
   __shared__ long long s_before;
   __shared__ int s_last;
   pdl_wait();
   pdl_launch_dependents();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
   const int cap = min((int64_t)p.max_blocks << p.page_shift, (int64_t)kMaxTokens);
-  const int lists = p.kv_heads * p.hgroups;     // tile lists of a request
+  const int lists = p.kv_heads * p.hgroups;     // lists of a request
   auto length = [&](int b) { return min(max(p.lens[b], 0), cap); };
 
-  // ---- this CTA's range of the list of all tiles
+  // ---- this CTA's range of the list of all steps
   const int per = (p.batch + kThreads - 1) / kThreads;
+  const int b0 = min(tid * per, p.batch), b1 = min(b0 + per, p.batch);
   long long mine = 0;
-  for (int b = tid * per; b < min((tid + 1) * per, p.batch); ++b) mine += (length(b) + kTile - 1) / kTile;
+  for (int b = b0; b < b1; ++b) mine += (length(b) + kStep - 1) / kStep;
   long long incl = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -122,8 +140,8 @@ __global__ void __launch_bounds__(kva::kThreads, NT == 1 ? 4 : 2) kv4_attention_
     if (w < warp) before += s_wide[w];
     total += s_wide[w];
   }
-  const long long N = total * lists;            // at most 2^28 / 64 * 2^14 * 2^10 < 2^47; times the CTAs below 2^58
-  const long long ctas = min((long long)gridDim.x, N);
+  const long long N = total * lists;            // below 2^48, times the CTAs below 2^59
+  const long long ctas = min((long long)gridDim.x, (N + kMinSteps - 1) / kMinSteps);
   const long long begin = blockIdx.x < ctas ? N * blockIdx.x / ctas : 0;
   const long long end = blockIdx.x < ctas ? N * (blockIdx.x + 1) / ctas : 0;
   // idle rows of the batch
@@ -133,10 +151,10 @@ __global__ void __launch_bounds__(kva::kThreads, NT == 1 ? 4 : 2) kv4_attention_
   if (begin == end) return;
   if (mine && before * lists <= begin && begin < (before + mine) * lists) {
     long long at = before;
-    for (int b = tid * per; b < min((tid + 1) * per, p.batch); ++b) {
-      const int t = (length(b) + kTile - 1) / kTile;
+    for (int b = b0; b < b1; ++b) {
+      const int t = (length(b) + kStep - 1) / kStep;
       if (begin < (at + t) * lists) {
-        s_find[0] = b;
+        s_find = b;
         s_before = at * lists;
         break;
       }
@@ -144,67 +162,77 @@ __global__ void __launch_bounds__(kva::kThreads, NT == 1 ? 4 : 2) kv4_attention_
     }
   }
   __syncthreads();
-  int b = s_find[0];
+  int b = s_find;
   long long req_begin = s_before;
 
-  const uint32_t ring = smem_addr(smem) + warp * RINGB;
+  const uint32_t ring = smem_addr(smem) + warp * WARPB, meta = ring + RINGB;
   const int tok_a = kva_token(g);               // rows g and g + 8 of the first product: tokens tok_a and 8 + tok_a
+  const int pmask = (1 << p.page_shift) - 1;
+  const int64_t page_codes = ((int64_t)2 * p.kv_heads * ROWB) << p.page_shift, v_codes = page_codes / 2;
+  const int64_t page_scales = ((int64_t)8 * p.kv_heads) << p.page_shift;
   bool bad_page = false;
 
   for (long long cur = begin; cur < end;) {
     int len = length(b);
-    int tiles = (len + kTile - 1) / kTile;
-    while (cur >= req_begin + (long long)tiles * lists) {       // next request that has tokens
-      req_begin += (long long)tiles * lists;
+    int steps = (len + kStep - 1) / kStep;
+    while (cur >= req_begin + (long long)steps * lists) {       // next request that has tokens
+      req_begin += (long long)steps * lists;
       ++b;
       len = length(b);
-      tiles = (len + kTile - 1) / kTile;
+      steps = (len + kStep - 1) / kStep;
     }
-    const int list = (int)((cur - req_begin) / tiles);
-    const long long list_begin = req_begin + (long long)list * tiles;
+    const int list = (int)((cur - req_begin) / steps);
+    const long long list_begin = req_begin + (long long)list * steps;
     const int t0 = (int)(cur - list_begin);
-    const int t1 = (int)min((long long)tiles, t0 + (end - cur));
+    const int t1 = (int)min((long long)steps, t0 + (end - cur));
     const int kvh = list / p.hgroups, hg = list - kvh * p.hgroups;
     const int head0 = kvh * p.group + hg * H;                   // first query head of this list
     const int nh = min(H, p.group - hg * H);
     cur += t1 - t0;
 
-    // ---- producer: step `st` (16 tokens) of this warp into ring slot st / kWarps % kStages
-    const int first = t0 * kWarps + warp, last = min(t1 * kWarps, (len + 15) / 16);   // steps first, first + kWarps, .. < last
+    // ---- producer: 32 tokens into a ring slot, 16 at a time (a page holds at least 16)
+    const int first = t0 + warp;                                // this warp's steps: first, first + kWarps, .. < t1
     const int32_t* trow = p.table + (size_t)b * p.ld_table;
-    const int pmask = (1 << p.page_shift) - 1;
-    uint32_t absent = 0;                        // bit i: ring slot i holds a step whose page is outside the cache
-    int next_page = first < last ? trow[first * 16 >> p.page_shift] : 0;
-    auto produce = [&](int st, int slot) {
-      if (st < last) {
-        const int page = next_page;
-        if (st + kWarps < last) next_page = trow[(st + kWarps) * 16 >> p.page_shift];
-        const bool ok = (unsigned)page < (unsigned)p.num_pages;
-        bad_page |= !ok;
-        absent = (absent & ~(1u << slot)) | ((ok ? 0u : 1u) << slot);
-        const size_t row = (((size_t)(ok ? page : 0) * 2 * p.kv_heads + kvh) << p.page_shift) + (st * 16 & pmask);
-        const size_t vrow = row + ((size_t)p.kv_heads << p.page_shift);
-        const uint32_t dst = ring + slot * STAGEB;
+    const unsigned char* kbase = p.codes + (((int64_t)kvh * ROWB) << p.page_shift) + lane * 16;
+    const unsigned char* sbase = p.scales + (((int64_t)kvh * 4) << p.page_shift) + ((lane & 4) ? page_scales / 2 : 0) + (lane & 3) * 16;
+    const int last_block = (len - 1) >> p.page_shift;
+    int page0 = 0, page1 = 0;                                   // of the step that is produced next
+    auto look = [&](int st) {
+      page0 = trow[min(st * kStep >> p.page_shift, last_block)];
+      page1 = trow[min((st * kStep + 16) >> p.page_shift, last_block)];
+    };
+    if (first < t1) look(first);
+    auto produce = [&](int st, uint32_t dst) {
+      if (st < t1) {
+        int page[2] = {page0, page1};
+        if (st + kWarps < t1) look(st + kWarps);
 #pragma unroll
-        for (int i = 0; i < CODEB / 512; ++i) {
-          const int ch = lane + 32 * i;         // 16-byte chunk of the step
-          uint32_t d = ch * 16;
-          if (DP == 128) d ^= ((ch >> 3) & 1) << 5;             // chunk of token t = ch / 4 moves to chunk ^ (t & 2)
+        for (int h = 0; h < 2; ++h) {
+          const bool ok = (unsigned)page[h] < (unsigned)p.num_pages;
+          bad_page |= !ok;
+          const int at = (st * kStep + 16 * h) & pmask;
           // an absent page copies nothing, from an address that exists
-          kva_cp16(dst + d, ok ? p.codes + row * ROWB + ch * 16 : (const unsigned char*)p.part, ok);
-          kva_cp16(dst + CODEB + d, ok ? p.codes + vrow * ROWB + ch * 16 : (const unsigned char*)p.part, ok);
+          const unsigned char* src = ok ? kbase + page[h] * page_codes + at * ROWB : (const unsigned char*)p.part;
+          const unsigned char* vsrc = ok ? src + v_codes : src;
+#pragma unroll
+          for (int i = 0; i < CODEB / 512; ++i) {
+            const int ch = lane + 32 * i;                       // 16-byte chunk of the half
+            uint32_t d = dst + h * CODEB + ch * 16;
+            if (DP == 128) d = dst + h * CODEB + ((ch * 16) ^ (((ch >> 3) & 1) << 5));   // chunk of token t = ch / 4 moves to chunk ^ (t & 2)
+            kva_cp16(d, src + i * 512, ok);
+            kva_cp16(d + 2 * CODEB, vsrc + i * 512, ok);
+          }
+          if ((lane >> 3) == h) kva_cp16(dst + OFF_SC + lane * 16, ok ? sbase + page[h] * page_scales + at * 4 : (const unsigned char*)p.part, ok);
         }
-        if (lane < 8)
-          kva_cp16(dst + 2 * CODEB + lane * 16, ok ? p.scales + (lane < 4 ? row : vrow) * 4 + (lane & 3) * 16 : (const unsigned char*)p.part, ok);
       }
       asm volatile("cp.async.commit_group;" ::: "memory");
     };
 #pragma unroll
-    for (int i = 0; i < kStages - 1; ++i) produce(first + i * kWarps, i);
+    for (int i = 0; i < kStages - 1; ++i) produce(first + i * kWarps, ring + i * STAGEB);
 
-    // ---- query fragments
-    uint32_t qf[NT][2 * QK];
-    float f[NT][2], fq[NT][2];                  // per head 8 nt + 2c + e: f 2^e_h, f sum(q)
+    // ---- query fragments: k index 2c + e of step 2i + j is channel 8 (KS c + i) + 2j + 4e, k index 8 + 2c + e the one behind it
+    uint32_t qf[NT][4 * KS];
+    float f[NT][2], fq[NT][2];                  // of heads 8 nt + 2c + e: f up, f sum(q)
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       const int h = nt * 8 + g;
@@ -212,9 +240,30 @@ __global__ void __launch_bounds__(kva::kThreads, NT == 1 ? 4 : 2) kv4_attention_
       float v[DP / 4];
       float top = 0.f, sum = 0.f;
 #pragma unroll
-      for (int i = 0; i < DP / 4; ++i) {
+      for (int i = 0; i < DP / 4; i += 8) {
         const int d = c * (DP / 4) + i;
-        v[i] = (h < nh && d < p.dk) ? kva_load(p.q, base + d, p.bf16) : 0.f;
+        if (h < nh && d < p.dk) {
+          if (p.q_vec) {
+            const uint4 w = *reinterpret_cast<const uint4*>(p.q + 2 * (base + d));
+            const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float2 t = p.bf16 ? __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&u[e]))
+                                      : __half22float2(*reinterpret_cast<const __half2*>(&u[e]));
+              v[i + 2 * e] = t.x;
+              v[i + 2 * e + 1] = t.y;
+            }
+          } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[i + e] = kva_load(p.q, base + d + e, p.bf16);
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[i + e] = 0.f;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < DP / 4; ++i) {
         top = fmaxf(top, fabsf(v[i]));
         sum += v[i];
       }
@@ -223,12 +272,12 @@ __global__ void __launch_bounds__(kva::kThreads, NT == 1 ? 4 : 2) kv4_attention_
         top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
         sum += __shfl_xor_sync(~0u, sum, o);
       }
-      // 2^-e with 2^e <= top < 2^(e + 1), kept where both powers are normal numbers; 1 for zeros and infinities
+      // down = 2^-e, up = 2^e for 2^e <= top < 2^(e + 1), where both are normal numbers; 1 for zeros and infinities
       const int eb = (__float_as_int(top) >> 23) & 255;
       const bool scaled = eb >= 1 && eb <= 253;
       const float down = scaled ? __int_as_float((254 - eb) << 23) : 1.f, up = scaled ? __int_as_float(eb << 23) : 1.f;
 #pragma unroll
-      for (int i = 0; i < DP / 32; ++i)
+      for (int i = 0; i < KS; ++i)
 #pragma unroll
         for (int n = 0; n < 4; ++n) {
           const __half2 h2 = __floats2half2_rn(v[8 * i + n] * down, v[8 * i + n + 4] * down);
@@ -251,32 +300,47 @@ __global__ void __launch_bounds__(kva::kThreads, NT == 1 ? 4 : 2) kv4_attention_
       for (int e = 0; e < 2; ++e) { M[nt][e] = kFloor; L[nt][e] = Z[nt][e] = 0.f; }
     }
 
-    int slot = 0;
-    for (int st = first; st < last; st += kWarps) {
-      const int fill = slot == 0 ? kStages - 1 : slot - 1;
+    uint32_t slot = ring, fill = ring + (kStages - 1) * STAGEB;
+    for (int st = first; st < t1; st += kWarps) {
       produce(st + (kStages - 1) * kWarps, fill);
+      fill = slot;
       asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
       __syncwarp();
-      const uint32_t sk = ring + slot * STAGEB, sv = sk + CODEB, ss = sv + CODEB;
-      // ---- scores of 16 tokens
-      float x[NT][4];
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) x[nt][0] = x[nt][1] = x[nt][2] = x[nt][3] = 0.f;
+      // ---- what the 32 tokens' scales stand for, one token a lane: s, m f-less, log2 s', 1 / s', m' / s'
       {
-        uint32_t wa[DP / 32], wb[DP / 32];
+        const uint32_t at = slot + OFF_SC + (lane >> 4) * 128 + (lane & 15) * 4;
+        const uint32_t km = kva_lds32(at), vm = kva_lds32(at + 64);
+        const float2 kf = __half22float2(*reinterpret_cast<const __half2*>(&km));
+        const float2 vf = __half22float2(*reinterpret_cast<const __half2*>(&vm));
+        const bool real = lane < len - st * kStep && vf.x != 0.f;     // a scale of 0: never written, or an absent page
+        const float vs = real ? fmaxf(vf.x, 5.9604645e-8f) : 1.f, r = kva_rcp(vs);
+        asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(meta + lane * 16), "f"(real ? kf.x : 0.f),
+                     "f"(real ? fmaf(8.f, kf.x, kf.y) : 0.f), "f"(real ? kva_log2(vs) : -INFINITY), "f"(r) : "memory");
+        asm volatile("st.shared.f32 [%0], %1;" ::"r"(meta + kStep * 16 + lane * 4), "f"(real ? fmaf(8.f, vf.x, vf.y) * r : 0.f) : "memory");
+      }
+      __syncwarp();
+      // ---- scores
+      float x[2][NT][4];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          x[h][nt][0] = x[h][nt][1] = x[h][nt][2] = x[h][nt][3] = 0.f;
+        }
+        uint32_t wa[KS], wb[KS];
         if (DP == 128) {
-          const uint32_t ad = sk + tok_a * ROWB + ((c * 16) ^ ((tok_a & 2) << 4));
+          const uint32_t ad = slot + h * CODEB + tok_a * ROWB + ((c * 16) ^ ((tok_a & 2) << 4));
           const uint4 a = lds128(ad), e = lds128(ad + 8 * ROWB);
-          wa[0] = a.x; wa[1] = a.y; wa[DP / 32 - 2] = a.z; wa[DP / 32 - 1] = a.w;
-          wb[0] = e.x; wb[1] = e.y; wb[DP / 32 - 2] = e.z; wb[DP / 32 - 1] = e.w;
+          wa[0] = a.x; wa[1] = a.y; wa[KS - 2] = a.z; wa[KS - 1] = a.w;
+          wb[0] = e.x; wb[1] = e.y; wb[KS - 2] = e.z; wb[KS - 1] = e.w;
         } else {
-          const uint32_t ad = sk + tok_a * ROWB + c * 8;
+          const uint32_t ad = slot + h * CODEB + tok_a * ROWB + c * 8;
           const uint2 a = lds64(ad), e = lds64(ad + 8 * ROWB);
           wa[0] = a.x; wa[1] = a.y;
           wb[0] = e.x; wb[1] = e.y;
         }
 #pragma unroll
-        for (int i = 0; i < DP / 32; ++i) {
+        for (int i = 0; i < KS; ++i) {
           const uint32_t a8 = wa[i] >> 8, b8 = wb[i] >> 8;
           const uint32_t lo[4] = {kv4_pair(wa[i], 0x64086408u), kv4_pair(wb[i], 0x64086408u),
                                   kv4_pair_hi(wa[i], 0xd480d480u), kv4_pair_hi(wb[i], 0xd480d480u)};
@@ -284,43 +348,38 @@ __global__ void __launch_bounds__(kva::kThreads, NT == 1 ? 4 : 2) kv4_attention_
                                   kv4_pair_hi(a8, 0xd480d480u), kv4_pair_hi(b8, 0xd480d480u)};
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
-            mma_m16n8k16(x[nt], lo, qf[nt][4 * i], qf[nt][4 * i + 1]);
-            mma_m16n8k16(x[nt], hi, qf[nt][4 * i + 2], qf[nt][4 * i + 3]);
+            mma_m16n8k16(x[h][nt], lo, qf[nt][4 * i], qf[nt][4 * i + 1]);
+            mma_m16n8k16(x[h][nt], hi, qf[nt][4 * i + 2], qf[nt][4 * i + 3]);
           }
         }
       }
       // ---- weights
-      const int limit = ((absent >> slot) & 1) ? 0 : len - st * 16;    // tokens of this step that exist
-      float ls[2], rs[2], zc[2];
+      float rs[2][2], rz[2][2];
       bool over = false;
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const int t = tok_a + 8 * r;
-        const uint32_t km = kva_lds32(ss + t * 4), vm = kva_lds32(ss + 64 + t * 4);
-        const float2 kf = __half22float2(*reinterpret_cast<const __half2*>(&km));
-        const float2 vf = __half22float2(*reinterpret_cast<const __half2*>(&vm));
-        const bool real = t < limit;
-        const float m = fmaf(8.f, kf.x, kf.y);
-        const float vs = real ? fmaxf(vf.x, 5.9604645e-8f) : 1.f;
-        ls[r] = real ? __log2f(vs) : -INFINITY;
-        rs[r] = __fdividef(1.f, vs);
-        zc[r] = real ? fmaf(8.f, vf.x, vf.y) : 0.f;
+      for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+        for (int r = 0; r < 2; ++r) {
+          const int t = 16 * h + tok_a + 8 * r;
+          const uint4 w = lds128(meta + t * 16);
+          const float s = __uint_as_float(w.x), m = __uint_as_float(w.y), ls = __uint_as_float(w.z);
+          rs[h][r] = __uint_as_float(w.w);
+          rz[h][r] = __uint_as_float(kva_lds32(meta + kStep * 16 + t * 4));
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            float y = fmaf(x[nt][2 * r + e] * kf.x, f[nt][e], m * fq[nt][e]) + ls[r];
-            y = real ? y : -INFINITY;
-            x[nt][2 * r + e] = y;
-            over |= y > M[nt][e] + 8.f;
-          }
-      }
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const float y = fmaf(x[h][nt][2 * r + e] * s, f[nt][e], fmaf(m, fq[nt][e], ls));
+              x[h][nt][2 * r + e] = y;
+              over |= y > M[nt][e] + 8.f;
+            }
+        }
       if (__any_sync(~0u, over)) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            float top = fmaxf(x[nt][e], x[nt][2 + e]);
+            float top = fmaxf(fmaxf(x[0][nt][e], x[0][nt][2 + e]), fmaxf(x[1][nt][e], x[1][nt][2 + e]));
 #pragma unroll
             for (int s = 4; s < 32; s <<= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, s));
             top = fmaxf(top, M[nt][e]);
@@ -332,24 +391,25 @@ __global__ void __launch_bounds__(kva::kThreads, NT == 1 ? 4 : 2) kv4_attention_
             for (int i = 0; i < MT; ++i) { o[nt][i][e] *= k; o[nt][i][2 + e] *= k; }
           }
       }
-      uint32_t pb[NT][2];
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          float w[2];
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            w[e] = kva_exp2(x[nt][2 * r + e] - M[nt][e]);
-            const float l = w[e] * rs[r];
-            L[nt][e] += l;
-            Z[nt][e] = fmaf(l, zc[r], Z[nt][e]);
-          }
-          const __half2 h2 = __floats2half2_rn(w[0], w[1]);
-          pb[nt][r] = kva_transpose(*reinterpret_cast<const uint32_t*>(&h2));
-        }
       // ---- weighted sums of the codes
-      {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        uint32_t pb[NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            float w[2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              w[e] = kva_exp2(x[h][nt][2 * r + e] - M[nt][e]);
+              L[nt][e] = fmaf(w[e], rs[h][r], L[nt][e]);
+              Z[nt][e] = fmaf(w[e], rz[h][r], Z[nt][e]);
+            }
+            const __half2 h2 = __floats2half2_rn(w[0], w[1]);
+            pb[nt][r] = kva_transpose(*reinterpret_cast<const uint32_t*>(&h2));
+          }
+        const uint32_t sv = slot + (2 + h) * CODEB;
         uint32_t u[4][DP / 64];                 // tokens c, 7 - c, 8 + c, 15 - c: this lane's words
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -361,47 +421,31 @@ __global__ void __launch_bounds__(kva::kThreads, NT == 1 ? 4 : 2) kv4_attention_
             u[j][0] = kva_lds32(sv + t * ROWB + g * 4);
           }
         }
+        // row g of tile n: nibble n of one word (DP 128: word 2g, channel 16 g + n; DP 64: word g, channel 8 g + n), row g + 8:
+        // of another (word 2g + 1, channel 16 g + 8 + n) or the word's upper half (channel 8 g + 4 + n)
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {  // nibbles 0-3, 4-7 of the words
-          const uint32_t sel = half ? 0x7632 : 0x5410;
-          uint32_t w[2][DP / 64];
+        for (int q4 = 0; q4 < MT / 4; ++q4) {   // tiles 4 q4 .. 4 q4 + 3
+          constexpr int k1 = DP / 64 - 1;
+          const uint32_t sel = q4 ? 0x7632 : 0x5410, sel1 = DP == 128 ? sel : 0x7632;
+          const uint32_t w[4] = {__byte_perm(u[0][0], u[1][0], sel), __byte_perm(u[0][k1], u[1][k1], sel1),
+                                 __byte_perm(u[2][0], u[3][0], sel), __byte_perm(u[2][k1], u[3][k1], sel1)};
+          uint32_t a[4][4];
 #pragma unroll
-          for (int k = 0; k < DP / 64; ++k) {
-            w[0][k] = __byte_perm(u[0][k], u[1][k], sel);
-            w[1][k] = __byte_perm(u[2][k], u[3][k], sel);
+          for (int k = 0; k < 4; ++k) {
+            const uint32_t w8 = w[k] >> 8;
+            a[0][k] = kv4_pair(w[k], 0x64086408u);
+            a[1][k] = kv4_pair_hi(w[k], 0xd480d480u);
+            a[2][k] = kv4_pair(w8, 0x64086408u);
+            a[3][k] = kv4_pair_hi(w8, 0xd480d480u);
           }
-          if (DP == 128) {
-            // row g: channel 16 g + n of word 2g, row g + 8: channel 16 g + 8 + n of word 2g + 1
-            constexpr int k1 = DP / 64 - 1;
-            const uint32_t s00 = w[0][0] >> 8, s01 = w[0][k1] >> 8, s10 = w[1][0] >> 8, s11 = w[1][k1] >> 8;
-            const uint32_t a[4][4] = {
-                {kv4_pair(w[0][0], 0x64086408u), kv4_pair(w[0][k1], 0x64086408u), kv4_pair(w[1][0], 0x64086408u), kv4_pair(w[1][k1], 0x64086408u)},
-                {kv4_pair_hi(w[0][0], 0xd480d480u), kv4_pair_hi(w[0][k1], 0xd480d480u), kv4_pair_hi(w[1][0], 0xd480d480u), kv4_pair_hi(w[1][k1], 0xd480d480u)},
-                {kv4_pair(s00, 0x64086408u), kv4_pair(s01, 0x64086408u), kv4_pair(s10, 0x64086408u), kv4_pair(s11, 0x64086408u)},
-                {kv4_pair_hi(s00, 0xd480d480u), kv4_pair_hi(s01, 0xd480d480u), kv4_pair_hi(s10, 0xd480d480u), kv4_pair_hi(s11, 0xd480d480u)}};
 #pragma unroll
-            for (int n = 0; n < 4; ++n)
+          for (int n = 0; n < 4; ++n)
 #pragma unroll
-              for (int nt = 0; nt < NT; ++nt) mma_m16n8k16(o[nt][4 * half % MT + n], a[n], pb[nt][0], pb[nt][1]);
-          } else if (half == 0) {
-            // row g: channel 8 g + n, row g + 8: channel 8 g + 4 + n of word g
-            const uint32_t h0 = __byte_perm(u[0][0], u[1][0], 0x7632), h1 = __byte_perm(u[2][0], u[3][0], 0x7632);
-            const uint32_t l0 = w[0][0], l1 = w[1][0];
-            const uint32_t l08 = l0 >> 8, l18 = l1 >> 8, h08 = h0 >> 8, h18 = h1 >> 8;
-            const uint32_t a[4][4] = {
-                {kv4_pair(l0, 0x64086408u), kv4_pair(h0, 0x64086408u), kv4_pair(l1, 0x64086408u), kv4_pair(h1, 0x64086408u)},
-                {kv4_pair_hi(l0, 0xd480d480u), kv4_pair_hi(h0, 0xd480d480u), kv4_pair_hi(l1, 0xd480d480u), kv4_pair_hi(h1, 0xd480d480u)},
-                {kv4_pair(l08, 0x64086408u), kv4_pair(h08, 0x64086408u), kv4_pair(l18, 0x64086408u), kv4_pair(h18, 0x64086408u)},
-                {kv4_pair_hi(l08, 0xd480d480u), kv4_pair_hi(h08, 0xd480d480u), kv4_pair_hi(l18, 0xd480d480u), kv4_pair_hi(h18, 0xd480d480u)}};
-#pragma unroll
-            for (int n = 0; n < 4; ++n)
-#pragma unroll
-              for (int nt = 0; nt < NT; ++nt) mma_m16n8k16(o[nt][n], a[n], pb[nt][0], pb[nt][1]);
-          }
+            for (int nt = 0; nt < NT; ++nt) mma_m16n8k16(o[nt][4 * q4 + n], a[n], pb[nt][0], pb[nt][1]);
         }
       }
       __syncwarp();                             // the slot's words are in registers of the whole warp before it is refilled
-      slot = slot + 1 == kStages ? 0 : slot + 1;
+      slot = slot == ring + (kStages - 1) * STAGEB ? ring : slot + STAGEB;
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
 
@@ -431,12 +475,11 @@ __global__ void __launch_bounds__(kva::kThreads, NT == 1 ? 4 : 2) kv4_attention_
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int h = nt * 8 + 2 * c + (e & 1);
-          // DP 128: tile i = nibble i, rows 16 g + i and 16 g + 8 + i; DP 64: rows 8 g + i and 8 g + 4 + i
           const int d = DP == 128 ? 16 * g + i + ((e & 2) ? 8 : 0) : 8 * g + i + ((e & 2) ? 4 : 0);
-          ex[(warp * H + h) * DP + d] = o[nt][i][e];
+          if (h < nh) ex[(warp * H + h) * DP + d] = o[nt][i][e];
         }
     __syncthreads();
-    const bool whole = t0 == 0 && t1 == tiles;
+    const bool whole = t0 == 0 && t1 == steps;
     // parts of a list sit in the slots of their CTAs: 2 cta + 1 if the list begins in the CTA's range, else 2 cta
     const int my_slot = 2 * (int)blockIdx.x + (t0 == 0 ? 1 : 0);
     for (int i = tid; i < nh * DP; i += kThreads) {
@@ -460,28 +503,56 @@ __global__ void __launch_bounds__(kva::kThreads, NT == 1 ? 4 : 2) kv4_attention_
       }
     }
     if (!whole) {
-      // CTAs of this list: the ones whose ranges hold its first and its last tile
-      const long long last_tile = list_begin + tiles - 1;
-      const int c0 = (int)(((list_begin + 1) * ctas - 1) / N), c1 = (int)(((last_tile + 1) * ctas - 1) / N);
+      // CTAs of this list: the ones whose ranges hold its first and its last step
+      const int c0 = (int)(((list_begin + 1) * ctas - 1) / N), c1 = (int)(((list_begin + steps) * ctas - 1) / N);
       __threadfence();
       __syncthreads();
       if (tid == 0) s_last = atomicAdd(p.tickets + c0, 1) == c1 - c0;
       __syncthreads();
       if (s_last) {
         __threadfence();
-        for (int i = tid; i < nh * DP; i += kThreads) {
-          const int h = i / DP, d = i - h * DP;
-          if (d >= p.dv) continue;
+        // a warp per head: lanes hold the parts' M and L, 32 at a time, then every lane adds up its channels part by part
+        for (int h = warp; h < nh; h += kWarps) {
+          auto part = [&](int k) { return p.part + ((size_t)(2 * k + (k == c0)) * H + h) * PSTR; };
           float top = kFloor;
-          for (int k = c0; k <= c1; ++k) top = fmaxf(top, __ldcg(p.part + ((size_t)(2 * k + (k == c0)) * H + h) * PSTR + DP));
-          float acc = 0.f, l = 0.f;
-          for (int k = c0; k <= c1; ++k) {
-            const float* src = p.part + ((size_t)(2 * k + (k == c0)) * H + h) * PSTR;
-            const float w = kva_exp2(__ldcg(src + DP) - top);
-            acc = fmaf(w, __ldcg(src + d), acc);
-            l = fmaf(w, __ldcg(src + DP + 1), l);
+          for (int k = c0 + lane; k <= c1; k += 32) top = fmaxf(top, __ldcg(part(k) + DP));
+#pragma unroll
+          for (int s = 16; s; s >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, s));
+          float acc[DP / 32], l = 0.f;
+#pragma unroll
+          for (int e = 0; e < DP / 32; ++e) acc[e] = 0.f;
+          for (int k0 = c0; k0 <= c1; k0 += 32) {
+            float w = 0.f, lw = 0.f;
+            if (k0 + lane <= c1) {
+              w = kva_exp2(__ldcg(part(k0 + lane) + DP) - top);
+              lw = w * __ldcg(part(k0 + lane) + DP + 1);
+            }
+#pragma unroll
+            for (int s = 16; s; s >>= 1) lw += __shfl_xor_sync(~0u, lw, s);
+            l += lw;
+            const int n = min(32, c1 - k0 + 1);
+#pragma unroll 8
+            for (int k = 0; k < n; ++k) {
+              const float wk = __shfl_sync(~0u, w, k);
+              const float* src = part(k0 + k) + lane * (DP / 32);
+              if (DP == 128) {
+                const float4 v = __ldcg(reinterpret_cast<const float4*>(src));
+                acc[0] = fmaf(wk, v.x, acc[0]);
+                acc[1] = fmaf(wk, v.y, acc[1]);
+                acc[DP / 32 - 2] = fmaf(wk, v.z, acc[DP / 32 - 2]);
+                acc[DP / 32 - 1] = fmaf(wk, v.w, acc[DP / 32 - 1]);
+              } else {
+                const float2 v = __ldcg(reinterpret_cast<const float2*>(src));
+                acc[0] = fmaf(wk, v.x, acc[0]);
+                acc[1] = fmaf(wk, v.y, acc[1]);
+              }
+            }
           }
-          kva_store(p.out, ((int64_t)b * p.heads + head0 + h) * p.dv + d, p.bf16, l == 0.f ? 0.f : acc / l);
+#pragma unroll
+          for (int e = 0; e < DP / 32; ++e) {
+            const int d = lane * (DP / 32) + e;
+            if (d < p.dv) kva_store(p.out, ((int64_t)b * p.heads + head0 + h) * p.dv + d, p.bf16, l == 0.f ? 0.f : acc[e] / l);
+          }
         }
         if (tid == 0) p.tickets[c0] = 0;
       }
@@ -493,13 +564,13 @@ __global__ void __launch_bounds__(kva::kThreads, NT == 1 ? 4 : 2) kv4_attention_
 
 template <int DP, int NT>
 static constexpr size_t kva_smem() {
-  const size_t ring = (size_t)kva::kWarps * kva::kStages * (16 * DP + 128);
+  const size_t ring = (size_t)kva::kWarps * (kva::kStages * (32 * DP + 256) + kva::kStep * 20);
   const size_t ex = (size_t)kva::kWarps * 8 * NT * DP * 4;
   return ring > ex ? ring : ex;
 }
 
 static int kva_ctas(int nt) {
-  const int n = device_info().sm_count * (nt == 1 ? 4 : 2);
+  const int n = device_info().sm_count * kva::per_sm(nt);
   return n < kva::kMaxCtas ? n : kva::kMaxCtas;
 }
 static int kva_nt(int64_t heads, int64_t kv_heads) { return heads / kv_heads > 8 ? 2 : 1; }
@@ -523,7 +594,7 @@ extern "C" size_t uniql_kv4_attention_scratch_bytes(int64_t batch, int64_t heads
   using namespace uniql;
   if (batch <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || (dp != 64 && dp != 128)) return 0;
   const int nt = kva_nt(heads, kv_heads);
-  return UNIQL_SCRATCH_COUNTER_BYTES + (size_t)2 * kva_ctas(nt) * 8 * nt * (dp + 2) * sizeof(float);
+  return UNIQL_SCRATCH_COUNTER_BYTES + (size_t)2 * kva_ctas(nt) * 8 * nt * (dp + 4) * sizeof(float);
 }
 
 extern "C" int uniql_kv4_attention(const void* q, int64_t q_batch_stride, int64_t q_head_stride, const void* codes,
@@ -556,6 +627,7 @@ extern "C" int uniql_kv4_attention(const void* q, int64_t q_batch_stride, int64_
   p.hgroups = (p.group + 8 * nt - 1) / (8 * nt);
   p.max_blocks = (int)max_blocks; p.num_pages = (int)num_pages; p.page_shift = page_shift_of(page_size);
   p.dk = (int)dk; p.dv = (int)dv; p.bf16 = dtype == UNIQL_BF16;
+  p.q_vec = aligned16(q) && !((q_batch_stride | q_head_stride) & 7);
   p.scale_log2 = softmax_scale * 1.44269504088896340736f;
   cudaStream_t s = (cudaStream_t)stream;
   if (dp == 128) return nt == 1 ? kva_launch<128, 1>(p, s) : kva_launch<128, 2>(p, s);
