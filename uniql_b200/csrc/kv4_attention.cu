@@ -168,8 +168,11 @@ __global__ void __launch_bounds__(kva::kThreads, kva::per_sm(NT)) kv4_attention_
   const uint32_t ring = smem_addr(smem) + warp * WARPB, meta = ring + RINGB;
   const int tok_a = kva_token(g);               // rows g and g + 8 of the first product: tokens tok_a and 8 + tok_a
   const int pmask = (1 << p.page_shift) - 1;
-  const int64_t page_codes = ((int64_t)2 * p.kv_heads * ROWB) << p.page_shift, v_codes = page_codes / 2;
-  const int64_t page_scales = ((int64_t)8 * p.kv_heads) << p.page_shift;
+  // bytes of a page (at most 2^25) and from its K to its V
+  const uint32_t page_codes = (uint32_t)(2 * p.kv_heads * ROWB) << p.page_shift, v_codes = page_codes / 2;
+  const uint32_t page_scales = (uint32_t)(8 * p.kv_heads) << p.page_shift;
+  // where a lane's 16-byte chunk of packed words goes: chunk of token t = lane / 4 moves to chunk ^ (t & 2)
+  const uint32_t lane_dst = DP == 128 ? (lane * 16) ^ ((lane & 8) << 2) : lane * 16;
   bool bad_page = false;
 
   for (long long cur = begin; cur < end;) {
@@ -190,7 +193,7 @@ __global__ void __launch_bounds__(kva::kThreads, kva::per_sm(NT)) kv4_attention_
     const int nh = min(H, p.group - hg * H);
     cur += t1 - t0;
 
-    // ---- producer: 32 tokens into a ring slot, 16 at a time (a page holds at least 16)
+    // ---- producer: 32 tokens into a ring slot.  A page of 16 holds half a step; larger ones hold whole steps
     const int first = t0 + warp;                                // this warp's steps: first, first + kWarps, .. < t1
     const int32_t* trow = p.table + (size_t)b * p.ld_table;
     const unsigned char* kbase = p.codes + (((int64_t)kvh * ROWB) << p.page_shift) + lane * 16;
@@ -198,31 +201,33 @@ __global__ void __launch_bounds__(kva::kThreads, kva::per_sm(NT)) kv4_attention_
     const int last_block = (len - 1) >> p.page_shift;
     int page0 = 0, page1 = 0;                                   // of the step that is produced next
     auto look = [&](int st) {
-      page0 = trow[min(st * kStep >> p.page_shift, last_block)];
-      page1 = trow[min((st * kStep + 16) >> p.page_shift, last_block)];
+      page0 = trow[st * kStep >> p.page_shift];
+      if (p.page_shift == 4) page1 = trow[min(2 * st + 1, last_block)];
     };
     if (first < t1) look(first);
     auto produce = [&](int st, uint32_t dst) {
       if (st < t1) {
-        int page[2] = {page0, page1};
+        int pg0 = page0, pg1 = p.page_shift == 4 ? page1 : page0;
         if (st + kWarps < t1) look(st + kWarps);
+        const bool ok0 = (unsigned)pg0 < (unsigned)p.num_pages, ok1 = (unsigned)pg1 < (unsigned)p.num_pages;
+        if (!ok0) pg0 = 0;                                      // an absent page: copies of no bytes, zeros in the ring
+        if (!ok1) pg1 = 0;
+        bad_page |= !(ok0 && ok1);
+        const uint32_t at = (st * kStep) & pmask;
+        const unsigned char* src0 = kbase + (uint64_t)pg0 * page_codes + at * ROWB;
+        // the second half is the next 16 rows, or the first 16 of the next page
+        const unsigned char* src1 = p.page_shift == 4 ? kbase + (uint64_t)pg1 * page_codes : src0 + CODEB;
+        const uint32_t d = dst + lane_dst;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const bool ok = (unsigned)page[h] < (unsigned)p.num_pages;
-          bad_page |= !ok;
-          const int at = (st * kStep + 16 * h) & pmask;
-          // an absent page copies nothing, from an address that exists
-          const unsigned char* src = ok ? kbase + page[h] * page_codes + at * ROWB : (const unsigned char*)p.part;
-          const unsigned char* vsrc = ok ? src + v_codes : src;
-#pragma unroll
-          for (int i = 0; i < CODEB / 512; ++i) {
-            const int ch = lane + 32 * i;                       // 16-byte chunk of the half
-            uint32_t d = dst + h * CODEB + ch * 16;
-            if (DP == 128) d = dst + h * CODEB + ((ch * 16) ^ (((ch >> 3) & 1) << 5));   // chunk of token t = ch / 4 moves to chunk ^ (t & 2)
-            kva_cp16(d, src + i * 512, ok);
-            kva_cp16(d + 2 * CODEB, vsrc + i * 512, ok);
-          }
-          if ((lane >> 3) == h) kva_cp16(dst + OFF_SC + lane * 16, ok ? sbase + page[h] * page_scales + at * 4 : (const unsigned char*)p.part, ok);
+        for (int i = 0; i < CODEB / 512; ++i) {
+          kva_cp16(d + 512 * i, src0 + 512 * i, ok0);
+          kva_cp16(d + 512 * i + CODEB, src1 + 512 * i, ok1);
+          kva_cp16(d + 512 * i + 2 * CODEB, src0 + v_codes + 512 * i, ok0);
+          kva_cp16(d + 512 * i + 3 * CODEB, src1 + v_codes + 512 * i, ok1);
+        }
+        if (lane < 16) {                                        // 64 bytes of K scales, 64 of V scales, twice
+          const uint32_t row = p.page_shift == 4 ? 0u : at + (lane & 8) * 2;
+          kva_cp16(dst + OFF_SC + lane * 16, sbase + (uint64_t)(lane < 8 ? pg0 : pg1) * page_scales + row * 4, lane < 8 ? ok0 : ok1);
         }
       }
       asm volatile("cp.async.commit_group;" ::: "memory");
@@ -323,9 +328,11 @@ __global__ void __launch_bounds__(kva::kThreads, kva::per_sm(NT)) kv4_attention_
       float x[2][NT][4];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
+        float x2[NT][4];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
           x[h][nt][0] = x[h][nt][1] = x[h][nt][2] = x[h][nt][3] = 0.f;
+          x2[nt][0] = x2[nt][1] = x2[nt][2] = x2[nt][3] = 0.f;  // a second chain of sums: half the latency
         }
         uint32_t wa[KS], wb[KS];
         if (DP == 128) {
@@ -349,9 +356,13 @@ __global__ void __launch_bounds__(kva::kThreads, kva::per_sm(NT)) kv4_attention_
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
             mma_m16n8k16(x[h][nt], lo, qf[nt][4 * i], qf[nt][4 * i + 1]);
-            mma_m16n8k16(x[h][nt], hi, qf[nt][4 * i + 2], qf[nt][4 * i + 3]);
+            mma_m16n8k16(x2[nt], hi, qf[nt][4 * i + 2], qf[nt][4 * i + 3]);
           }
         }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[h][nt][e] += x2[nt][e];
       }
       // ---- weights
       float rs[2][2], rz[2][2];
@@ -619,7 +630,8 @@ extern "C" int uniql_kv4_attention(const void* q, int64_t q_batch_stride, int64_
     return UNIQL_ESCRATCH;
   KvaParams p;
   p.q = (const unsigned char*)q; p.q_bs = q_batch_stride; p.q_hs = q_head_stride;
-  p.codes = (const unsigned char*)codes; p.scales = (const unsigned char*)scales;
+  // without pages every copy is of no bytes, but from an address that exists
+  p.codes = (const unsigned char*)(num_pages ? codes : scratch); p.scales = (const unsigned char*)(num_pages ? scales : scratch);
   p.table = block_table; p.ld_table = ld_table; p.lens = lens; p.out = (unsigned char*)out;
   p.tickets = (int*)scratch; p.part = (float*)((char*)scratch + UNIQL_SCRATCH_COUNTER_BYTES); p.status_word = status_word;
   const int nt = kva_nt(heads, kv_heads);
