@@ -7,11 +7,12 @@ namespace uniql {
 
 // ------------------------------------------------------------------------------------------------ page plan
 // need_i = ceil((len_i + new_i) / P) - ceil(len_i / P), cut at the width of the table; the exclusive sums of need and new
-// say which entries of the free stack and which places of the packed tokens a request owns.  Every CTA of one cluster
-// computes both sums for the whole batch (8 bytes a request from L2) and keeps them in shared memory; the new pages and
-// the new tokens are then flat lists that all threads walk, each finding its request by bisection, so that one prompt of
-// thousands of tokens costs no more than thousands of single ones.  lens and free_count may be overwritten in place: that
-// is done behind a cluster barrier, when every CTA has read them.
+// say which entries of the free stack and which places of the packed tokens a request owns.  Every CTA computes both sums
+// for the whole batch (8 bytes a request from L2) and keeps them in shared memory; the new pages and the new tokens are then
+// flat lists that all threads walk, each finding its request by bisection, so that one prompt of thousands of tokens costs no
+// more than thousands of single ones.  lens and free_count may be overwritten in place, so what goes there waits for every CTA's
+// reads: up to 8 CTAs are one cluster with a barrier; a step of more tokens than those have threads for takes a grid over the
+// GPU and a second launch of one CTA (257328 tokens of 1024 requests: 35 us in one cluster, 9.5 as grid and second launch).
 constexpr int kPlanThreads = 1024, kPlanCap = 1 << 30;
 
 struct PlanParams {
@@ -29,6 +30,7 @@ struct PlanParams {
   int* status_word;
   int64_t total_new;
   int batch, max_blocks, free_cap, page_shift;
+  int lists, totals;                            // what this launch does: pages and tokens; lengths, starts and count
 };
 
 // largest i with start[i] <= x, for start[0] = 0 <= x
@@ -107,6 +109,7 @@ __global__ void __launch_bounds__(kPlanThreads) kv_page_plan_kernel(const __grid
   }
   const int tokens = s_cu[p.batch], pages = s_first[p.batch], count = s_count;
   const int rank = blockIdx.x, ranks = gridDim.x, step = ranks * kPlanThreads;
+  if (p.lists) {
   for (int x = rank * kPlanThreads + tid; x < pages; x += step) {
     const int i = plan_find(s_first, p.batch, x);
     const int had = (s_len[i] + pmask) >> p.page_shift;
@@ -132,6 +135,8 @@ __global__ void __launch_bounds__(kPlanThreads) kv_page_plan_kernel(const __grid
   }
   if ((short_table || (rank == 0 && tid == 0 && (pages > count || tokens > p.total_new))) && p.status_word)
     atomicOr(p.status_word, UNIQL_STATUS_NO_PAGE);
+  }
+  if (!p.totals) return;
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
   if (rank == 0) {
@@ -144,34 +149,19 @@ __global__ void __launch_bounds__(kPlanThreads) kv_page_plan_kernel(const __grid
 }
 
 // ------------------------------------------------------------------------------------------------ append
-// A row (one token, one head, K or V) is DP / 8 lanes with eight channels each: one 16-byte load, four shuffles for the
-// extremes, one packed word stored.  HBM-bound by the reads: 4 bytes a channel against 0.5 written.
-__device__ __forceinline__ void kv4_load8(const void* src, int bf16, float (&x)[8]) {
-  const uint4 w = *reinterpret_cast<const uint4*>(src);
-  const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    float2 f;
-    if (bf16) f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&u[e]));
-    else f = __half22float2(*reinterpret_cast<const __half2*>(&u[e]));
-    x[2 * e] = f.x;
-    x[2 * e + 1] = f.y;
-  }
-}
-
-// Nearest code to (x - z) / s, ties to even.  The product with 1 / s is within 3 * 2^-24 of the quotient (relative); where
-// that leaves the side of a half-way point open the two sides are compared exactly: x - z spans at most 41 bits and
-// (k + 1/2) * s sixteen, both exact in fp64.
-__device__ __forceinline__ uint32_t kv4_code(float x, float z, float s, float inv) {
-  const float y = fminf(fmaxf((x - z) * inv, 0.f), 15.f);
-  const float k = floorf(y);
-  const float frac = y - k;
-  if (fabsf(frac - 0.5f) < 1e-4f) {
-    const double d = (double)x - (double)z, mid = ((double)k + 0.5) * (double)s;
-    const int ki = (int)k;
-    return (uint32_t)(d > mid || (d == mid && (ki & 1)) ? ki + 1 : ki);
-  }
-  return (uint32_t)__float2int_rn(y);
+// A row (one token, one head, K or V) is DP / 8 lanes with eight channels each: one 16-byte load, the extremes over the lanes
+// (least value and negated greatest one as a 16-bit pair: one shuffle a level), one packed word stored.  HBM-bound by the
+// reads, 4 bytes a channel against 0.5 written, if the instructions are few: the packed minimum carries NaN along, the codes
+// are rounded by adding 1.5 * 2^23 and joined as the low bits of those sums.
+//
+// Codes.  y = (x - z) * (1 / s) is within 3 * 2^-24 of the quotient (relative).  Where that leaves the side of a half-way point
+// open, the two sides are compared exactly: x - z spans at most 41 bits and (k + 1/2) * s sixteen, both exact in fp64.
+constexpr float kRound = 12582912.f;            // 1.5 * 2^23
+__device__ __noinline__ uint32_t kv4_exact_code(float x, float z, float s, float y) {
+  const float k = floorf(fminf(fmaxf(y, 0.f), 15.f));
+  const double d = (double)x - (double)z, mid = ((double)k + 0.5) * (double)s;
+  const int ki = (int)k;
+  return (uint32_t)min(d > mid || (d == mid && (ki & 1)) ? ki + 1 : ki, 15);
 }
 
 struct AppendParams {
@@ -181,68 +171,120 @@ struct AppendParams {
   uint32_t* codes;
   __half2* scales;
   int* status_word;
-  int64_t tokens, num_slots;
-  int heads, d[2], bf16, page_shift;
+  int64_t num_slots;
+  uint32_t rows;                                // tokens * 2 * heads, below 2^31
+  FastDiv heads;
+  int d[2], page_shift;
 };
 
 constexpr int kAppendThreads = 256;
 
-template <int DP>
+template <bool BF16>
+struct Pair16 {
+  using T = __half2;
+};
+template <>
+struct Pair16<true> {
+  using T = __nv_bfloat162;
+};
+
+template <int DP, bool BF16>
 __global__ void __launch_bounds__(kAppendThreads) kv4_append_kernel(const __grid_constant__ AppendParams p) {
   constexpr int W = DP / 8;                     // lanes of a row
+  using T2 = typename Pair16<BF16>::T;
   pdl_wait();
   pdl_launch_dependents();
   const int sub = threadIdx.x % W;
-  const int64_t rows = p.tokens * 2 * p.heads;
-  const int64_t step = (int64_t)gridDim.x * (kAppendThreads / W);
-  const int pmask = (1 << p.page_shift) - 1;
-  // all lanes of a warp stay in the loop together: the shuffles below name the whole warp
-  const int64_t first = (int64_t)blockIdx.x * (kAppendThreads / W) + threadIdx.x / W;
-  const int64_t warp_first = first - (threadIdx.x % 32) / W;
-  for (int64_t r = first, wr = warp_first; wr < rows; r += step, wr += step) {
-    const bool live = r < rows;
-    const int64_t pair = live ? r / p.heads : 0;
-    const int h = live ? (int)(r - pair * p.heads) : 0, kv = (int)(pair & 1);
-    const int64_t t = pair >> 1;
+  const uint32_t step = gridDim.x * (kAppendThreads / W);
+  // the lanes of a warp stay in the loop together: the shuffles below name the whole warp
+  const uint32_t first = blockIdx.x * (kAppendThreads / W) + threadIdx.x / W, ahead = (threadIdx.x % 32) / W;
+  for (uint32_t r = first; r - ahead < p.rows; r += step) {
+    const bool live = r < p.rows;
+    const uint32_t pair = live ? p.heads.quot(r) : 0, h = live ? r - pair * p.heads.d : 0, t = pair >> 1;
+    const int kv = pair & 1;
     const int64_t slot = live ? p.slots[t] : -1;
     const bool stored = slot >= 0 && slot < p.num_slots;
-    const bool mine = stored && sub * 8 < p.d[kv];
-    float x[8];
+    const bool mine = stored && sub * 8 < (kv ? p.d[1] : p.d[0]);
+    uint4 raw = make_uint4(0, 0, 0, 0);
     if (mine)
-      kv4_load8(p.src[kv] + 2 * (t * p.token_stride[kv] + h * p.head_stride[kv] + sub * 8), p.bf16, x);
-    float lo = 65504.f, hi = -65504.f;
-    bool nan = false;
-    if (mine) {
+      raw = *reinterpret_cast<const uint4*>((kv ? p.src[1] : p.src[0]) +
+                                            2 * (t * (kv ? p.token_stride[1] : p.token_stride[0]) + h * (kv ? p.head_stride[1] : p.head_stride[0]) + sub * 8));
+    const uint32_t u[4] = {raw.x, raw.y, raw.z, raw.w};
+    // (least, -greatest) of the row; lanes without channels hold infinities
+    T2 least = *reinterpret_cast<const T2*>(&u[0]), most = least;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        nan |= x[e] != x[e];
-        x[e] = fminf(fmaxf(x[e], -65504.f), 65504.f);
-        lo = fminf(lo, x[e]);
-        hi = fmaxf(hi, x[e]);
-      }
+    for (int e = 1; e < 4; ++e) {
+      least = __hmin2_nan(least, *reinterpret_cast<const T2*>(&u[e]));
+      most = __hmax2_nan(most, *reinterpret_cast<const T2*>(&u[e]));
     }
-    unsigned bad = nan;
+    T2 ends;
+    ends.x = __hmin_nan(least.x, least.y);
+    ends.y = __hneg(__hmax_nan(most.x, most.y));
+    uint32_t eb = mine ? *reinterpret_cast<const uint32_t*>(&ends) : (BF16 ? 0x7f807f80u : 0x7c007c00u);
 #pragma unroll
     for (int o = W / 2; o; o >>= 1) {
-      lo = fminf(lo, __shfl_xor_sync(~0u, lo, o));
-      hi = fmaxf(hi, __shfl_xor_sync(~0u, hi, o));
-      bad |= __shfl_xor_sync(~0u, bad, o);
+      const uint32_t other = __shfl_xor_sync(~0u, eb, o);
+      ends = __hmin2_nan(*reinterpret_cast<const T2*>(&eb), *reinterpret_cast<const T2*>(&other));
+      eb = *reinterpret_cast<const uint32_t*>(&ends);
     }
+    ends = *reinterpret_cast<const T2*>(&eb);
+    float lo, hi;
+    if constexpr (BF16) {
+      lo = __bfloat162float(ends.x);
+      hi = -__bfloat162float(ends.y);
+    } else {
+      lo = __half2float(ends.x);
+      hi = -__half2float(ends.y);
+    }
+    const bool nan = lo != lo || hi != hi, wide = lo < -65504.f || hi > 65504.f;
+    lo = fminf(fmaxf(lo, -65504.f), 65504.f);
+    hi = fminf(fmaxf(hi, -65504.f), 65504.f);
     __half sh = __float2half_rn(__fdiv_rn(hi - lo, 15.f));
     if (__half2float(sh) < 5.9604645e-8f) sh = __ushort_as_half(1);      // 2^-24: a scale is never zero
     __half zh = __float2half_rn(lo);
     const float s = __half2float(sh), z = __half2float(zh), inv = __frcp_rn(s);
     uint32_t word = 0;
-    if (mine && !bad) {
+    if (mine && !nan) {
+      float x[8], y[8], far = 0.f;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) word |= kv4_code(x[e], z, s, inv) << (4 * e);
+      for (int e = 0; e < 4; ++e) {
+        float2 f;
+        if constexpr (BF16) f = __bfloat1622float2(*reinterpret_cast<const T2*>(&u[e]));
+        else f = __half22float2(*reinterpret_cast<const T2*>(&u[e]));
+        x[2 * e] = f.x;
+        x[2 * e + 1] = f.y;
+      }
+      if (wide) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = fminf(fmaxf(x[e], -65504.f), 65504.f);
+      }
+      constexpr uint32_t kBits = 0x4b400000u;   // of kRound; what eight of them add to the word:
+      constexpr uint32_t kAll = kBits + (kBits << 4) + (kBits << 8) + (kBits << 12) + (kBits << 16) + (kBits << 20) + (kBits << 24) + (kBits << 28);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        y[e] = fminf(fmaxf((x[e] - z) * inv, 0.f), 15.f);
+        const float up = y[e] + kRound;
+        far = fmaxf(far, fabsf(y[e] - (up - kRound)));
+        word += __float_as_uint(up) << (4 * e);
+      }
+      word -= kAll;
+      if (far > 0.49998f) {                     // some quotient within 2e-5 of a half-way point
+        word = 0;
+#pragma unroll 1
+        for (int e = 0; e < 8; ++e) {
+          float xe = BF16 ? __uint_as_float((e & 1) ? u[e >> 1] & 0xffff0000u : u[e >> 1] << 16)
+                                : __half2float(__ushort_as_half((unsigned short)(u[e >> 1] >> (16 * (e & 1)))));
+          xe = fminf(fmaxf(xe, -65504.f), 65504.f);
+          word |= kv4_exact_code(xe, z, s, (xe - z) * inv) << (4 * e);
+        }
+      }
     }
     if (stored) {
       const int64_t page = slot >> p.page_shift;
-      const int64_t row = ((page * 2 + kv) * p.heads + h) * (pmask + 1) + (slot & pmask);
+      const int64_t row = (((page * 2 + kv) * p.heads.d + h) << p.page_shift) + (slot & ((1 << p.page_shift) - 1));
       p.codes[row * W + sub] = word;
       if (sub == 0) {
-        if (bad) sh = zh = __ushort_as_half(0x7fff);
+        if (nan) sh = zh = __ushort_as_half(0x7fff);
         p.scales[row] = __halves2half2(sh, zh);
       }
     } else if (live && slot != -1 && sub == 0 && p.status_word) {
@@ -253,9 +295,9 @@ __global__ void __launch_bounds__(kAppendThreads) kv4_append_kernel(const __grid
 
 // ------------------------------------------------------------------------------------------------ gather
 // zero + scale * code, fused so that it is rounded once, from the packed rows of a token range.  HBM-bound by the writes.
-// A CTA owns kGatherTokens packed places: one thread per place finds request, page and row (bisection over cu), then all
-// walk the places' rows, DP / 8 lanes a row, one word in and 16 bytes out each.
-constexpr int kGatherThreads = 256, kGatherTokens = 16;
+// A CTA owns kGatherTokens packed places: one thread per place finds request, page and row (bisection over cu, the batch's last
+// narrowing in shared memory), then all walk the places' rows, DP / 8 lanes a row, one word in and 16 bytes out each.
+constexpr int kGatherThreads = 256, kGatherTokens = 16, kGatherCu = 1024;
 
 struct GatherParams {
   const uint32_t* codes;
@@ -266,80 +308,93 @@ struct GatherParams {
   unsigned char* out[2];
   int* status_word;
   int64_t ld_table, num_pages, total;
-  int batch, max_blocks, heads, d[2], bf16, page_shift;
+  FastDiv heads;
+  int batch, max_blocks, d[2], page_shift;
 };
 
-template <int DP>
+template <int DP, bool BF16>
 __global__ void __launch_bounds__(kGatherThreads) kv4_gather_kernel(const __grid_constant__ GatherParams p) {
   constexpr int W = DP / 8, ROWS = kGatherThreads / W;
   __shared__ int64_t s_row[kGatherTokens];      // row of head 0 of K on the token's page, or -1
+  __shared__ int s_cu[kGatherCu + 1];
   pdl_wait();
   pdl_launch_dependents();
   const int64_t t0 = (int64_t)blockIdx.x * kGatherTokens;
-  const int P = 1 << p.page_shift;
+  const int heads = p.heads.d;
+  const bool local = p.batch <= kGatherCu;
+  if (local)
+    for (int i = threadIdx.x; i <= p.batch; i += kGatherThreads) s_cu[i] = p.cu[i];
+  __syncthreads();
   if (threadIdx.x < kGatherTokens) {
+    const int32_t* cu = local ? s_cu : p.cu;
     const int64_t t = t0 + threadIdx.x;
     int64_t row = -1;
-    if (t < p.total && p.batch > 0 && t >= p.cu[0] && t < p.cu[p.batch]) {
+    if (t < p.total && p.batch > 0 && t >= cu[0] && t < cu[p.batch]) {
       int lo = 0, hi = p.batch;
       while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
-        if (p.cu[mid] <= t) lo = mid; else hi = mid;
+        if (cu[mid] <= t) lo = mid; else hi = mid;
       }
-      const int64_t at = t - p.cu[lo] + (p.starts ? max(p.starts[lo], 0) : 0);
+      const int64_t at = t - cu[lo] + (p.starts ? max(p.starts[lo], 0) : 0);
       const int64_t block = at >> p.page_shift;
       int page = -1;
       if (block < p.max_blocks) page = p.table[(size_t)lo * p.ld_table + block];
-      if (page >= 0 && page < p.num_pages) row = (int64_t)page * 2 * p.heads * P + (at & (P - 1));
+      if (page >= 0 && page < p.num_pages) row = (((int64_t)page * 2 * heads) << p.page_shift) + (at & ((1 << p.page_shift) - 1));
       else if (p.status_word) atomicOr(p.status_word, UNIQL_STATUS_BAD_INDEX);
     }
     s_row[threadIdx.x] = row;
   }
   __syncthreads();
-  const int n = (int)(p.total - t0 < kGatherTokens ? p.total - t0 : kGatherTokens);
-  const int sub = threadIdx.x % W;
-  const int per_kv = n * p.heads;
-  for (int r = threadIdx.x / W; r < 2 * per_kv; r += ROWS) {
-    const int kv = r >= per_kv, rr = r - kv * per_kv;
-    const int i = rr / p.heads, h = rr - i * p.heads;
-    if (sub * 8 >= p.d[kv]) continue;
-    const int64_t row0 = s_row[i];
-    uint4 o = make_uint4(0, 0, 0, 0);
-    if (row0 >= 0) {
-      const int64_t row = row0 + ((int64_t)kv * p.heads + h) * P;
-      const uint32_t w = p.codes[row * W + sub];
-      const __half2 sz = p.scales[row];
-      uint32_t c[4];
-      kv4_codes(w, c);                          // (d, d + 4) pairs
-      if (!p.bf16) {
-        const __half2 s2 = __low2half2(sz), z2 = __high2half2(sz);
-        uint32_t v[4];
+  const uint32_t n = (uint32_t)(p.total - t0 < kGatherTokens ? p.total - t0 : kGatherTokens);
+  const uint32_t sub = threadIdx.x % W;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const __half2 f = __hfma2(*reinterpret_cast<const __half2*>(&c[e]), s2, z2);
-          v[e] = *reinterpret_cast<const uint32_t*>(&f);
-        }
-        o = make_uint4(__byte_perm(v[0], v[1], 0x5410), __byte_perm(v[2], v[3], 0x5410), __byte_perm(v[0], v[1], 0x7632),
-                       __byte_perm(v[2], v[3], 0x7632));
-      } else {
-        const float s = __low2float(sz), z = __high2float(sz);
-        float v[8];
+  for (int kv = 0; kv < 2; ++kv) {
+    const uint32_t d = p.d[kv];
+    if (sub * 8 >= d) continue;
+    unsigned char* out = p.out[kv] + 2 * (t0 * heads * d + sub * 8);
+    const uint32_t* codes = p.codes + sub;
+    const int64_t shift_rows = kv ? (int64_t)heads << p.page_shift : 0;
+#pragma unroll 4
+    for (uint32_t r = threadIdx.x / W; r < n * heads; r += ROWS) {
+      const uint32_t i = p.heads.quot(r), h = r - i * heads;
+      const int64_t row0 = s_row[i];
+      uint4 o = make_uint4(0, 0, 0, 0);
+      if (row0 >= 0) {
+        const int64_t row = row0 + shift_rows + ((int64_t)h << p.page_shift);
+        const uint32_t w = codes[row * W];
+        const __half2 sz = p.scales[row];
+        uint32_t c[4];
+        kv4_codes(w, c);                        // (d, d + 4) pairs
+        if constexpr (!BF16) {
+          const __half2 s2 = __low2half2(sz), z2 = __high2half2(sz);
+          uint32_t v[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&c[e]));
-          v[e] = fmaf(f.x, s, z);
-          v[e + 4] = fmaf(f.y, s, z);
-        }
-        uint32_t u[4];
+          for (int e = 0; e < 4; ++e) {
+            const __half2 f = __hfma2(*reinterpret_cast<const __half2*>(&c[e]), s2, z2);
+            v[e] = *reinterpret_cast<const uint32_t*>(&f);
+          }
+          o = make_uint4(__byte_perm(v[0], v[1], 0x5410), __byte_perm(v[2], v[3], 0x5410), __byte_perm(v[0], v[1], 0x7632),
+                         __byte_perm(v[2], v[3], 0x7632));
+        } else {
+          const float s = __low2float(sz), z = __high2float(sz);
+          float v[8];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const __nv_bfloat162 b = __floats2bfloat162_rn(v[2 * e], v[2 * e + 1]);
-          u[e] = *reinterpret_cast<const uint32_t*>(&b);
+          for (int e = 0; e < 4; ++e) {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&c[e]));
+            v[e] = fmaf(f.x, s, z);
+            v[e + 4] = fmaf(f.y, s, z);
+          }
+          uint32_t u[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const __nv_bfloat162 b = __floats2bfloat162_rn(v[2 * e], v[2 * e + 1]);
+            u[e] = *reinterpret_cast<const uint32_t*>(&b);
+          }
+          o = make_uint4(u[0], u[1], u[2], u[3]);
         }
-        o = make_uint4(u[0], u[1], u[2], u[3]);
       }
+      *reinterpret_cast<uint4*>(out + (size_t)(2 * r) * d) = o;
     }
-    *reinterpret_cast<uint4*>(p.out[kv] + 2 * (((t0 + i) * p.heads + h) * (int64_t)p.d[kv] + sub * 8)) = o;
   }
 }
 
@@ -375,24 +430,30 @@ extern "C" int uniql_kv_page_plan(const int32_t* lens, const int32_t* new_lens, 
       if (dev >= 0 && dev < 64) attr_set[dev] = true;
     }
   }
-  // one thread per token up to the eight CTAs of a portable cluster
-  int ctas = (int)((total_new + kPlanThreads - 1) / kPlanThreads);
-  ctas = ctas < 1 ? 1 : ctas > 8 ? 8 : ctas;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)ctas);
-  cfg.blockDim = dim3(kPlanThreads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = (cudaStream_t)stream;
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = (unsigned)ctas;
-  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 2;
-  UNIQL_CUDA_TRY(cudaLaunchKernelEx(&cfg, kv_page_plan_kernel, p));
-  return UNIQL_OK;
+  const int64_t ctas = (total_new + kPlanThreads - 1) / kPlanThreads;
+  auto launch = [&](int64_t grid, int cluster, int lists, int totals) {
+    p.lists = lists;
+    p.totals = totals;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)grid);
+    cfg.blockDim = dim3(kPlanThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = (cudaStream_t)stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = (unsigned)cluster;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    UNIQL_CUDA_TRY(cudaLaunchKernelEx(&cfg, kv_page_plan_kernel, (const PlanParams&)p));
+    return (int)UNIQL_OK;
+  };
+  if (ctas <= 8) return launch(ctas < 1 ? 1 : ctas, ctas < 1 ? 1 : (int)ctas, 1, 1);
+  const int64_t sms = device_info().sm_count;
+  const int st = launch(ctas < sms ? ctas : sms, 1, 1, 0);
+  return st != UNIQL_OK ? st : launch(1, 1, 0, 1);
 }
 
 extern "C" int uniql_kv4_append(const void* k, int64_t k_token_stride, int64_t k_head_stride, const void* v,
@@ -410,18 +471,27 @@ extern "C" int uniql_kv4_append(const void* k, int64_t k_token_stride, int64_t k
   if (!k || !v || !slots || !aligned16(k) || !aligned16(v)) return UNIQL_EINVAL;
   if (num_pages > 0 && (!codes || !scales || !aligned16(codes) || !aligned16(scales))) return UNIQL_EINVAL;
   AppendParams p;
-  p.src[0] = (const unsigned char*)k; p.src[1] = (const unsigned char*)v;
   p.token_stride[0] = k_token_stride; p.token_stride[1] = v_token_stride;
   p.head_stride[0] = k_head_stride; p.head_stride[1] = v_head_stride;
-  p.slots = slots; p.codes = (uint32_t*)codes; p.scales = (__half2*)scales; p.status_word = status_word;
-  p.tokens = tokens; p.num_slots = num_pages * page_size; p.heads = (int)kv_heads; p.d[0] = (int)dk; p.d[1] = (int)dv;
-  p.bf16 = dtype == UNIQL_BF16; p.page_shift = page_shift_of(page_size);
-  const int64_t rows = tokens * 2 * kv_heads, per = kAppendThreads / (dp / 8);
-  int64_t ctas = (rows + per - 1) / per;
-  const int64_t cap = 8 * (int64_t)device_info().sm_count;
-  if (ctas > cap) ctas = cap;
-  return dp == 128 ? launch_pdl(kv4_append_kernel<128>, (unsigned)ctas, kAppendThreads, 0, (cudaStream_t)stream, p)
-                   : launch_pdl(kv4_append_kernel<64>, (unsigned)ctas, kAppendThreads, 0, (cudaStream_t)stream, p);
+  p.codes = (uint32_t*)codes; p.scales = (__half2*)scales; p.status_word = status_word;
+  p.num_slots = num_pages * page_size; p.heads = FastDiv((uint32_t)kv_heads); p.d[0] = (int)dk; p.d[1] = (int)dv;
+  p.page_shift = page_shift_of(page_size);
+  const bool bf16 = dtype == UNIQL_BF16;
+  auto kernel = dp == 128 ? (bf16 ? kv4_append_kernel<128, true> : kv4_append_kernel<128, false>)
+                          : (bf16 ? kv4_append_kernel<64, true> : kv4_append_kernel<64, false>);
+  const int64_t per = kAppendThreads / (dp / 8), cap = 8 * (int64_t)device_info().sm_count;
+  const int64_t slab = ((int64_t)1 << 30) / (2 * kv_heads);             // tokens of a launch: rows stay below 2^31
+  for (int64_t t0 = 0; t0 < tokens; t0 += slab) {
+    const int64_t n = tokens - t0 < slab ? tokens - t0 : slab;
+    p.src[0] = (const unsigned char*)k + 2 * t0 * k_token_stride;
+    p.src[1] = (const unsigned char*)v + 2 * t0 * v_token_stride;
+    p.slots = slots + t0;
+    p.rows = (uint32_t)(n * 2 * kv_heads);
+    const int64_t ctas = ((int64_t)p.rows + per - 1) / per;
+    const int err = launch_pdl(kernel, (unsigned)(ctas < cap ? ctas : cap), kAppendThreads, 0, (cudaStream_t)stream, p);
+    if (err != UNIQL_OK) return err;
+  }
+  return UNIQL_OK;
 }
 
 extern "C" int uniql_kv4_gather(const void* codes, const void* scales, int64_t num_pages, int64_t page_size, int64_t dp,
@@ -443,9 +513,10 @@ extern "C" int uniql_kv4_gather(const void* codes, const void* scales, int64_t n
   p.codes = (const uint32_t*)codes; p.scales = (const __half2*)scales; p.table = block_table; p.starts = starts; p.cu = cu;
   p.out[0] = (unsigned char*)k_out; p.out[1] = (unsigned char*)v_out; p.status_word = status_word;
   p.ld_table = ld_table; p.num_pages = num_pages; p.total = total; p.batch = (int)batch; p.max_blocks = (int)max_blocks;
-  p.heads = (int)kv_heads; p.d[0] = (int)dk; p.d[1] = (int)dv; p.bf16 = dtype == UNIQL_BF16;
-  p.page_shift = page_shift_of(page_size);
+  p.heads = FastDiv((uint32_t)kv_heads); p.d[0] = (int)dk; p.d[1] = (int)dv; p.page_shift = page_shift_of(page_size);
   const unsigned ctas = (unsigned)((total + kGatherTokens - 1) / kGatherTokens);
-  return dp == 128 ? launch_pdl(kv4_gather_kernel<128>, ctas, kGatherThreads, 0, (cudaStream_t)stream, p)
-                   : launch_pdl(kv4_gather_kernel<64>, ctas, kGatherThreads, 0, (cudaStream_t)stream, p);
+  const bool bf16 = dtype == UNIQL_BF16;
+  auto kernel = dp == 128 ? (bf16 ? kv4_gather_kernel<128, true> : kv4_gather_kernel<128, false>)
+                          : (bf16 ? kv4_gather_kernel<64, true> : kv4_gather_kernel<64, false>);
+  return launch_pdl(kernel, ctas, kGatherThreads, 0, (cudaStream_t)stream, p);
 }

@@ -38,6 +38,18 @@ static int launch_pdl(void (*kernel)(const P), unsigned ctas, int threads, size_
   return UNIQL_OK;
 }
 
+// Quotient by a divisor that the host knows (Granlund and Montgomery: division by invariant integers), for n below 2^31.
+struct FastDiv {
+  uint32_t d, mul, shift;
+  explicit FastDiv(uint32_t div = 1) : d(div), mul(0), shift(0) {
+    while (((uint64_t)1 << shift) < div) ++shift;               // 2^shift >= div
+    mul = (uint32_t)((((uint64_t)1 << (31 + shift)) + div - 1) / div);   // at most 2^32 - 1 for div > 1: see quot
+  }
+  __device__ __forceinline__ uint32_t quot(uint32_t n) const {
+    return d == 1 ? n : (uint32_t)(((uint64_t)n * mul) >> 31) >> shift;
+  }
+};
+
 // The two nibbles at bits [3:0] and [19:16] of w as exact fp16 (c - bias), bias given as the fp16 pair 1024 + bias; and those at
 // bits [7:4] and [23:20], where 1024 + 16 c is brought down with one fused multiply-add.
 __device__ __forceinline__ uint32_t kv4_pair(uint32_t w, uint32_t sub) {
