@@ -149,12 +149,14 @@ __global__ void __launch_bounds__(kPlanThreads) kv_page_plan_kernel(const __grid
 }
 
 // ------------------------------------------------------------------------------------------------ append
-// A row (one token, one head, K or V) is DP / 8 lanes with eight channels each: one 16-byte load, the extremes over the lanes
-// (least value and negated greatest one as a 16-bit pair: one shuffle a level), one packed word stored.  HBM-bound by the
+// A row (one token, one head, K or V) is DP / 16 lanes with sixteen channels each: two 16-byte loads, the extremes over the lanes
+// (least value and negated greatest one as a 16-bit pair: one shuffle a level), two packed words stored.  HBM-bound by the
 // reads, 4 bytes a channel against 0.5 written, if the instructions are few: the packed minimum carries NaN along, the codes
-// are rounded by adding 1.5 * 2^23 and joined as the low bits of those sums.
+// are rounded by adding 1.5 * 2^23 and joined as the low bits of those sums, and sixteen channels a lane share what a row costs
+// (eight: 50 us for 14760 tokens of 8 heads, 121 MB read; sixteen: 31).  (hi - lo) / 15 is the quotient by the reciprocal and one
+// residual step (Markstein), equal to the division for every mantissa.
 //
-// Codes.  y = (x - z) * (1 / s) is within 3 * 2^-24 of the quotient (relative).  Where that leaves the side of a half-way point
+// Codes.  y = (x - z) * (1 / s) is within 2^-22 of the quotient (relative).  Where that leaves the side of a half-way point
 // open, the two sides are compared exactly: x - z spans at most 41 bits and (k + 1/2) * s sixteen, both exact in fp64.
 constexpr float kRound = 12582912.f;            // 1.5 * 2^23
 __device__ __noinline__ uint32_t kv4_exact_code(float x, float z, float s, float y) {
@@ -190,12 +192,13 @@ struct Pair16<true> {
 
 template <int DP, bool BF16>
 __global__ void __launch_bounds__(kAppendThreads) kv4_append_kernel(const __grid_constant__ AppendParams p) {
-  constexpr int W = DP / 8;                     // lanes of a row
+  constexpr int W = DP / 16;                    // lanes of a row
   using T2 = typename Pair16<BF16>::T;
   pdl_wait();
   pdl_launch_dependents();
-  const int sub = threadIdx.x % W;
+  const uint32_t sub = threadIdx.x % W;
   const uint32_t step = gridDim.x * (kAppendThreads / W);
+  const uint32_t kInfs = BF16 ? 0x7f807f80u : 0x7c007c00u;
   // the lanes of a warp stay in the loop together: the shuffles below name the whole warp
   const uint32_t first = blockIdx.x * (kAppendThreads / W) + threadIdx.x / W, ahead = (threadIdx.x % 32) / W;
   for (uint32_t r = first; r - ahead < p.rows; r += step) {
@@ -204,30 +207,42 @@ __global__ void __launch_bounds__(kAppendThreads) kv4_append_kernel(const __grid
     const int kv = pair & 1;
     const int64_t slot = live ? p.slots[t] : -1;
     const bool stored = slot >= 0 && slot < p.num_slots;
-    const bool mine = stored && sub * 8 < (kv ? p.d[1] : p.d[0]);
-    uint4 raw = make_uint4(0, 0, 0, 0);
-    if (mine)
-      raw = *reinterpret_cast<const uint4*>((kv ? p.src[1] : p.src[0]) +
-                                            2 * (t * (kv ? p.token_stride[1] : p.token_stride[0]) + h * (kv ? p.head_stride[1] : p.head_stride[0]) + sub * 8));
-    const uint32_t u[4] = {raw.x, raw.y, raw.z, raw.w};
-    // (least, -greatest) of the row; lanes without channels hold infinities
-    T2 least = *reinterpret_cast<const T2*>(&u[0]), most = least;
+    const int left = (kv ? p.d[1] : p.d[0]) - (int)sub * 16;    // channels from this lane's first on
+    const bool mine[2] = {stored && left > 0, stored && left > 8};
+    uint4 raw[2];
+    const unsigned char* src = (kv ? p.src[1] : p.src[0]) +
+                               2 * (t * (kv ? p.token_stride[1] : p.token_stride[0]) + h * (kv ? p.head_stride[1] : p.head_stride[0]) + sub * 16);
 #pragma unroll
-    for (int e = 1; e < 4; ++e) {
-      least = __hmin2_nan(least, *reinterpret_cast<const T2*>(&u[e]));
-      most = __hmax2_nan(most, *reinterpret_cast<const T2*>(&u[e]));
+    for (int j = 0; j < 2; ++j) {
+      raw[j] = make_uint4(0, 0, 0, 0);
+      if (mine[j]) raw[j] = *reinterpret_cast<const uint4*>(src + 16 * j);
     }
-    T2 ends;
-    ends.x = __hmin_nan(least.x, least.y);
-    ends.y = __hneg(__hmax_nan(most.x, most.y));
-    uint32_t eb = mine ? *reinterpret_cast<const uint32_t*>(&ends) : (BF16 ? 0x7f807f80u : 0x7c007c00u);
+    // (least, -greatest) of the row; places without channels hold infinities
+    uint32_t eb = kInfs;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const uint32_t u[4] = {raw[j].x, raw[j].y, raw[j].z, raw[j].w};
+      T2 least = *reinterpret_cast<const T2*>(&u[0]), most = least;
+#pragma unroll
+      for (int e = 1; e < 4; ++e) {
+        least = __hmin2_nan(least, *reinterpret_cast<const T2*>(&u[e]));
+        most = __hmax2_nan(most, *reinterpret_cast<const T2*>(&u[e]));
+      }
+      T2 ends;
+      ends.x = __hmin_nan(least.x, least.y);
+      ends.y = __hneg(__hmax_nan(most.x, most.y));
+      if (mine[j]) {
+        ends = __hmin2_nan(ends, *reinterpret_cast<const T2*>(&eb));
+        eb = *reinterpret_cast<const uint32_t*>(&ends);
+      }
+    }
 #pragma unroll
     for (int o = W / 2; o; o >>= 1) {
       const uint32_t other = __shfl_xor_sync(~0u, eb, o);
-      ends = __hmin2_nan(*reinterpret_cast<const T2*>(&eb), *reinterpret_cast<const T2*>(&other));
+      const T2 ends = __hmin2_nan(*reinterpret_cast<const T2*>(&eb), *reinterpret_cast<const T2*>(&other));
       eb = *reinterpret_cast<const uint32_t*>(&ends);
     }
-    ends = *reinterpret_cast<const T2*>(&eb);
+    const T2 ends = *reinterpret_cast<const T2*>(&eb);
     float lo, hi;
     if constexpr (BF16) {
       lo = __bfloat162float(ends.x);
@@ -239,12 +254,19 @@ __global__ void __launch_bounds__(kAppendThreads) kv4_append_kernel(const __grid
     const bool nan = lo != lo || hi != hi, wide = lo < -65504.f || hi > 65504.f;
     lo = fminf(fmaxf(lo, -65504.f), 65504.f);
     hi = fminf(fmaxf(hi, -65504.f), 65504.f);
-    __half sh = __float2half_rn(__fdiv_rn(hi - lo, 15.f));
+    constexpr float k15 = 1.f / 15.f;
+    const float span = hi - lo, q0 = span * k15;
+    __half sh = __float2half_rn(fmaf(fmaf(-15.f, q0, span), k15, q0));
     if (__half2float(sh) < 5.9604645e-8f) sh = __ushort_as_half(1);      // 2^-24: a scale is never zero
     __half zh = __float2half_rn(lo);
-    const float s = __half2float(sh), z = __half2float(zh), inv = __frcp_rn(s);
-    uint32_t word = 0;
-    if (mine && !nan) {
+    const float s = __half2float(sh), z = __half2float(zh);
+    float inv;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(s));
+    uint32_t word[2] = {0, 0};
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      if (!mine[j] || nan) continue;
+      const uint32_t u[4] = {raw[j].x, raw[j].y, raw[j].z, raw[j].w};
       float x[8], y[8], far = 0.f;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
@@ -260,29 +282,31 @@ __global__ void __launch_bounds__(kAppendThreads) kv4_append_kernel(const __grid
       }
       constexpr uint32_t kBits = 0x4b400000u;   // of kRound; what eight of them add to the word:
       constexpr uint32_t kAll = kBits + (kBits << 4) + (kBits << 8) + (kBits << 12) + (kBits << 16) + (kBits << 20) + (kBits << 24) + (kBits << 28);
+      uint32_t w = 0u - kAll;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         y[e] = fminf(fmaxf((x[e] - z) * inv, 0.f), 15.f);
         const float up = y[e] + kRound;
         far = fmaxf(far, fabsf(y[e] - (up - kRound)));
-        word += __float_as_uint(up) << (4 * e);
+        w += __float_as_uint(up) << (4 * e);
       }
-      word -= kAll;
       if (far > 0.49998f) {                     // some quotient within 2e-5 of a half-way point
-        word = 0;
+        w = 0;
 #pragma unroll 1
         for (int e = 0; e < 8; ++e) {
-          float xe = BF16 ? __uint_as_float((e & 1) ? u[e >> 1] & 0xffff0000u : u[e >> 1] << 16)
-                                : __half2float(__ushort_as_half((unsigned short)(u[e >> 1] >> (16 * (e & 1)))));
+          const uint32_t ue = (e >> 1) == 0 ? u[0] : (e >> 1) == 1 ? u[1] : (e >> 1) == 2 ? u[2] : u[3];
+          float xe = BF16 ? __uint_as_float((e & 1) ? ue & 0xffff0000u : ue << 16)
+                          : __half2float(__ushort_as_half((unsigned short)(ue >> (16 * (e & 1)))));
           xe = fminf(fmaxf(xe, -65504.f), 65504.f);
-          word |= kv4_exact_code(xe, z, s, (xe - z) * inv) << (4 * e);
+          w |= kv4_exact_code(xe, z, s, (xe - z) * inv) << (4 * e);
         }
       }
+      word[j] = w;
     }
     if (stored) {
       const int64_t page = slot >> p.page_shift;
       const int64_t row = (((page * 2 + kv) * p.heads.d + h) << p.page_shift) + (slot & ((1 << p.page_shift) - 1));
-      p.codes[row * W + sub] = word;
+      *reinterpret_cast<uint2*>(p.codes + row * (DP / 8) + 2 * sub) = make_uint2(word[0], word[1]);
       if (sub == 0) {
         if (nan) sh = zh = __ushort_as_half(0x7fff);
         p.scales[row] = __halves2half2(sh, zh);
@@ -297,7 +321,7 @@ __global__ void __launch_bounds__(kAppendThreads) kv4_append_kernel(const __grid
 // zero + scale * code, fused so that it is rounded once, from the packed rows of a token range.  HBM-bound by the writes.
 // A CTA owns kGatherTokens packed places: one thread per place finds request, page and row (bisection over cu, the batch's last
 // narrowing in shared memory), then all walk the places' rows, DP / 8 lanes a row, one word in and 16 bytes out each.
-constexpr int kGatherThreads = 256, kGatherTokens = 16, kGatherCu = 1024;
+constexpr int kGatherThreads = 256, kGatherTokens = 16, kGatherRows = 4, kGatherCu = 1024;
 
 struct GatherParams {
   const uint32_t* codes;
@@ -354,19 +378,32 @@ __global__ void __launch_bounds__(kGatherThreads) kv4_gather_kernel(const __grid
     unsigned char* out = p.out[kv] + 2 * (t0 * heads * d + sub * 8);
     const uint32_t* codes = p.codes + sub;
     const int64_t shift_rows = kv ? (int64_t)heads << p.page_shift : 0;
-#pragma unroll 4
-    for (uint32_t r = threadIdx.x / W; r < n * heads; r += ROWS) {
-      const uint32_t i = p.heads.quot(r), h = r - i * heads;
-      const int64_t row0 = s_row[i];
-      uint4 o = make_uint4(0, 0, 0, 0);
-      if (row0 >= 0) {
-        const int64_t row = row0 + shift_rows + ((int64_t)h << p.page_shift);
-        const uint32_t w = codes[row * W];
-        const __half2 sz = p.scales[row];
+    for (uint32_t r0 = threadIdx.x / W; r0 < n * heads; r0 += kGatherRows * ROWS) {
+      uint32_t w[kGatherRows];
+      __half2 sz[kGatherRows];
+#pragma unroll
+      for (int j = 0; j < kGatherRows; ++j) {
+        const uint32_t r = r0 + j * ROWS;
+        w[j] = 0;
+        sz[j] = __halves2half2(__ushort_as_half(0), __ushort_as_half(0));
+        if (r < n * heads) {
+          const uint32_t i = p.heads.quot(r), h = r - i * heads;
+          if (s_row[i] >= 0) {
+            const int64_t row = s_row[i] + shift_rows + ((int64_t)h << p.page_shift);
+            w[j] = codes[row * W];
+            sz[j] = p.scales[row];
+          }
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < kGatherRows; ++j) {
+        const uint32_t r = r0 + j * ROWS;
+        if (r >= n * heads) break;
+        uint4 o;
         uint32_t c[4];
-        kv4_codes(w, c);                        // (d, d + 4) pairs
+        kv4_codes(w[j], c);                     // (d, d + 4) pairs; absent rows are 0 + 0 * 0
         if constexpr (!BF16) {
-          const __half2 s2 = __low2half2(sz), z2 = __high2half2(sz);
+          const __half2 s2 = __low2half2(sz[j]), z2 = __high2half2(sz[j]);
           uint32_t v[4];
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
@@ -376,7 +413,7 @@ __global__ void __launch_bounds__(kGatherThreads) kv4_gather_kernel(const __grid
           o = make_uint4(__byte_perm(v[0], v[1], 0x5410), __byte_perm(v[2], v[3], 0x5410), __byte_perm(v[0], v[1], 0x7632),
                          __byte_perm(v[2], v[3], 0x7632));
         } else {
-          const float s = __low2float(sz), z = __high2float(sz);
+          const float s = __low2float(sz[j]), z = __high2float(sz[j]);
           float v[8];
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
@@ -392,8 +429,8 @@ __global__ void __launch_bounds__(kGatherThreads) kv4_gather_kernel(const __grid
           }
           o = make_uint4(u[0], u[1], u[2], u[3]);
         }
+        *reinterpret_cast<uint4*>(out + (size_t)(2 * r) * d) = o;
       }
-      *reinterpret_cast<uint4*>(out + (size_t)(2 * r) * d) = o;
     }
   }
 }
@@ -479,7 +516,7 @@ extern "C" int uniql_kv4_append(const void* k, int64_t k_token_stride, int64_t k
   const bool bf16 = dtype == UNIQL_BF16;
   auto kernel = dp == 128 ? (bf16 ? kv4_append_kernel<128, true> : kv4_append_kernel<128, false>)
                           : (bf16 ? kv4_append_kernel<64, true> : kv4_append_kernel<64, false>);
-  const int64_t per = kAppendThreads / (dp / 8), cap = 8 * (int64_t)device_info().sm_count;
+  const int64_t per = kAppendThreads / (dp / 16), cap = 8 * (int64_t)device_info().sm_count;
   const int64_t slab = ((int64_t)1 << 30) / (2 * kv_heads);             // tokens of a launch: rows stay below 2^31
   for (int64_t t0 = 0; t0 < tokens; t0 += slab) {
     const int64_t n = tokens - t0 < slab ? tokens - t0 : slab;
