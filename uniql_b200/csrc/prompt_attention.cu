@@ -24,7 +24,12 @@ namespace uniql {
 
 namespace pa {
 constexpr int kMmaWarp = 8, kLoadWarp = 9;   // warps 0-7: softmax
-constexpr int kThreads = 320;
+constexpr int kThreads = 384;                   // three warpgroups; the third has two idle warps
+constexpr int kSoftmaxRegs = 208, kOtherRegs = 80;      // 2 * 208 + 80 <= 3 * 168, what the block is launched with
+#ifndef PA_EMU
+#define PA_EMU 4
+#endif
+constexpr int kPoly = PA_EMU;                   // of 16 pairs of exponentials, how many run as polynomials
 constexpr int kRows = 128, kKeys = 128;
 constexpr int kTmemCols = 512;                  // S0, S1, O0, O1: 128 columns each
 template <int DP>
@@ -33,11 +38,16 @@ struct Cfg {
   static constexpr int kStages = 5;
   static constexpr int kOffKv = 2 * kTileBytes;
   static constexpr int kOffBar = kOffKv + kStages * kTileBytes;
-  static constexpr int kBars = 1 + 2 * kStages + 6 + 1;
+  static constexpr int kBars = 1 + 2 * kStages + 8 + 1;
   static constexpr int kSmem = kOffBar + kBars * 8 + 16 + 1024;
   static_assert(kSmem <= 227 * 1024, "shared memory");
 };
 }  // namespace pa
+
+template <bool V>
+struct PaFlag {
+  static constexpr bool value = V;
+};
 
 struct PaParams {
   const int32_t* cu_q;
@@ -98,6 +108,64 @@ __device__ __forceinline__ void pa_mma_ts(uint32_t d, uint32_t a, uint64_t b, ui
       ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(acc)
       : "memory");
 }
+__device__ __forceinline__ void pa_st16(uint32_t taddr, const uint32_t* u) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+      ::"r"(taddr), "r"(u[0]), "r"(u[1]), "r"(u[2]), "r"(u[3]), "r"(u[4]), "r"(u[5]), "r"(u[6]), "r"(u[7]), "r"(u[8]),
+        "r"(u[9]), "r"(u[10]), "r"(u[11]), "r"(u[12]), "r"(u[13]), "r"(u[14]), "r"(u[15])
+      : "memory");
+}
+// Two floats side by side: one instruction of the FMA pipe for both.
+__device__ __forceinline__ uint64_t pa_two(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 pa_split(uint64_t v) {
+  float2 f;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(v));
+  return f;
+}
+__device__ __forceinline__ uint64_t pa_fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t pa_add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ float pa_max3(float a, float b, float c) {   // NaN if any is
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+// 2^v for two finite v below 128, without the special-function unit: v = n + r with n the nearest integer (taken by adding 1.5 *
+// 2^23), a polynomial in r, n added to the exponent.  Coefficients: minimax of the relative error on [-1/2, 1/2] (Remez);
+// degree 3 is within 2^-13.7, for bf16 weights, degree 4 within 2^-18.5, for fp16 ones.  Below -126 it stays at 2^-126.
+template <int DEG>
+__device__ __forceinline__ uint64_t pa_poly_exp2(uint64_t v) {
+  const float2 f = pa_split(v);
+  const uint64_t x = pa_two(fmaxf(f.x, -126.f), fmaxf(f.y, -126.f));
+  const uint64_t round = pa_two(12582912.f, 12582912.f), back = pa_two(-12582912.f, -12582912.f), neg = pa_two(-1.f, -1.f);
+  const uint64_t n = pa_add2(x, round), r = pa_fma2(pa_add2(n, back), neg, x);
+  auto c = [](float k) { return pa_two(k, k); };
+  uint64_t y;
+  if (DEG == 3) {
+    y = pa_fma2(c(0.0551716685295105f), r, c(0.2426111251115799f));
+    y = pa_fma2(y, r, c(0.6932609677314758f));
+    y = pa_fma2(y, r, c(0.9999280571937561f));
+  } else {
+    y = pa_fma2(c(0.009570102207362652f), r, c(0.05591785907745361f));
+    y = pa_fma2(y, r, c(0.240247443318367f));
+    y = pa_fma2(y, r, c(0.6931217908859253f));
+    y = pa_fma2(y, r, c(0.9999992847442627f));
+  }
+  const float2 a = pa_split(y), e = pa_split(n);
+  return pa_two(__uint_as_float(__float_as_uint(a.x) + (__float_as_uint(e.x) << 23)),
+                __uint_as_float(__float_as_uint(a.y) + (__float_as_uint(e.y) << 23)));
+}
 template <bool BF16>
 __device__ __forceinline__ uint32_t pa_pack(float a, float b) {
   if (BF16) {
@@ -121,7 +189,7 @@ prompt_attention_kernel(const __grid_constant__ PaParams p, const __grid_constan
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_unaligned) + 1023) & ~(uintptr_t)1023);
   const uint32_t sbase = tc_smem_addr(smem);
   const uint32_t bar_q = sbase + C::kOffBar, bar_full = bar_q + 8, bar_empty = bar_full + 8 * C::kStages;
-  const uint32_t bar_s = bar_empty + 8 * C::kStages, bar_p = bar_s + 16, bar_o = bar_p + 16, bar_clean = bar_o + 16;
+  const uint32_t bar_s = bar_empty + 8 * C::kStages, bar_p = bar_s + 16, bar_o = bar_p + 32, bar_clean = bar_o + 16;
   volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(smem + C::kOffBar + C::kBars * 8);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
@@ -142,7 +210,8 @@ prompt_attention_kernel(const __grid_constant__ PaParams p, const __grid_constan
     }
     for (int t = 0; t < 2; ++t) {
       tc_mbar_init(bar_s + 8 * t, 1);
-      tc_mbar_init(bar_p + 8 * t, 4);
+      tc_mbar_init(bar_p + 16 * t, 4);          // the first 64 columns of P, then the others
+      tc_mbar_init(bar_p + 16 * t + 8, 4);
       tc_mbar_init(bar_o + 8 * t, 1);
     }
     tc_mbar_init(bar_clean, 1);
@@ -222,6 +291,8 @@ prompt_attention_kernel(const __grid_constant__ PaParams p, const __grid_constan
     const int nmax = max(n[0], n[1]);
     const bool dirty = nmax * kKeys > nk;       // the last tile of V reaches behind the request
 
+    if (warp >= kMmaWarp) {
+      asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
     if (warp == kLoadWarp) {
       // ------------------------------------------------------------------ loads: Q, then K 0, V 0, K 1, V 1, ...
       if (tc_elect() && nmax > 0) {
@@ -276,14 +347,18 @@ prompt_attention_kernel(const __grid_constant__ PaParams p, const __grid_constan
                         tc_smem_desc(kt + (s >> 2) * SUB) + 2 * (s & 3), idesc_s, s > 0);
           tc_commit(bar_s + 8 * t);
         };
-        auto values = [&](int t, int it, uint32_t acc) {        // O_t (+)= P_t V
+        auto values = [&](int t, int it, uint32_t acc, uint32_t parity) {        // O_t (+)= P_t V, half by half as P arrives
           const uint32_t vt = sbase + C::kOffKv + (it % C::kStages) * C::kTileBytes;
           // MN-major, 128-byte swizzle: 64-channel sub-tiles SUB bytes apart, groups of 8 keys 1024 bytes apart
           const uint64_t vd = (uint64_t)((vt & 0x3FFFFu) >> 4) | ((uint64_t)(SUB >> 4) << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
-          if (!timed_out)
 #pragma unroll
-            for (int s = 0; s < 8; ++s)
-              pa_mma_ts(tmem + 256 + t * 128, tmem + t * 128 + 8 * s, vd + 128 * s, idesc_o, s > 0 ? 1u : acc);
+          for (int h = 0; h < 2; ++h) {
+            wait(bar_p + 16 * t + 8 * h, parity);
+            if (!timed_out)
+#pragma unroll
+              for (int s = 4 * h; s < 4 * h + 4; ++s)
+                pa_mma_ts(tmem + 256 + t * 128, tmem + t * 128 + 8 * s, vd + 128 * s, idesc_o, s > 0 ? 1u : acc);
+          }
           tc_commit(bar_o + 8 * t);
         };
         wait(bar_q, 0);
@@ -299,18 +374,17 @@ prompt_attention_kernel(const __grid_constant__ PaParams p, const __grid_constan
           else if (dirty) wait(bar_clean, 0);
 #pragma unroll
           for (int t = 0; t < 2; ++t) {
-            if (j < n[t]) {
-              wait(bar_p + 8 * t, j & 1);
-              values(t, iv, j > 0);
-            }
+            if (j < n[t]) values(t, iv, j > 0, j & 1);
             if (t == 1) tc_commit(bar_empty + 8 * sv);
             if (j + 1 < n[t]) scores(t, ik);
           }
           if (j + 1 < nmax) tc_commit(bar_empty + 8 * sk);
         }
       }
+    }
     } else {
       // ------------------------------------------------------------------ softmax, one query row a thread
+      asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
       const int t = warp >> 2;
       const int nt = t ? n[1] : n[0], row0 = t ? row[1] : row[0], i = row0 + (warp & 3) * 32 + lane;
       const int limit = p.causal ? min(nk, max(i + 1 + shift, 0)) : nk;
@@ -326,19 +400,24 @@ prompt_attention_kernel(const __grid_constant__ PaParams p, const __grid_constan
 #pragma unroll
         for (int c = 0; c < 4; ++c) pa_ld32(ts + 32 * c, s + 32 * c);
         pa_wait_ld();
-        if ((j + 1) * kKeys > full) {
+        const bool masked = (j + 1) * kKeys > full;
+        if (masked) {
           const int left = limit - j * kKeys;
 #pragma unroll
           for (int c = 0; c < 128; ++c) s[c] = c < left ? s[c] : -INFINITY;
         }
-        float top = fmaxf(s[0], s[1]);
+        float top4[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-        for (int c = 2; c < 128; ++c) top = fmaxf(top, s[c]);
+        for (int c = 4; c < 124; c += 8)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) top4[e] = pa_max3(top4[e], s[c + e], s[c + 4 + e]);
+        float top = pa_max3(pa_max3(top4[0], top4[1], top4[2]), pa_max3(top4[3], s[124], s[125]), pa_max3(s[126], s[127], s[127]));
         top = i < nq ? top * f : -INFINITY;     // rows of another request have no say in when m is raised
+        if (top != top) m = top;                // a NaN among the scores: all of the row is
         if (__any_sync(~0u, top > m + 8.f)) {
           const float mn = fmaxf(m, top);
-          const float k = mn == -INFINITY ? 1.f : pa_exp2(m - mn);
-          m = mn;
+          const float k = m == m ? (mn == -INFINITY ? 1.f : pa_exp2(m - mn)) : m;
+          m = m == m ? mn : m;
           l *= k;
           if (j > 0) {
             if (!timed_out && !tc_mbar_wait(bar_o + 8 * t, (j - 1) & 1)) timed_out = true;
@@ -355,24 +434,39 @@ prompt_attention_kernel(const __grid_constant__ PaParams p, const __grid_constan
           }
         }
         const float base = m == -INFINITY ? 0.f : m;
-        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+        const uint64_t ff = pa_two(f, f), nb = pa_two(-base, -base);
+        uint64_t sum[2] = {0, 0};
+        auto weights = [&](auto poly) {         // P = 2^(f S - m), 32 columns at a time
 #pragma unroll
-        for (int c = 0; c < 128; ++c) {
-          s[c] = pa_exp2(fmaf(s[c], f, -base));
-          sum[c & 3] += s[c];
-        }
-        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+          for (int q = 0; q < 4; ++q) {
+            uint32_t w[16];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          uint32_t w[32];
-#pragma unroll
-          for (int c = 0; c < 32; ++c) w[c] = pa_pack<BF16>(s[64 * h + 2 * c], s[64 * h + 2 * c + 1]);
-          pa_st32(ts + 32 * h, w);
-        }
-        pa_wait_st();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) tc_mbar_arrive(bar_p + 8 * t);
+            for (int c = 0; c < 16; ++c) {
+              uint64_t v = pa_fma2(pa_two(s[32 * q + 2 * c], s[32 * q + 2 * c + 1]), ff, nb);
+              if (poly.value && (c * kPoly) % 16 + kPoly >= 16) {
+                v = pa_poly_exp2<BF16 ? 3 : 4>(v);
+              } else {
+                const float2 e = pa_split(v);
+                v = pa_two(pa_exp2(e.x), pa_exp2(e.y));
+              }
+              sum[c & 1] = pa_add2(sum[c & 1], v);
+              const float2 e = pa_split(v);
+              w[c] = pa_pack<BF16>(e.x, e.y);
+            }
+            pa_st16(ts + 16 * q, w);
+            if (q & 1) {
+              pa_wait_st();
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) tc_mbar_arrive(bar_p + 16 * t + 8 * (q >> 1));
+            }
+          }
+        };
+        // the polynomial has no zero for -inf, so tiles with masked places take the special-function unit alone
+        if (masked) weights(PaFlag<false>{});
+        else weights(PaFlag<true>{});
+        const float2 s0 = pa_split(sum[0]), s1 = pa_split(sum[1]);
+        l += (s0.x + s0.y) + (s1.x + s1.y);
       }
       // ---- O / l
       if (u0 + t < units) {
