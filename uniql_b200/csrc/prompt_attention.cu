@@ -14,7 +14,12 @@
 //
 // Masked places: keys behind a request's last are set to -inf in S, and the rows of V behind it in its last tile, which belong
 // to another request, are cleared in shared memory before they are multiplied by the zeros of P.
-// Bound: tensor pipe and the exponentials, 4 * 128 * 128 * d flops against 128 * 128 exponentials (16 a clock and SM) per tile.
+// Bound: 128 keys of both units cost 2048 cycles of MMA, 2048 of shared memory traffic (Q and K are both read from there) and 2048
+// of exponentials (16 a clock and SM); they take 3135, the rest being the hops S -> softmax -> P -> O of a unit that the other
+// unit's work does not cover, at the 1.6 GHz that the part's power limit leaves (16384 tokens, 32 heads of 128, fp16, causal: 1.8 ms
+// in a short burst, 2.0 ms back to back = 1.1 PFLOP/s).  Tried without gain: S in two 64-key buffers a unit (Q is read twice as
+// often: 2.07 ms against 1.79), P handed over in quarters (1.83 to 2.0), a quarter of the exponentials as polynomials on the FMA
+// pipe (1.75 to 1.96), waits polled without a suspend time (2.00 against 2.05 back to back).
 // Every wait is bounded; a wait that gives up sets UNIQL_STATUS_WAIT_TIMEOUT and the kernel drains.
 #include "common.cuh"
 #include "kv_cache.cuh"
@@ -26,10 +31,6 @@ namespace pa {
 constexpr int kMmaWarp = 8, kLoadWarp = 9;   // warps 0-7: softmax
 constexpr int kThreads = 384;                   // three warpgroups; the third has two idle warps
 constexpr int kSoftmaxRegs = 208, kOtherRegs = 80;      // 2 * 208 + 80 <= 3 * 168, what the block is launched with
-#ifndef PA_EMU
-#define PA_EMU 4
-#endif
-constexpr int kPoly = PA_EMU;                   // of 16 pairs of exponentials, how many run as polynomials
 constexpr int kRows = 128, kKeys = 128;
 constexpr int kTmemCols = 512;                  // S0, S1, O0, O1: 128 columns each
 template <int DP>
@@ -43,11 +44,6 @@ struct Cfg {
   static_assert(kSmem <= 227 * 1024, "shared memory");
 };
 }  // namespace pa
-
-template <bool V>
-struct PaFlag {
-  static constexpr bool value = V;
-};
 
 struct PaParams {
   const int32_t* cu_q;
@@ -140,31 +136,6 @@ __device__ __forceinline__ float pa_max3(float a, float b, float c) {   // NaN i
   float r;
   asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
-}
-// 2^v for two finite v below 128, without the special-function unit: v = n + r with n the nearest integer (taken by adding 1.5 *
-// 2^23), a polynomial in r, n added to the exponent.  Coefficients: minimax of the relative error on [-1/2, 1/2] (Remez);
-// degree 3 is within 2^-13.7, for bf16 weights, degree 4 within 2^-18.5, for fp16 ones.  Below -126 it stays at 2^-126.
-template <int DEG>
-__device__ __forceinline__ uint64_t pa_poly_exp2(uint64_t v) {
-  const float2 f = pa_split(v);
-  const uint64_t x = pa_two(fmaxf(f.x, -126.f), fmaxf(f.y, -126.f));
-  const uint64_t round = pa_two(12582912.f, 12582912.f), back = pa_two(-12582912.f, -12582912.f), neg = pa_two(-1.f, -1.f);
-  const uint64_t n = pa_add2(x, round), r = pa_fma2(pa_add2(n, back), neg, x);
-  auto c = [](float k) { return pa_two(k, k); };
-  uint64_t y;
-  if (DEG == 3) {
-    y = pa_fma2(c(0.0551716685295105f), r, c(0.2426111251115799f));
-    y = pa_fma2(y, r, c(0.6932609677314758f));
-    y = pa_fma2(y, r, c(0.9999280571937561f));
-  } else {
-    y = pa_fma2(c(0.009570102207362652f), r, c(0.05591785907745361f));
-    y = pa_fma2(y, r, c(0.240247443318367f));
-    y = pa_fma2(y, r, c(0.6931217908859253f));
-    y = pa_fma2(y, r, c(0.9999992847442627f));
-  }
-  const float2 a = pa_split(y), e = pa_split(n);
-  return pa_two(__uint_as_float(__float_as_uint(a.x) + (__float_as_uint(e.x) << 23)),
-                __uint_as_float(__float_as_uint(a.y) + (__float_as_uint(e.y) << 23)));
 }
 template <bool BF16>
 __device__ __forceinline__ uint32_t pa_pack(float a, float b) {
@@ -436,35 +407,24 @@ prompt_attention_kernel(const __grid_constant__ PaParams p, const __grid_constan
         const float base = m == -INFINITY ? 0.f : m;
         const uint64_t ff = pa_two(f, f), nb = pa_two(-base, -base);
         uint64_t sum[2] = {0, 0};
-        auto weights = [&](auto poly) {         // P = 2^(f S - m), 32 columns at a time
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            uint32_t w[16];
+        for (int q = 0; q < 4; ++q) {           // P = 2^(f S - m), 32 columns at a time
+          uint32_t w[16];
 #pragma unroll
-            for (int c = 0; c < 16; ++c) {
-              uint64_t v = pa_fma2(pa_two(s[32 * q + 2 * c], s[32 * q + 2 * c + 1]), ff, nb);
-              if (poly.value && (c * kPoly) % 16 + kPoly >= 16) {
-                v = pa_poly_exp2<BF16 ? 3 : 4>(v);
-              } else {
-                const float2 e = pa_split(v);
-                v = pa_two(pa_exp2(e.x), pa_exp2(e.y));
-              }
-              sum[c & 1] = pa_add2(sum[c & 1], v);
-              const float2 e = pa_split(v);
-              w[c] = pa_pack<BF16>(e.x, e.y);
-            }
-            pa_st16(ts + 16 * q, w);
-            if (q & 1) {
-              pa_wait_st();
-              tc_fence_before();
-              __syncwarp();
-              if (lane == 0) tc_mbar_arrive(bar_p + 16 * t + 8 * (q >> 1));
-            }
+          for (int c = 0; c < 16; ++c) {
+            const float2 x = pa_split(pa_fma2(pa_two(s[32 * q + 2 * c], s[32 * q + 2 * c + 1]), ff, nb));
+            const float2 e = make_float2(pa_exp2(x.x), pa_exp2(x.y));
+            sum[c & 1] = pa_add2(sum[c & 1], pa_two(e.x, e.y));
+            w[c] = pa_pack<BF16>(e.x, e.y);
           }
-        };
-        // the polynomial has no zero for -inf, so tiles with masked places take the special-function unit alone
-        if (masked) weights(PaFlag<false>{});
-        else weights(PaFlag<true>{});
+          pa_st16(ts + 16 * q, w);
+          if (q & 1) {
+            pa_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) tc_mbar_arrive(bar_p + 16 * t + 8 * (q >> 1));
+          }
+        }
         const float2 s0 = pa_split(sum[0]), s1 = pa_split(sum[1]);
         l += (s0.x + s0.y) + (s1.x + s1.y);
       }
