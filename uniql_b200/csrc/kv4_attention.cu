@@ -1,10 +1,12 @@
 // Attention of one query token per request over a paged KV cache held in 4 bits.  Layout and rules: include/uniql_b200.h.
 //
 // Mathematics.  With a cached row k_t = z + s c and m = z + 8 s the score is  x_t = f (s (q . (c - 8)) + m sum(q)),  f =
-// softmax_scale log2(e): the products run over the exact centred codes on the tensor cores (mma.sync m16n8k16, fp32 sums), scale
-// and zero enter once per token in fp32.  (mma.sync on e4m3, where a code needs no conversion, was built and taken out: this part
-// runs it as conversions and fp16 products, 478 instructions per 16 tokens either way.)  Queries are taken to fp16 after a
-// division by the power of two below their largest channel: exact, but for channels under 2^-14 of the largest.
+// softmax_scale log2(e).  q . (c - 8) is exact integer arithmetic on the tensor cores: four codes are the bytes of one AND, q is
+// rounded to 2^-19 of its largest channel or less and split into three signed base-128 digits, and mma.sync m16n8k32 (u8 x s8) sums
+// digit times code for each.  A packed word costs three instructions, all a half-rate pipe's, against five of that pipe and four of
+// the other one as two fp16 pairs: what bounds the arithmetic is that pipe (LOP3, PRMT, shifts: two cycles each).
+// (e4m3, where a code is its own subnormal number,
+// runs as conversions and fp16 products on this part.)  Scale and zero enter once per token in fp32.
 // The value side folds its scale into the exponent: with y_t = x_t + log2 s'_t, M a running bound of y and w_t = 2^(y_t - M),
 //     out = (sum w_t (c'_t - 8) + sum (w_t / s'_t) m'_t) / sum (w_t / s'_t),
 // so that w is the one operand that is rounded (fp16, 2^-12 relative above 6e-5; it is at most 2^8, see below), next to exact
@@ -26,6 +28,8 @@
 #include "common.cuh"
 #include "kv_cache.cuh"
 #include "tma.cuh"
+
+#include <type_traits>
 
 namespace uniql {
 
@@ -83,6 +87,40 @@ __device__ __forceinline__ void kva_store(unsigned char* p, int64_t i, int bf16,
   else reinterpret_cast<__half*>(p)[i] = __float2half_rn(v);
 }
 
+__device__ __forceinline__ void kva_mma_u8s8(int (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// Two floats side by side (two heads of a token): one instruction of the FMA pipe for both.
+__device__ __forceinline__ uint64_t kva_two(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 kva_split(uint64_t v) {
+  float2 f;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(v));
+  return f;
+}
+__device__ __forceinline__ uint64_t kva_fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t kva_mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t kva_add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ void kva_lds2(uint32_t a, uint64_t& x, uint64_t& y) {
+  asm volatile("ld.shared.v2.u64 {%0, %1}, [%2];" : "=l"(x), "=l"(y) : "r"(a) : "memory");
+}
 __device__ __forceinline__ float kva_log2(float x) {
   float y;
   asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -98,14 +136,14 @@ __device__ __forceinline__ float kva_rcp(float x) {
 // a row) and the columns (eight lanes a row, four tokens) are read from shared memory without bank conflicts.
 __device__ __forceinline__ int kva_token(int r) { return (r & 8) + ((r & 1) ? 7 - ((r & 7) >> 1) : ((r & 7) >> 1)); }
 
-template <int DP, int NT>
+template <int DP, int NT, bool PAGE16>
 __global__ void __launch_bounds__(kva::kThreads, kva::per_sm(NT)) kv4_attention_kernel(const __grid_constant__ KvaParams p) {
   using namespace kva;
   constexpr int ROWB = DP / 2;                  // bytes of a packed row
   constexpr int CODEB = 16 * ROWB;              // packed rows of 16 tokens, K or V
   constexpr int OFF_SC = 4 * CODEB;             // of a stage: K codes (two halves of 16 tokens), V codes, then 128 bytes of scales a half
   constexpr int STAGEB = OFF_SC + 256;
-  constexpr int RINGB = kStages * STAGEB, WARPB = RINGB + kStep * 20;
+  constexpr int RINGB = kStages * STAGEB, WARPB = RINGB + kStep * 40;
   constexpr int H = 8 * NT, MT = DP / 16, KS = DP / 32;
   constexpr int PSTR = DP + 4;                  // floats of one head's partial: sums, M, L
   extern __shared__ __align__(16) unsigned char smem[];
@@ -205,12 +243,12 @@ __global__ void __launch_bounds__(kva::kThreads, kva::per_sm(NT)) kv4_attention_
     int page0 = 0, page1 = 0;                                   // of the step that is produced next
     auto look = [&](int st) {
       page0 = trow[st * kStep >> p.page_shift];
-      if (p.page_shift == 4) page1 = trow[min(2 * st + 1, last_block)];
+      if (PAGE16) page1 = trow[min(2 * st + 1, last_block)];
     };
     if (first < t1) look(first);
     auto produce = [&](int st, uint32_t dst) {
       if (st < t1) {
-        int pg0 = page0, pg1 = p.page_shift == 4 ? page1 : page0;
+        int pg0 = page0, pg1 = PAGE16 ? page1 : page0;
         if (st + kWarps < t1) look(st + kWarps);
         const bool ok0 = (unsigned)pg0 < (unsigned)p.num_pages, ok1 = (unsigned)pg1 < (unsigned)p.num_pages;
         if (!ok0) pg0 = 0;                                      // an absent page: copies of no bytes, zeros in the ring
@@ -219,7 +257,7 @@ __global__ void __launch_bounds__(kva::kThreads, kva::per_sm(NT)) kv4_attention_
         const uint32_t at = (st * kStep) & pmask;
         const unsigned char* src0 = kbase + (uint64_t)pg0 * page_codes + at * ROWB;
         // the second half is the next 16 rows, or the first 16 of the next page
-        const unsigned char* src1 = p.page_shift == 4 ? kbase + (uint64_t)pg1 * page_codes : src0 + CODEB;
+        const unsigned char* src1 = PAGE16 ? kbase + (uint64_t)pg1 * page_codes : src0 + CODEB;
         const uint32_t d = dst + lane_dst;
 #pragma unroll
         for (int i = 0; i < CODEB / 512; ++i) {
@@ -229,7 +267,7 @@ __global__ void __launch_bounds__(kva::kThreads, kva::per_sm(NT)) kv4_attention_
           kva_cp16(d + 512 * i + 3 * CODEB, src1 + v_codes + 512 * i, ok1);
         }
         if (lane < 16) {                                        // 64 bytes of K scales, 64 of V scales, twice
-          const uint32_t row = p.page_shift == 4 ? 0u : at + (lane & 8) * 2;
+          const uint32_t row = PAGE16 ? 0u : at + (lane & 8) * 2;
           kva_cp16(dst + OFF_SC + lane * 16, sbase + (uint64_t)(lane < 8 ? pg0 : pg1) * page_scales + row * 4, lane < 8 ? ok0 : ok1);
         }
       }
@@ -238,9 +276,10 @@ __global__ void __launch_bounds__(kva::kThreads, kva::per_sm(NT)) kv4_attention_
 #pragma unroll
     for (int i = 0; i < kStages - 1; ++i) produce(first + i * kWarps, ring + i * STAGEB);
 
-    // ---- query fragments: k index 2c + e of step 2i + j is channel 8 (KS c + i) + 2j + 4e, k index 8 + 2c + e the one behind it
-    uint32_t qf[NT][4 * KS];
-    float f[NT][2], fq[NT][2];                  // of heads 8 nt + 2c + e: f up, f sum(q)
+    // ---- query digits: k index 4c + e of step i is channel 8 (KS c + i) + 2e, k index 16 + 4c + e the one behind it
+    uint32_t qf[NT][3][KS][2];
+    uint64_t f[NT], fq[NT];                     // pairs of heads 8 nt + 2c, 2c + 1: f times the unit of the digits, f sum(q)
+    int init[NT][2];                            // -8 times the digits' value, summed
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       const int h = nt * 8 + g;
@@ -280,32 +319,55 @@ __global__ void __launch_bounds__(kva::kThreads, kva::per_sm(NT)) kv4_attention_
         top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
         sum += __shfl_xor_sync(~0u, sum, o);
       }
-      // down = 2^-e, up = 2^e for 2^e <= top < 2^(e + 1), where both are normal numbers; 1 for zeros and infinities
+      // down = 2^(18 - e), up = 2^(e - 18) for 2^e <= top < 2^(e + 1); a row below 2^-107 counts as zeros, and one that is not
+      // finite (sum - sum is NaN then, or top is infinite) makes its scores NaN
       const int eb = (__float_as_int(top) >> 23) & 255;
-      const bool scaled = eb >= 1 && eb <= 253;
-      const float down = scaled ? __int_as_float((254 - eb) << 23) : 1.f, up = scaled ? __int_as_float(eb << 23) : 1.f;
+      const bool live = eb >= 20 && eb < 255;
+      const float down = live ? __int_as_float((272 - eb) << 23) : 0.f, up = live ? __int_as_float((eb - 18) << 23) : 0.f;
+      int digits[3] = {0, 0, 0};                // their sums
 #pragma unroll
       for (int i = 0; i < KS; ++i)
 #pragma unroll
-        for (int n = 0; n < 4; ++n) {
-          const __half2 h2 = __floats2half2_rn(v[8 * i + n] * down, v[8 * i + n + 4] * down);
-          qf[nt][4 * i + n] = *reinterpret_cast<const uint32_t*>(&h2);
-        }
-      const float fh = p.scale_log2 * up, fs = p.scale_log2 * sum;
+        for (int odd = 0; odd < 2; ++odd) {
+          uint32_t w[3] = {0, 0, 0};
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {             // heads 2c and 2c + 1 are lanes' g = 2c, 2c + 1
-        f[nt][e] = __shfl_sync(~0u, fh, (2 * c + e) * 4);
-        fq[nt][e] = __shfl_sync(~0u, fs, (2 * c + e) * 4);
-      }
+          for (int e = 0; e < 4; ++e) {
+            // q down rounded to an integer in the low bits of a float, raised by 64 (1 + 128 + 128^2) to stay
+            // between 0 and 2^21: base-128 digits 0 to 127
+            const uint32_t x = __float_as_uint(fmaf(v[8 * i + 2 * e + odd], down, 12582912.f + 1056832.f));
+#pragma unroll
+            for (int k = 0; k < 3; ++k) {
+              const int right = 7 * (2 - k) - 8 * e;
+              w[k] |= (right >= 0 ? x >> right : x << -right) & (127u << (8 * e));
+            }
+          }
+#pragma unroll
+          for (int k = 0; k < 3; ++k) {         // less 64, all four bytes at once: bit 6 becomes the sign
+            w[k] = (w[k] ^ 0x40404040u) | ((~w[k] & 0x40404040u) << 1);
+            digits[k] = __dp4a((int)w[k], 0x01010101, digits[k]);
+            qf[nt][k][i][odd] = w[k];
+          }
+        }
+      int value = (digits[0] * 128 + digits[1]) * 128 + digits[2];
+#pragma unroll
+      for (int o = 1; o < 4; o <<= 1) value += __shfl_xor_sync(~0u, value, o);
+      const float fh = eb == 255 ? __int_as_float(0x7fffffff) : p.scale_log2 * up + (sum - sum), fs = p.scale_log2 * sum;
+      // heads 2c and 2c + 1 are lanes' g = 2c, 2c + 1
+      f[nt] = kva_two(__shfl_sync(~0u, fh, 8 * c), __shfl_sync(~0u, fh, 8 * c + 4));
+      fq[nt] = kva_two(__shfl_sync(~0u, fs, 8 * c), __shfl_sync(~0u, fs, 8 * c + 4));
+#pragma unroll
+      for (int e = 0; e < 2; ++e) init[nt][e] = -8 * __shfl_sync(~0u, value, 8 * c + 4 * e);
     }
 
-    float o[NT][MT][4], M[NT][2], L[NT][2], Z[NT][2];
+    float o[NT][MT][4], M[NT][2];
+    uint64_t L[NT], Z[NT];                      // of the two heads
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
       for (int i = 0; i < MT; ++i) o[nt][i][0] = o[nt][i][1] = o[nt][i][2] = o[nt][i][3] = 0.f;
 #pragma unroll
-      for (int e = 0; e < 2; ++e) { M[nt][e] = kFloor; L[nt][e] = Z[nt][e] = 0.f; }
+      for (int e = 0; e < 2; ++e) M[nt][e] = kFloor;
+      L[nt] = Z[nt] = 0;
     }
 
     uint32_t slot = ring, fill = ring + (kStages - 1) * STAGEB;
@@ -314,29 +376,27 @@ __global__ void __launch_bounds__(kva::kThreads, kva::per_sm(NT)) kv4_attention_
       fill = slot;
       asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
       __syncwarp();
-      // ---- what the 32 tokens' scales stand for, one token a lane: s, m f-less, log2 s', 1 / s', m' / s'
+      // ---- what the 32 tokens' scales stand for, one token a lane: s, m, log2 s', 1 / s', m' / s',
+      // each twice, since they are multiplied into pairs of heads
       {
         const uint32_t at = slot + OFF_SC + (lane >> 4) * 128 + (lane & 15) * 4;
-        const uint32_t km = kva_lds32(at), vm = kva_lds32(at + 64);
+        const uint32_t k0 = kva_lds32(at), v0 = kva_lds32(at + 64);
+        const bool real = lane < len - st * kStep && (v0 & 0xffff) != 0;        // a scale of 0: never written, or an absent page
+        const uint32_t km = real ? k0 : 0, vm = real ? v0 : 0x3c00u;
         const float2 kf = __half22float2(*reinterpret_cast<const __half2*>(&km));
         const float2 vf = __half22float2(*reinterpret_cast<const __half2*>(&vm));
-        const bool real = lane < len - st * kStep && vf.x != 0.f;     // a scale of 0: never written, or an absent page
-        const float vs = real ? fmaxf(vf.x, 5.9604645e-8f) : 1.f, r = kva_rcp(vs);
-        asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(meta + lane * 16), "f"(real ? kf.x : 0.f),
-                     "f"(real ? fmaf(8.f, kf.x, kf.y) : 0.f), "f"(real ? kva_log2(vs) : -INFINITY), "f"(r) : "memory");
-        asm volatile("st.shared.f32 [%0], %1;" ::"r"(meta + kStep * 16 + lane * 4), "f"(real ? fmaf(8.f, vf.x, vf.y) * r : 0.f) : "memory");
+        // (kf, vf: zeros, and a scale of 1 with weight 0, where there is no token)
+        const float ks = kf.x, km8 = fmaf(8.f, kf.x, kf.y), ls = real ? kva_log2(vf.x) : -INFINITY;
+        const float r = kva_rcp(vf.x), rz = fmaf(8.f, vf.x, vf.y) * r;
+        asm volatile("st.shared.v4.f32 [%0], {%1, %1, %2, %2};" ::"r"(meta + lane * 16), "f"(ks), "f"(km8) : "memory");
+        asm volatile("st.shared.v4.f32 [%0], {%1, %1, %2, %2};" ::"r"(meta + kStep * 16 + lane * 16), "f"(ls), "f"(r) : "memory");
+        asm volatile("st.shared.v2.f32 [%0], {%1, %1};" ::"r"(meta + kStep * 32 + lane * 8), "f"(rz) : "memory");
       }
       __syncwarp();
       // ---- scores
-      float x[2][NT][4];
+      uint64_t x[2][NT][2];                     // pairs of heads of tokens tok_a and tok_a + 8 of each half
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        float x2[NT][4];
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          x[h][nt][0] = x[h][nt][1] = x[h][nt][2] = x[h][nt][3] = 0.f;
-          x2[nt][0] = x2[nt][1] = x2[nt][2] = x2[nt][3] = 0.f;  // a second chain of sums: half the latency
-        }
         uint32_t wa[KS], wb[KS];
         if (DP == 128) {
           const uint32_t ad = slot + h * CODEB + tok_a * ROWB + ((c * 16) ^ ((tok_a & 2) << 4));
@@ -349,61 +409,68 @@ __global__ void __launch_bounds__(kva::kThreads, kva::per_sm(NT)) kv4_attention_
           wa[0] = a.x; wa[1] = a.y;
           wb[0] = e.x; wb[1] = e.y;
         }
+        uint32_t a[KS][4];
 #pragma unroll
         for (int i = 0; i < KS; ++i) {
-          const uint32_t a8 = wa[i] >> 8, b8 = wb[i] >> 8;
-          const uint32_t lo[4] = {kv4_pair(wa[i], 0x64086408u), kv4_pair(wb[i], 0x64086408u),
-                                  kv4_pair_hi(wa[i], 0xd480d480u), kv4_pair_hi(wb[i], 0xd480d480u)};
-          const uint32_t hi[4] = {kv4_pair(a8, 0x64086408u), kv4_pair(b8, 0x64086408u),
-                                  kv4_pair_hi(a8, 0xd480d480u), kv4_pair_hi(b8, 0xd480d480u)};
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            mma_m16n8k16(x[h][nt], lo, qf[nt][4 * i], qf[nt][4 * i + 1]);
-            mma_m16n8k16(x2[nt], hi, qf[nt][4 * i + 2], qf[nt][4 * i + 3]);
-          }
+          a[i][0] = wa[i] & 0x0f0f0f0fu;
+          a[i][1] = wb[i] & 0x0f0f0f0fu;
+          a[i][2] = (wa[i] >> 4) & 0x0f0f0f0fu;
+          a[i][3] = (wb[i] >> 4) & 0x0f0f0f0fu;
         }
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+        for (int nt = 0; nt < NT; ++nt) {
+          // three chains side by side: one behind the other, as the starts of the next, their latency shows (249 us against 236)
+          int acc[3][4] = {{0, 0, 0, 0}, {0, 0, 0, 0}, {init[nt][0], init[nt][1], init[nt][0], init[nt][1]}};
 #pragma unroll
-          for (int e = 0; e < 4; ++e) x[h][nt][e] += x2[nt][e];
+          for (int i = 0; i < KS; ++i)
+#pragma unroll
+            for (int k = 0; k < 3; ++k) kva_mma_u8s8(acc[k], a[i], qf[nt][k][i][0], qf[nt][k][i][1]);
+          int sum[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) sum[e] = (acc[0][e] * 128 + acc[1][e]) * 128 + acc[2][e];
+          x[h][nt][0] = kva_two(__int2float_rn(sum[0]), __int2float_rn(sum[1]));
+          x[h][nt][1] = kva_two(__int2float_rn(sum[2]), __int2float_rn(sum[3]));
+        }
       }
       // ---- weights
-      float rs[2][2], rz[2][2];
-      bool over = false;
+      uint64_t rs[2][2], rz[2][2];
+      float over = -INFINITY;
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
           const int t = 16 * h + tok_a + 8 * r;
-          const uint4 w = lds128(meta + t * 16);
-          const float s = __uint_as_float(w.x), m = __uint_as_float(w.y), ls = __uint_as_float(w.z);
-          rs[h][r] = __uint_as_float(w.w);
-          rz[h][r] = __uint_as_float(kva_lds32(meta + kStep * 16 + t * 4));
+          uint64_t s, m, ls;
+          kva_lds2(meta + t * 16, s, m);
+          kva_lds2(meta + kStep * 16 + t * 16, ls, rs[h][r]);
+          const uint2 z = lds64(meta + kStep * 32 + t * 8);
+          rz[h][r] = kva_two(__uint_as_float(z.x), __uint_as_float(z.y));
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const float y = fmaf(x[h][nt][2 * r + e] * s, f[nt][e], fmaf(m, fq[nt][e], ls));
-              x[h][nt][2 * r + e] = y;
-              over |= y > M[nt][e] + 8.f;
-            }
+          for (int nt = 0; nt < NT; ++nt) {
+            x[h][nt][r] = kva_fma2(kva_mul2(x[h][nt][r], s), f[nt], kva_fma2(m, fq[nt], ls));
+            const float2 y = kva_split(kva_add2(x[h][nt][r], kva_two(-M[nt][0], -M[nt][1])));
+            over = fmaxf(over, fmaxf(y.x, y.y));
+          }
         }
-      if (__any_sync(~0u, over)) {
+      if (__any_sync(~0u, over > 8.f)) {
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+        for (int nt = 0; nt < NT; ++nt) {
+          const float2 y0 = kva_split(x[0][nt][0]), y1 = kva_split(x[0][nt][1]), y2 = kva_split(x[1][nt][0]), y3 = kva_split(x[1][nt][1]);
+          float top[2] = {fmaxf(fmaxf(y0.x, y1.x), fmaxf(y2.x, y3.x)), fmaxf(fmaxf(y0.y, y1.y), fmaxf(y2.y, y3.y))}, k[2];
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            float top = fmaxf(fmaxf(x[0][nt][e], x[0][nt][2 + e]), fmaxf(x[1][nt][e], x[1][nt][2 + e]));
 #pragma unroll
-            for (int s = 4; s < 32; s <<= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, s));
-            top = fmaxf(top, M[nt][e]);
-            const float k = kva_exp2(M[nt][e] - top);
-            M[nt][e] = top;
-            L[nt][e] *= k;
-            Z[nt][e] *= k;
+            for (int s = 4; s < 32; s <<= 1) top[e] = fmaxf(top[e], __shfl_xor_sync(~0u, top[e], s));
+            top[e] = fmaxf(top[e], M[nt][e]);
+            k[e] = kva_exp2(M[nt][e] - top[e]);
+            M[nt][e] = top[e];
 #pragma unroll
-            for (int i = 0; i < MT; ++i) { o[nt][i][e] *= k; o[nt][i][2 + e] *= k; }
+            for (int i = 0; i < MT; ++i) { o[nt][i][e] *= k[e]; o[nt][i][2 + e] *= k[e]; }
           }
+          const uint64_t k2 = kva_two(k[0], k[1]);
+          L[nt] = kva_mul2(L[nt], k2);
+          Z[nt] = kva_mul2(Z[nt], k2);
+        }
       }
       // ---- weighted sums of the codes
 #pragma unroll
@@ -413,14 +480,12 @@ __global__ void __launch_bounds__(kva::kThreads, kva::per_sm(NT)) kv4_attention_
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
-            float w[2];
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              w[e] = kva_exp2(x[h][nt][2 * r + e] - M[nt][e]);
-              L[nt][e] = fmaf(w[e], rs[h][r], L[nt][e]);
-              Z[nt][e] = fmaf(w[e], rz[h][r], Z[nt][e]);
-            }
-            const __half2 h2 = __floats2half2_rn(w[0], w[1]);
+            const float2 y = kva_split(kva_add2(x[h][nt][r], kva_two(-M[nt][0], -M[nt][1])));
+            const float2 w = make_float2(kva_exp2(y.x), kva_exp2(y.y));
+            const uint64_t w2 = kva_two(w.x, w.y);
+            L[nt] = kva_fma2(w2, rs[h][r], L[nt]);
+            Z[nt] = kva_fma2(w2, rz[h][r], Z[nt]);
+            const __half2 h2 = __floats2half2_rn(w.x, w.y);
             pb[nt][r] = kva_transpose(*reinterpret_cast<const uint32_t*>(&h2));
           }
         const uint32_t sv = slot + (2 + h) * CODEB;
@@ -465,21 +530,24 @@ __global__ void __launch_bounds__(kva::kThreads, kva::per_sm(NT)) kv4_attention_
 
     // ---- join the warps: sums over the lanes that share a head, then over the warps through shared memory
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
+    for (int nt = 0; nt < NT; ++nt) {
+      const float2 l2 = kva_split(L[nt]), z2 = kva_split(Z[nt]);
+      float l[2] = {l2.x, l2.y}, z[2] = {z2.x, z2.y};
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
 #pragma unroll
         for (int s = 4; s < 32; s <<= 1) {
-          L[nt][e] += __shfl_xor_sync(~0u, L[nt][e], s);
-          Z[nt][e] += __shfl_xor_sync(~0u, Z[nt][e], s);
+          l[e] += __shfl_xor_sync(~0u, l[e], s);
+          z[e] += __shfl_xor_sync(~0u, z[e], s);
         }
         if (g == 0) {
           const int h = nt * 8 + 2 * c + e;
           s_m[warp][h] = M[nt][e];
-          s_l[warp][h] = L[nt][e];
-          s_z[warp][h] = Z[nt][e];
+          s_l[warp][h] = l[e];
+          s_z[warp][h] = z[e];
         }
       }
+    }
     __syncthreads();                            // every warp has read its ring: it becomes the exchange area
     float* ex = reinterpret_cast<float*>(smem);   // [warp][head][DP]
 #pragma unroll
@@ -578,7 +646,7 @@ __global__ void __launch_bounds__(kva::kThreads, kva::per_sm(NT)) kv4_attention_
 
 template <int DP, int NT>
 static constexpr size_t kva_smem() {
-  const size_t ring = (size_t)kva::kWarps * (kva::kStages * (32 * DP + 256) + kva::kStep * 20);
+  const size_t ring = (size_t)kva::kWarps * (kva::kStages * (32 * DP + 256) + kva::kStep * 40);
   const size_t ex = (size_t)kva::kWarps * 8 * NT * DP * 4;
   return ring > ex ? ring : ex;
 }
@@ -589,17 +657,17 @@ static int kva_ctas(int nt) {
 }
 static int kva_nt(int64_t heads, int64_t kv_heads) { return heads / kv_heads > 8 ? 2 : 1; }
 
-template <int DP, int NT>
+template <int DP, int NT, bool PAGE16>
 static int kva_launch(KvaParams& p, cudaStream_t stream) {
   static thread_local bool attr_set[64] = {};
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev < 0 || dev >= 64 || !attr_set[dev]) {
-    UNIQL_CUDA_TRY(cudaFuncSetAttribute(kv4_attention_kernel<DP, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    UNIQL_CUDA_TRY(cudaFuncSetAttribute(kv4_attention_kernel<DP, NT, PAGE16>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                         (int)kva_smem<DP, NT>()));
     if (dev >= 0 && dev < 64) attr_set[dev] = true;
   }
-  return launch_pdl(kv4_attention_kernel<DP, NT>, (unsigned)kva_ctas(NT), kva::kThreads, kva_smem<DP, NT>(), stream, p);
+  return launch_pdl(kv4_attention_kernel<DP, NT, PAGE16>, (unsigned)kva_ctas(NT), kva::kThreads, kva_smem<DP, NT>(), stream, p);
 }
 
 }  // namespace uniql
@@ -645,6 +713,10 @@ extern "C" int uniql_kv4_attention(const void* q, int64_t q_batch_stride, int64_
   p.q_vec = aligned16(q) && !((q_batch_stride | q_head_stride) & 7);
   p.scale_log2 = softmax_scale * 1.44269504088896340736f;
   cudaStream_t s = (cudaStream_t)stream;
-  if (dp == 128) return nt == 1 ? kva_launch<128, 1>(p, s) : kva_launch<128, 2>(p, s);
-  return nt == 1 ? kva_launch<64, 1>(p, s) : kva_launch<64, 2>(p, s);
+  auto launch = [&](auto small) {
+    constexpr bool P16 = decltype(small)::value;
+    if (dp == 128) return nt == 1 ? kva_launch<128, 1, P16>(p, s) : kva_launch<128, 2, P16>(p, s);
+    return nt == 1 ? kva_launch<64, 1, P16>(p, s) : kva_launch<64, 2, P16>(p, s);
+  };
+  return page_size == 16 ? launch(std::true_type{}) : launch(std::false_type{});
 }

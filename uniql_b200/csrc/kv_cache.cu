@@ -483,7 +483,7 @@ extern "C" int uniql_kv_page_plan(const int32_t* lens, const int32_t* new_lens, 
     attr[1].val.clusterDim.x = (unsigned)cluster;
     attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 2;
+    cfg.numAttrs = cluster > 1 ? 2 : 1;         // a cluster launch costs the host 3 us more
     UNIQL_CUDA_TRY(cudaLaunchKernelEx(&cfg, kv_page_plan_kernel, (const PlanParams&)p));
     return (int)UNIQL_OK;
   };
