@@ -156,10 +156,11 @@ __global__ void __launch_bounds__(kPlanThreads) kv_page_plan_kernel(const __grid
 // (eight: 50 us for 14760 tokens of 8 heads, 121 MB read; sixteen: 31).  (hi - lo) / 15 is the quotient by the reciprocal and one
 // residual step (Markstein), equal to the division for every mantissa.
 //
-// Codes.  y = (x - z) * (1 / s) is within 2^-22 of the quotient (relative).  Where that leaves the side of a half-way point
-// open, the two sides are compared exactly: x - z spans at most 41 bits and (k + 1/2) * s sixteen, both exact in fp64.
+// Codes are taken from a quotient in fp32.  Where that leaves the side of a half-way point open, the two sides are compared
+// exactly: x - z spans at most 41 bits and (k + 1/2) * s sixteen, both exact in fp64.
 constexpr float kRound = 12582912.f;            // 1.5 * 2^23
 __device__ __noinline__ uint32_t kv4_exact_code(float x, float z, float s, float y) {
+  // y: the quotient within 2^-22 (relative), so its integer part lies on the right side of the half-way point below it
   const float k = floorf(fminf(fmaxf(y, 0.f), 15.f));
   const double d = (double)x - (double)z, mid = ((double)k + 0.5) * (double)s;
   const int ki = (int)k;
@@ -262,35 +263,31 @@ __global__ void __launch_bounds__(kAppendThreads) kv4_append_kernel(const __grid
     const float s = __half2float(sh), z = __half2float(zh);
     float inv;
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(s));
+    // The usual row: y = x / s - z / s in one fused step, which is within 2^-17 of the quotient while |z / s| is at most 64, and no
+    // quotient leaves 0..15 by half a step (z is the minimum itself, s is off by less than 1/30).  Any other row takes the exact
+    // comparisons throughout, as does a half row with a quotient near a half-way point.
+    const float zi = -z * inv;
+    const bool odd = wide || z != lo || fabsf(zi) > 64.f || s < 1e-6f;
     uint32_t word[2] = {0, 0};
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       if (!mine[j] || nan) continue;
       const uint32_t u[4] = {raw[j].x, raw[j].y, raw[j].z, raw[j].w};
-      float x[8], y[8], far = 0.f;
+      float far = odd ? 1.f : 0.f;
+      constexpr uint32_t kBits = 0x4b400000u;   // of kRound; what eight of them add to the word:
+      constexpr uint32_t kAll = kBits + (kBits << 4) + (kBits << 8) + (kBits << 12) + (kBits << 16) + (kBits << 20) + (kBits << 24) + (kBits << 28);
+      uint32_t w = 0u - kAll;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         float2 f;
         if constexpr (BF16) f = __bfloat1622float2(*reinterpret_cast<const T2*>(&u[e]));
         else f = __half22float2(*reinterpret_cast<const T2*>(&u[e]));
-        x[2 * e] = f.x;
-        x[2 * e + 1] = f.y;
+        const float y0 = fmaf(f.x, inv, zi), y1 = fmaf(f.y, inv, zi);
+        const float up0 = y0 + kRound, up1 = y1 + kRound;
+        far = fmaxf(far, fmaxf(fabsf(y0 - (up0 - kRound)), fabsf(y1 - (up1 - kRound))));
+        w += (__float_as_uint(up0) << (8 * e)) + (__float_as_uint(up1) << (8 * e + 4));
       }
-      if (wide) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = fminf(fmaxf(x[e], -65504.f), 65504.f);
-      }
-      constexpr uint32_t kBits = 0x4b400000u;   // of kRound; what eight of them add to the word:
-      constexpr uint32_t kAll = kBits + (kBits << 4) + (kBits << 8) + (kBits << 12) + (kBits << 16) + (kBits << 20) + (kBits << 24) + (kBits << 28);
-      uint32_t w = 0u - kAll;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        y[e] = fminf(fmaxf((x[e] - z) * inv, 0.f), 15.f);
-        const float up = y[e] + kRound;
-        far = fmaxf(far, fabsf(y[e] - (up - kRound)));
-        w += __float_as_uint(up) << (4 * e);
-      }
-      if (far > 0.49998f) {                     // some quotient within 2e-5 of a half-way point
+      if (far > 0.49998f) {                     // some quotient within 2e-5 of a half-way point, or an odd row
         w = 0;
 #pragma unroll 1
         for (int e = 0; e < 8; ++e) {
@@ -516,7 +513,8 @@ extern "C" int uniql_kv4_append(const void* k, int64_t k_token_stride, int64_t k
   const bool bf16 = dtype == UNIQL_BF16;
   auto kernel = dp == 128 ? (bf16 ? kv4_append_kernel<128, true> : kv4_append_kernel<128, false>)
                           : (bf16 ? kv4_append_kernel<64, true> : kv4_append_kernel<64, false>);
-  const int64_t per = kAppendThreads / (dp / 16), cap = 8 * (int64_t)device_info().sm_count;
+  // one wave: six CTAs of 40 registers a thread fit an SM
+  const int64_t per = kAppendThreads / (dp / 16), cap = 6 * (int64_t)device_info().sm_count;
   const int64_t slab = ((int64_t)1 << 30) / (2 * kv_heads);             // tokens of a launch: rows stay below 2^31
   for (int64_t t0 = 0; t0 < tokens; t0 += slab) {
     const int64_t n = tokens - t0 < slab ? tokens - t0 : slab;

@@ -310,6 +310,16 @@ CacheView check_cache(const at::Tensor& codes, const at::Tensor& scales) {
   return {codes.size(0), codes.size(2), codes.size(3), codes.size(4) * 8};
 }
 
+// A 1-D tensor over part of a byte buffer: several results of one call share an allocation, which costs a microsecond.
+at::Tensor part_of(const at::Tensor& bytes, int64_t offset, int64_t n, at::ScalarType type) {
+  auto dtype = c10::scalarTypeToTypeMeta(type);
+  at::Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(bytes.storage()), bytes.key_set(), dtype);
+  auto* impl = t.unsafeGetTensorImpl();
+  impl->set_storage_offset(offset / (int64_t)dtype.itemsize());
+  impl->set_sizes_contiguous({n});
+  return t;
+}
+
 std::vector<at::Tensor> kv_page_plan(const at::Tensor& lens, const at::Tensor& new_lens, const at::Tensor& block_table,
                                      const at::Tensor& free_pages, const at::Tensor& free_count, int64_t page_size,
                                      int64_t total_new, bool in_place) {
@@ -325,11 +335,12 @@ std::vector<at::Tensor> kv_page_plan(const at::Tensor& lens, const at::Tensor& n
   TORCH_CHECK(total_new >= 0, "total_new must not be negative");
   const c10::cuda::CUDAGuard guard(lens.device());
   const int dev = lens.device().index();
-  const auto i64 = lens.options().dtype(at::kLong);
-  at::Tensor slots = at::empty({total_new}, i64), positions = at::empty({total_new}, i64);
-  at::Tensor cu = at::empty({batch + 1}, lens.options());
-  at::Tensor lens_out = in_place ? lens : at::empty({batch}, lens.options());
-  at::Tensor count_out = in_place ? free_count : at::empty({1}, lens.options());
+  const int64_t longs = 16 * total_new, ints = 4 * (batch + 1);
+  at::Tensor buf = at::empty({longs + 2 * ints + 4}, lens.options().dtype(at::kByte));
+  at::Tensor slots = part_of(buf, 0, total_new, at::kLong), positions = part_of(buf, 8 * total_new, total_new, at::kLong);
+  at::Tensor cu = part_of(buf, longs, batch + 1, at::kInt);
+  at::Tensor lens_out = in_place ? lens : part_of(buf, longs + ints, batch, at::kInt);
+  at::Tensor count_out = in_place ? free_count : part_of(buf, longs + 2 * ints, 1, at::kInt);
   at::Tensor status = status_tensor(dev);
   const int code = uniql_kv_page_plan(
       (const int32_t*)lens.data_ptr(), (const int32_t*)new_lens.data_ptr(), batch, (int32_t*)block_table.data_ptr(),
