@@ -92,32 +92,6 @@ __device__ __forceinline__ void kva_mma_u8s8(int (&d)[4], const uint32_t (&a)[4]
       : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// Two floats side by side (two heads of a token): one instruction of the FMA pipe for both.
-__device__ __forceinline__ uint64_t kva_two(float a, float b) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-  return r;
-}
-__device__ __forceinline__ float2 kva_split(uint64_t v) {
-  float2 f;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(v));
-  return f;
-}
-__device__ __forceinline__ uint64_t kva_fma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
-__device__ __forceinline__ uint64_t kva_mul2(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ uint64_t kva_add2(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
 __device__ __forceinline__ void kva_lds2(uint32_t a, uint64_t& x, uint64_t& y) {
   asm volatile("ld.shared.v2.u64 {%0, %1}, [%2];" : "=l"(x), "=l"(y) : "r"(a) : "memory");
 }
@@ -353,8 +327,8 @@ __global__ void __launch_bounds__(kva::kThreads, kva::per_sm(NT)) kv4_attention_
       for (int o = 1; o < 4; o <<= 1) value += __shfl_xor_sync(~0u, value, o);
       const float fh = eb == 255 ? __int_as_float(0x7fffffff) : p.scale_log2 * up + (sum - sum), fs = p.scale_log2 * sum;
       // heads 2c and 2c + 1 are lanes' g = 2c, 2c + 1
-      f[nt] = kva_two(__shfl_sync(~0u, fh, 8 * c), __shfl_sync(~0u, fh, 8 * c + 4));
-      fq[nt] = kva_two(__shfl_sync(~0u, fs, 8 * c), __shfl_sync(~0u, fs, 8 * c + 4));
+      f[nt] = two(__shfl_sync(~0u, fh, 8 * c), __shfl_sync(~0u, fh, 8 * c + 4));
+      fq[nt] = two(__shfl_sync(~0u, fs, 8 * c), __shfl_sync(~0u, fs, 8 * c + 4));
 #pragma unroll
       for (int e = 0; e < 2; ++e) init[nt][e] = -8 * __shfl_sync(~0u, value, 8 * c + 4 * e);
     }
@@ -428,8 +402,8 @@ __global__ void __launch_bounds__(kva::kThreads, kva::per_sm(NT)) kv4_attention_
           int sum[4];
 #pragma unroll
           for (int e = 0; e < 4; ++e) sum[e] = (acc[0][e] * 128 + acc[1][e]) * 128 + acc[2][e];
-          x[h][nt][0] = kva_two(__int2float_rn(sum[0]), __int2float_rn(sum[1]));
-          x[h][nt][1] = kva_two(__int2float_rn(sum[2]), __int2float_rn(sum[3]));
+          x[h][nt][0] = two(__int2float_rn(sum[0]), __int2float_rn(sum[1]));
+          x[h][nt][1] = two(__int2float_rn(sum[2]), __int2float_rn(sum[3]));
         }
       }
       // ---- weights
@@ -444,18 +418,18 @@ __global__ void __launch_bounds__(kva::kThreads, kva::per_sm(NT)) kv4_attention_
           kva_lds2(meta + t * 16, s, m);
           kva_lds2(meta + kStep * 16 + t * 16, ls, rs[h][r]);
           const uint2 z = lds64(meta + kStep * 32 + t * 8);
-          rz[h][r] = kva_two(__uint_as_float(z.x), __uint_as_float(z.y));
+          rz[h][r] = two(__uint_as_float(z.x), __uint_as_float(z.y));
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
-            x[h][nt][r] = kva_fma2(kva_mul2(x[h][nt][r], s), f[nt], kva_fma2(m, fq[nt], ls));
-            const float2 y = kva_split(kva_add2(x[h][nt][r], kva_two(-M[nt][0], -M[nt][1])));
+            x[h][nt][r] = fma2(mul2(x[h][nt][r], s), f[nt], fma2(m, fq[nt], ls));
+            const float2 y = split2(add2(x[h][nt][r], two(-M[nt][0], -M[nt][1])));
             over = fmaxf(over, fmaxf(y.x, y.y));
           }
         }
       if (__any_sync(~0u, over > 8.f)) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          const float2 y0 = kva_split(x[0][nt][0]), y1 = kva_split(x[0][nt][1]), y2 = kva_split(x[1][nt][0]), y3 = kva_split(x[1][nt][1]);
+          const float2 y0 = split2(x[0][nt][0]), y1 = split2(x[0][nt][1]), y2 = split2(x[1][nt][0]), y3 = split2(x[1][nt][1]);
           float top[2] = {fmaxf(fmaxf(y0.x, y1.x), fmaxf(y2.x, y3.x)), fmaxf(fmaxf(y0.y, y1.y), fmaxf(y2.y, y3.y))}, k[2];
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
@@ -467,9 +441,9 @@ __global__ void __launch_bounds__(kva::kThreads, kva::per_sm(NT)) kv4_attention_
 #pragma unroll
             for (int i = 0; i < MT; ++i) { o[nt][i][e] *= k[e]; o[nt][i][2 + e] *= k[e]; }
           }
-          const uint64_t k2 = kva_two(k[0], k[1]);
-          L[nt] = kva_mul2(L[nt], k2);
-          Z[nt] = kva_mul2(Z[nt], k2);
+          const uint64_t k2 = two(k[0], k[1]);
+          L[nt] = mul2(L[nt], k2);
+          Z[nt] = mul2(Z[nt], k2);
         }
       }
       // ---- weighted sums of the codes
@@ -480,11 +454,11 @@ __global__ void __launch_bounds__(kva::kThreads, kva::per_sm(NT)) kv4_attention_
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
-            const float2 y = kva_split(kva_add2(x[h][nt][r], kva_two(-M[nt][0], -M[nt][1])));
+            const float2 y = split2(add2(x[h][nt][r], two(-M[nt][0], -M[nt][1])));
             const float2 w = make_float2(kva_exp2(y.x), kva_exp2(y.y));
-            const uint64_t w2 = kva_two(w.x, w.y);
-            L[nt] = kva_fma2(w2, rs[h][r], L[nt]);
-            Z[nt] = kva_fma2(w2, rz[h][r], Z[nt]);
+            const uint64_t w2 = two(w.x, w.y);
+            L[nt] = fma2(w2, rs[h][r], L[nt]);
+            Z[nt] = fma2(w2, rz[h][r], Z[nt]);
             const __half2 h2 = __floats2half2_rn(w.x, w.y);
             pb[nt][r] = kva_transpose(*reinterpret_cast<const uint32_t*>(&h2));
           }
@@ -531,7 +505,7 @@ __global__ void __launch_bounds__(kva::kThreads, kva::per_sm(NT)) kv4_attention_
     // ---- join the warps: sums over the lanes that share a head, then over the warps through shared memory
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      const float2 l2 = kva_split(L[nt]), z2 = kva_split(Z[nt]);
+      const float2 l2 = split2(L[nt]), z2 = split2(Z[nt]);
       float l[2] = {l2.x, l2.y}, z[2] = {z2.x, z2.y};
 #pragma unroll
       for (int e = 0; e < 2; ++e) {

@@ -149,11 +149,12 @@ __global__ void __launch_bounds__(kPlanThreads) kv_page_plan_kernel(const __grid
 }
 
 // ------------------------------------------------------------------------------------------------ append
-// A row (one token, one head, K or V) is DP / 16 lanes with sixteen channels each: two 16-byte loads, the extremes over the lanes
+// A row (one token, one head) is DP / 16 lanes with sixteen channels each: two 16-byte loads, the extremes over the lanes
 // (least value and negated greatest one as a 16-bit pair: one shuffle a level), two packed words stored.  HBM-bound by the
 // reads, 4 bytes a channel against 0.5 written, if the instructions are few: the packed minimum carries NaN along, the codes
 // are rounded by adding 1.5 * 2^23 and joined as the low bits of those sums, and sixteen channels a lane share what a row costs
-// (eight: 50 us for 14760 tokens of 8 heads, 121 MB read; sixteen: 31).  (hi - lo) / 15 is the quotient by the reciprocal and one
+// (eight: 50 us for 14760 tokens of 8 heads, 60 MB read; sixteen: 34; with K's and V's rows in one turn and packed
+// arithmetic: 30).  (hi - lo) / 15 is the quotient by the reciprocal and one
 // residual step (Markstein), equal to the division for every mantissa.
 //
 // Codes are taken from a quotient in fp32.  Where that leaves the side of a half-way point open, the two sides are compared
@@ -175,12 +176,12 @@ struct AppendParams {
   __half2* scales;
   int* status_word;
   int64_t num_slots;
-  uint32_t rows;                                // tokens * 2 * heads, below 2^31
+  uint32_t rows;                                // tokens * heads, below 2^31
   FastDiv heads;
   int d[2], page_shift;
 };
 
-constexpr int kAppendThreads = 256;
+constexpr int kAppendThreads = 256, kAppendCtas = 6;      // CTAs an SM holds: one wave
 
 template <bool BF16>
 struct Pair16 {
@@ -192,7 +193,7 @@ struct Pair16<true> {
 };
 
 template <int DP, bool BF16>
-__global__ void __launch_bounds__(kAppendThreads) kv4_append_kernel(const __grid_constant__ AppendParams p) {
+__global__ void __launch_bounds__(kAppendThreads, kAppendCtas) kv4_append_kernel(const __grid_constant__ AppendParams p) {
   constexpr int W = DP / 16;                    // lanes of a row
   using T2 = typename Pair16<BF16>::T;
   pdl_wait();
@@ -204,20 +205,26 @@ __global__ void __launch_bounds__(kAppendThreads) kv4_append_kernel(const __grid
   const uint32_t first = blockIdx.x * (kAppendThreads / W) + threadIdx.x / W, ahead = (threadIdx.x % 32) / W;
   for (uint32_t r = first; r - ahead < p.rows; r += step) {
     const bool live = r < p.rows;
-    const uint32_t pair = live ? p.heads.quot(r) : 0, h = live ? r - pair * p.heads.d : 0, t = pair >> 1;
-    const int kv = pair & 1;
+    const uint32_t t = live ? p.heads.quot(r) : 0, h = live ? r - t * p.heads.d : 0;
     const int64_t slot = live ? p.slots[t] : -1;
     const bool stored = slot >= 0 && slot < p.num_slots;
-    const int left = (kv ? p.d[1] : p.d[0]) - (int)sub * 16;    // channels from this lane's first on
-    const bool mine[2] = {stored && left > 0, stored && left > 8};
-    uint4 raw[2];
-    const unsigned char* src = (kv ? p.src[1] : p.src[0]) +
-                               2 * (t * (kv ? p.token_stride[1] : p.token_stride[0]) + h * (kv ? p.head_stride[1] : p.head_stride[0]) + sub * 16);
+    if (live && !stored && slot != -1 && sub == 0 && p.status_word) atomicOr(p.status_word, UNIQL_STATUS_BAD_INDEX);
+    // K's row and V's row of the token and head: one index, both loads in flight
+    uint4 raws[2][2];
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      raw[j] = make_uint4(0, 0, 0, 0);
-      if (mine[j]) raw[j] = *reinterpret_cast<const uint4*>(src + 16 * j);
+    for (int kv = 0; kv < 2; ++kv) {
+      const unsigned char* src = p.src[kv] + 2 * (t * p.token_stride[kv] + h * p.head_stride[kv] + sub * 16);
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        raws[kv][j] = make_uint4(0, 0, 0, 0);
+        if (stored && (int)sub * 16 + 8 * j < p.d[kv]) raws[kv][j] = *reinterpret_cast<const uint4*>(src + 16 * j);
+      }
     }
+    const int64_t krow = ((((slot >> p.page_shift) * 2) * p.heads.d + h) << p.page_shift) + (slot & ((1 << p.page_shift) - 1));
+#pragma unroll
+    for (int kv = 0; kv < 2; ++kv) {
+    const uint4 (&raw)[2] = raws[kv];
+    const bool mine[2] = {stored && (int)sub * 16 < p.d[kv], stored && (int)sub * 16 + 8 < p.d[kv]};
     // (least, -greatest) of the row; places without channels hold infinities
     uint32_t eb = kInfs;
 #pragma unroll
@@ -282,10 +289,10 @@ __global__ void __launch_bounds__(kAppendThreads) kv4_append_kernel(const __grid
         float2 f;
         if constexpr (BF16) f = __bfloat1622float2(*reinterpret_cast<const T2*>(&u[e]));
         else f = __half22float2(*reinterpret_cast<const T2*>(&u[e]));
-        const float y0 = fmaf(f.x, inv, zi), y1 = fmaf(f.y, inv, zi);
-        const float up0 = y0 + kRound, up1 = y1 + kRound;
-        far = fmaxf(far, fmaxf(fabsf(y0 - (up0 - kRound)), fabsf(y1 - (up1 - kRound))));
-        w += (__float_as_uint(up0) << (8 * e)) + (__float_as_uint(up1) << (8 * e + 4));
+        const uint64_t y = fma2(two(f.x, f.y), two(inv, inv), two(zi, zi)), up = add2(y, two(kRound, kRound));
+        const float2 off = split2(fma2(add2(up, two(-kRound, -kRound)), two(-1.f, -1.f), y)), n = split2(up);
+        far = fmaxf(far, fmaxf(fabsf(off.x), fabsf(off.y)));
+        w += (__float_as_uint(n.x) << (8 * e)) + (__float_as_uint(n.y) << (8 * e + 4));
       }
       if (far > 0.49998f) {                     // some quotient within 2e-5 of a half-way point, or an odd row
         w = 0;
@@ -301,15 +308,13 @@ __global__ void __launch_bounds__(kAppendThreads) kv4_append_kernel(const __grid
       word[j] = w;
     }
     if (stored) {
-      const int64_t page = slot >> p.page_shift;
-      const int64_t row = (((page * 2 + kv) * p.heads.d + h) << p.page_shift) + (slot & ((1 << p.page_shift) - 1));
+      const int64_t row = krow + (kv ? (int64_t)p.heads.d << p.page_shift : 0);
       *reinterpret_cast<uint2*>(p.codes + row * (DP / 8) + 2 * sub) = make_uint2(word[0], word[1]);
       if (sub == 0) {
         if (nan) sh = zh = __ushort_as_half(0x7fff);
         p.scales[row] = __halves2half2(sh, zh);
       }
-    } else if (live && slot != -1 && sub == 0 && p.status_word) {
-      atomicOr(p.status_word, UNIQL_STATUS_BAD_INDEX);
+    }
     }
   }
 }
@@ -513,15 +518,14 @@ extern "C" int uniql_kv4_append(const void* k, int64_t k_token_stride, int64_t k
   const bool bf16 = dtype == UNIQL_BF16;
   auto kernel = dp == 128 ? (bf16 ? kv4_append_kernel<128, true> : kv4_append_kernel<128, false>)
                           : (bf16 ? kv4_append_kernel<64, true> : kv4_append_kernel<64, false>);
-  // one wave: six CTAs of 40 registers a thread fit an SM
-  const int64_t per = kAppendThreads / (dp / 16), cap = 6 * (int64_t)device_info().sm_count;
-  const int64_t slab = ((int64_t)1 << 30) / (2 * kv_heads);             // tokens of a launch: rows stay below 2^31
+  const int64_t per = kAppendThreads / (dp / 16), cap = kAppendCtas * (int64_t)device_info().sm_count;
+  const int64_t slab = ((int64_t)1 << 30) / kv_heads;                   // tokens of a launch: rows stay below 2^31
   for (int64_t t0 = 0; t0 < tokens; t0 += slab) {
     const int64_t n = tokens - t0 < slab ? tokens - t0 : slab;
     p.src[0] = (const unsigned char*)k + 2 * t0 * k_token_stride;
     p.src[1] = (const unsigned char*)v + 2 * t0 * v_token_stride;
     p.slots = slots + t0;
-    p.rows = (uint32_t)(n * 2 * kv_heads);
+    p.rows = (uint32_t)(n * kv_heads);
     const int64_t ctas = ((int64_t)p.rows + per - 1) / per;
     const int err = launch_pdl(kernel, (unsigned)(ctas < cap ? ctas : cap), kAppendThreads, 0, (cudaStream_t)stream, p);
     if (err != UNIQL_OK) return err;

@@ -111,27 +111,6 @@ __device__ __forceinline__ void pa_st16(uint32_t taddr, const uint32_t* u) {
         "r"(u[9]), "r"(u[10]), "r"(u[11]), "r"(u[12]), "r"(u[13]), "r"(u[14]), "r"(u[15])
       : "memory");
 }
-// Two floats side by side: one instruction of the FMA pipe for both.
-__device__ __forceinline__ uint64_t pa_two(float a, float b) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-  return r;
-}
-__device__ __forceinline__ float2 pa_split(uint64_t v) {
-  float2 f;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(v));
-  return f;
-}
-__device__ __forceinline__ uint64_t pa_fma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
-__device__ __forceinline__ uint64_t pa_add2(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
 __device__ __forceinline__ float pa_max3(float a, float b, float c) {   // NaN if any is
   float r;
   asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
@@ -405,16 +384,16 @@ prompt_attention_kernel(const __grid_constant__ PaParams p, const __grid_constan
           }
         }
         const float base = m == -INFINITY ? 0.f : m;
-        const uint64_t ff = pa_two(f, f), nb = pa_two(-base, -base);
+        const uint64_t ff = two(f, f), nb = two(-base, -base);
         uint64_t sum[2] = {0, 0};
 #pragma unroll
         for (int q = 0; q < 4; ++q) {           // P = 2^(f S - m), 32 columns at a time
           uint32_t w[16];
 #pragma unroll
           for (int c = 0; c < 16; ++c) {
-            const float2 x = pa_split(pa_fma2(pa_two(s[32 * q + 2 * c], s[32 * q + 2 * c + 1]), ff, nb));
+            const float2 x = split2(fma2(two(s[32 * q + 2 * c], s[32 * q + 2 * c + 1]), ff, nb));
             const float2 e = make_float2(pa_exp2(x.x), pa_exp2(x.y));
-            sum[c & 1] = pa_add2(sum[c & 1], pa_two(e.x, e.y));
+            sum[c & 1] = add2(sum[c & 1], two(e.x, e.y));
             w[c] = pa_pack<BF16>(e.x, e.y);
           }
           pa_st16(ts + 16 * q, w);
@@ -425,7 +404,7 @@ prompt_attention_kernel(const __grid_constant__ PaParams p, const __grid_constan
             if (lane == 0) tc_mbar_arrive(bar_p + 16 * t + 8 * (q >> 1));
           }
         }
-        const float2 s0 = pa_split(sum[0]), s1 = pa_split(sum[1]);
+        const float2 s0 = split2(sum[0]), s1 = split2(sum[1]);
         l += (s0.x + s0.y) + (s1.x + s1.y);
       }
       // ---- O / l
