@@ -19,12 +19,16 @@
 // tokens of a lane meet pairwise: byte permutes join the same nibbles of two tokens.  So the 4-bit words go from shared memory
 // to the tensor cores in registers.
 //
-// Bound: HBM, (dk + dv) / 2 + 8 bytes per token and kv head.  Each warp keeps a ring of kStages steps of 32 tokens in flight
-// with cp.async.  Split: the 32-token steps of all requests form one list (a step: one request, one kv head), cut into equal
-// ranges, one per CTA; lengths are read on the device.  Every list
-// begins with kOpen places that stand for what a CTA pays to open it (queries, first loads, the join), so that ranges with several
-// lists hold fewer steps (64 ragged requests: 57 us without, 50 with 16).  A CTA whose range covers only a part of a request's list stores an
-// fp32 partial (sums, M), and the last CTA of that request to arrive joins the parts in order: deterministic.
+// Bound: HBM, (dk + dv) / 2 + 8 bytes per token and kv head, and close behind it the arithmetic: at 8 x 131072 tokens, 8 kv heads
+// (174 us at the measured copy rate), the loads alone take 180 us, the arithmetic alone 195 (as fp16 products), both 222.  Each
+// warp keeps a ring of kStages steps of 32 tokens in flight with cp.async.
+//
+// Split: the 32-token steps of all requests form one list (a step: one request, one kv head), cut into equal ranges, one per
+// CTA; lengths are read on the device.  Every list begins with kOpen places that stand for what a CTA pays to open it (queries,
+// first loads, the join), so that ranges with several lists hold fewer steps (64 ragged requests: 57 us without, 50 with 16).  A
+// CTA whose range covers only a part of a request's list stores an fp32 partial (sums, M), and the last CTA of that request to
+// arrive joins the parts in order: deterministic.  Short contexts are bound by that chain of dependent steps: 1000 tokens of one
+// request take 9 us in the kernel, of which the step itself is 0.8.
 #include "common.cuh"
 #include "kv_cache.cuh"
 #include "tma.cuh"
@@ -109,6 +113,76 @@ __device__ __forceinline__ float kva_rcp(float x) {
 // and 15 - c.  With it, and the 16-byte chunks of 64-byte rows swapped in pairs by bit 1 of the token, both the rows (four lanes
 // a row) and the columns (eight lanes a row, four tokens) are read from shared memory without bank conflicts.
 __device__ __forceinline__ int kva_token(int r) { return (r & 8) + ((r & 1) ? 7 - ((r & 7) >> 1) : ((r & 7) >> 1)); }
+
+template <int DP>
+struct KvaVec {                                 // a lane's channels of a part
+  using T = float4;
+};
+template <>
+struct KvaVec<64> {
+  using T = float2;
+};
+
+// The parts of a list, from CTAs c0 .. c1, into `rows` rows of the output from `row0` on.  A warp per head: lanes hold the parts' M and
+// L, 32 at a time, then every lane adds up its channels part by part; the first parts' sums are on their way meanwhile (two: with
+// eight the registers of the loop spill, 222 -> 227 us at 8 x 131072 tokens).
+template <int DP, int H>
+__device__ __forceinline__ void kva_join_parts(const KvaParams& p, int64_t row0, int rows, int c0, int c1) {
+  using namespace kva;
+  using Vec = typename KvaVec<DP>::T;
+  constexpr int PSTR = DP + 4, AHEAD = 2;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  for (int h = warp; h < rows; h += kWarps) {
+    auto part = [&](int k) { return p.part + ((size_t)(2 * k + (k == c0)) * H + h) * PSTR; };
+    auto sums = [&](int k) { return __ldcg(reinterpret_cast<const Vec*>(part(k) + lane * (DP / 32))); };
+    Vec ahead[AHEAD];
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k)
+      if (c0 + k <= c1) ahead[k] = sums(c0 + k);
+    float m = kFloor, lw = 0.f;
+    if (c0 + lane <= c1) {
+      m = __ldcg(part(c0 + lane) + DP);
+      lw = __ldcg(part(c0 + lane) + DP + 1);
+    }
+    float top = m;
+    for (int k = c0 + 32 + lane; k <= c1; k += 32) top = fmaxf(top, __ldcg(part(k) + DP));
+#pragma unroll
+    for (int s = 16; s; s >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, s));
+    float acc[DP / 32], l = 0.f;
+#pragma unroll
+    for (int e = 0; e < DP / 32; ++e) acc[e] = 0.f;
+    auto add = [&](float wk, const Vec& v) {
+      const float* x = reinterpret_cast<const float*>(&v);
+#pragma unroll
+      for (int e = 0; e < DP / 32; ++e) acc[e] = fmaf(wk, x[e], acc[e]);
+    };
+    for (int k0 = c0; k0 <= c1; k0 += 32) {
+      const int n = min(32, c1 - k0 + 1);
+      if (k0 > c0 && lane < n) {
+        m = __ldcg(part(k0 + lane) + DP);
+        lw = __ldcg(part(k0 + lane) + DP + 1);
+      }
+      const float w = lane < n ? kva_exp2(m - top) : 0.f;
+      float sum = lane < n ? w * lw : 0.f;
+#pragma unroll
+      for (int s = 16; s; s >>= 1) sum += __shfl_xor_sync(~0u, sum, s);
+      l += sum;
+      int k = 0;
+      if (k0 == c0) {
+#pragma unroll
+        for (; k < AHEAD; ++k)
+          if (k < n) add(__shfl_sync(~0u, w, k), ahead[k]);
+      }
+#pragma unroll 4
+      for (; k < n; ++k) add(__shfl_sync(~0u, w, k), sums(k0 + k));
+    }
+#pragma unroll
+    for (int e = 0; e < DP / 32; ++e) {
+      const int d = lane * (DP / 32) + e;
+      if (d < p.dv) kva_store(p.out, (row0 + h) * p.dv + d, p.bf16, l == 0.f ? 0.f : acc[e] / l);
+    }
+  }
+}
 
 template <int DP, int NT, bool PAGE16>
 __global__ void __launch_bounds__(kva::kThreads, kva::per_sm(NT)) kv4_attention_kernel(const __grid_constant__ KvaParams p) {
@@ -220,6 +294,38 @@ __global__ void __launch_bounds__(kva::kThreads, kva::per_sm(NT)) kv4_attention_
       if (PAGE16) page1 = trow[min(2 * st + 1, last_block)];
     };
     if (first < t1) look(first);
+
+    // ---- this list's queries, while the first page number is on its way
+    float v[NT][DP / 4];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int h = nt * 8 + g;
+      const int64_t base = (int64_t)b * p.q_bs + (int64_t)(head0 + h) * p.q_hs;
+#pragma unroll
+      for (int i = 0; i < DP / 4; i += 8) {
+        const int d = c * (DP / 4) + i;
+        if (h < nh && d < p.dk) {
+          if (p.q_vec) {
+            const uint4 w = *reinterpret_cast<const uint4*>(p.q + 2 * (base + d));
+            const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float2 t = p.bf16 ? __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&u[e]))
+                                      : __half22float2(*reinterpret_cast<const __half2*>(&u[e]));
+              v[nt][i + 2 * e] = t.x;
+              v[nt][i + 2 * e + 1] = t.y;
+            }
+          } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[nt][i + e] = kva_load(p.q, base + d + e, p.bf16);
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[nt][i + e] = 0.f;
+        }
+      }
+    }
+
     auto produce = [&](int st, uint32_t dst) {
       if (st < t1) {
         int pg0 = page0, pg1 = PAGE16 ? page1 : page0;
@@ -256,37 +362,11 @@ __global__ void __launch_bounds__(kva::kThreads, kva::per_sm(NT)) kv4_attention_
     int init[NT][2];                            // -8 times the digits' value, summed
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      const int h = nt * 8 + g;
-      const int64_t base = (int64_t)b * p.q_bs + (int64_t)(head0 + h) * p.q_hs;
-      float v[DP / 4];
       float top = 0.f, sum = 0.f;
 #pragma unroll
-      for (int i = 0; i < DP / 4; i += 8) {
-        const int d = c * (DP / 4) + i;
-        if (h < nh && d < p.dk) {
-          if (p.q_vec) {
-            const uint4 w = *reinterpret_cast<const uint4*>(p.q + 2 * (base + d));
-            const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float2 t = p.bf16 ? __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&u[e]))
-                                      : __half22float2(*reinterpret_cast<const __half2*>(&u[e]));
-              v[i + 2 * e] = t.x;
-              v[i + 2 * e + 1] = t.y;
-            }
-          } else {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) v[i + e] = kva_load(p.q, base + d + e, p.bf16);
-          }
-        } else {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) v[i + e] = 0.f;
-        }
-      }
-#pragma unroll
       for (int i = 0; i < DP / 4; ++i) {
-        top = fmaxf(top, fabsf(v[i]));
-        sum += v[i];
+        top = fmaxf(top, fabsf(v[nt][i]));
+        sum += v[nt][i];
       }
 #pragma unroll
       for (int o = 1; o < 4; o <<= 1) {
@@ -308,7 +388,7 @@ __global__ void __launch_bounds__(kva::kThreads, kva::per_sm(NT)) kv4_attention_
           for (int e = 0; e < 4; ++e) {
             // q down rounded to an integer in the low bits of a float, raised by 64 (1 + 128 + 128^2) to stay
             // between 0 and 2^21: base-128 digits 0 to 127
-            const uint32_t x = __float_as_uint(fmaf(v[8 * i + 2 * e + odd], down, 12582912.f + 1056832.f));
+            const uint32_t x = __float_as_uint(fmaf(v[nt][8 * i + 2 * e + odd], down, 12582912.f + 1056832.f));
 #pragma unroll
             for (int k = 0; k < 3; ++k) {
               const int right = 7 * (2 - k) - 8 * e;
@@ -333,14 +413,13 @@ __global__ void __launch_bounds__(kva::kThreads, kva::per_sm(NT)) kv4_attention_
       for (int e = 0; e < 2; ++e) init[nt][e] = -8 * __shfl_sync(~0u, value, 8 * c + 4 * e);
     }
 
-    float o[NT][MT][4], M[NT][2];
-    uint64_t L[NT], Z[NT];                      // of the two heads
+    float o[NT][MT][4];
+    uint64_t nM[NT], L[NT], Z[NT];              // -M, the sum of the weights and of their m', of the two heads
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
       for (int i = 0; i < MT; ++i) o[nt][i][0] = o[nt][i][1] = o[nt][i][2] = o[nt][i][3] = 0.f;
-#pragma unroll
-      for (int e = 0; e < 2; ++e) M[nt][e] = kFloor;
+      nM[nt] = two(-kFloor, -kFloor);
       L[nt] = Z[nt] = 0;
     }
 
@@ -422,7 +501,7 @@ __global__ void __launch_bounds__(kva::kThreads, kva::per_sm(NT)) kv4_attention_
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
             x[h][nt][r] = fma2(mul2(x[h][nt][r], s), f[nt], fma2(m, fq[nt], ls));
-            const float2 y = split2(add2(x[h][nt][r], two(-M[nt][0], -M[nt][1])));
+            const float2 y = split2(add2(x[h][nt][r], nM[nt]));
             over = fmaxf(over, fmaxf(y.x, y.y));
           }
         }
@@ -430,17 +509,19 @@ __global__ void __launch_bounds__(kva::kThreads, kva::per_sm(NT)) kv4_attention_
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
           const float2 y0 = split2(x[0][nt][0]), y1 = split2(x[0][nt][1]), y2 = split2(x[1][nt][0]), y3 = split2(x[1][nt][1]);
+          const float2 old = split2(nM[nt]);
+          const float M[2] = {-old.x, -old.y};
           float top[2] = {fmaxf(fmaxf(y0.x, y1.x), fmaxf(y2.x, y3.x)), fmaxf(fmaxf(y0.y, y1.y), fmaxf(y2.y, y3.y))}, k[2];
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
 #pragma unroll
             for (int s = 4; s < 32; s <<= 1) top[e] = fmaxf(top[e], __shfl_xor_sync(~0u, top[e], s));
-            top[e] = fmaxf(top[e], M[nt][e]);
-            k[e] = kva_exp2(M[nt][e] - top[e]);
-            M[nt][e] = top[e];
+            top[e] = fmaxf(top[e], M[e]);
+            k[e] = kva_exp2(M[e] - top[e]);
 #pragma unroll
             for (int i = 0; i < MT; ++i) { o[nt][i][e] *= k[e]; o[nt][i][2 + e] *= k[e]; }
           }
+          nM[nt] = two(-top[0], -top[1]);
           const uint64_t k2 = two(k[0], k[1]);
           L[nt] = mul2(L[nt], k2);
           Z[nt] = mul2(Z[nt], k2);
@@ -454,7 +535,7 @@ __global__ void __launch_bounds__(kva::kThreads, kva::per_sm(NT)) kv4_attention_
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
-            const float2 y = split2(add2(x[h][nt][r], two(-M[nt][0], -M[nt][1])));
+            const float2 y = split2(add2(x[h][nt][r], nM[nt]));
             const float2 w = make_float2(kva_exp2(y.x), kva_exp2(y.y));
             const uint64_t w2 = two(w.x, w.y);
             L[nt] = fma2(w2, rs[h][r], L[nt]);
@@ -505,7 +586,7 @@ __global__ void __launch_bounds__(kva::kThreads, kva::per_sm(NT)) kv4_attention_
     // ---- join the warps: sums over the lanes that share a head, then over the warps through shared memory
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      const float2 l2 = split2(L[nt]), z2 = split2(Z[nt]);
+      const float2 l2 = split2(L[nt]), z2 = split2(Z[nt]), m2 = split2(nM[nt]);
       float l[2] = {l2.x, l2.y}, z[2] = {z2.x, z2.y};
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
@@ -516,7 +597,7 @@ __global__ void __launch_bounds__(kva::kThreads, kva::per_sm(NT)) kv4_attention_
         }
         if (g == 0) {
           const int h = nt * 8 + 2 * c + e;
-          s_m[warp][h] = M[nt][e];
+          s_m[warp][h] = e ? -m2.y : -m2.x;
           s_l[warp][h] = l[e];
           s_z[warp][h] = z[e];
         }
@@ -561,55 +642,15 @@ __global__ void __launch_bounds__(kva::kThreads, kva::per_sm(NT)) kv4_attention_
     if (!whole) {
       // CTAs of this list: the ones whose ranges hold its first and its last step
       const int c0 = (int)(((list_begin + kOpen + 1) * ctas - 1) / N), c1 = (int)(((list_begin + size) * ctas - 1) / N);
-      __threadfence();
       __syncthreads();
-      if (tid == 0) s_last = atomicAdd(p.tickets + c0, 1) == c1 - c0;
+      if (tid == 0) {                           // behind the barrier its fence speaks for the whole CTA
+        __threadfence();
+        s_last = atomicAdd(p.tickets + c0, 1) == c1 - c0;
+        __threadfence();
+      }
       __syncthreads();
       if (s_last) {
-        __threadfence();
-        // a warp per head: lanes hold the parts' M and L, 32 at a time, then every lane adds up its channels part by part
-        for (int h = warp; h < nh; h += kWarps) {
-          auto part = [&](int k) { return p.part + ((size_t)(2 * k + (k == c0)) * H + h) * PSTR; };
-          float top = kFloor;
-          for (int k = c0 + lane; k <= c1; k += 32) top = fmaxf(top, __ldcg(part(k) + DP));
-#pragma unroll
-          for (int s = 16; s; s >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, s));
-          float acc[DP / 32], l = 0.f;
-#pragma unroll
-          for (int e = 0; e < DP / 32; ++e) acc[e] = 0.f;
-          for (int k0 = c0; k0 <= c1; k0 += 32) {
-            float w = 0.f, lw = 0.f;
-            if (k0 + lane <= c1) {
-              w = kva_exp2(__ldcg(part(k0 + lane) + DP) - top);
-              lw = w * __ldcg(part(k0 + lane) + DP + 1);
-            }
-#pragma unroll
-            for (int s = 16; s; s >>= 1) lw += __shfl_xor_sync(~0u, lw, s);
-            l += lw;
-            const int n = min(32, c1 - k0 + 1);
-#pragma unroll 8
-            for (int k = 0; k < n; ++k) {
-              const float wk = __shfl_sync(~0u, w, k);
-              const float* src = part(k0 + k) + lane * (DP / 32);
-              if (DP == 128) {
-                const float4 v = __ldcg(reinterpret_cast<const float4*>(src));
-                acc[0] = fmaf(wk, v.x, acc[0]);
-                acc[1] = fmaf(wk, v.y, acc[1]);
-                acc[DP / 32 - 2] = fmaf(wk, v.z, acc[DP / 32 - 2]);
-                acc[DP / 32 - 1] = fmaf(wk, v.w, acc[DP / 32 - 1]);
-              } else {
-                const float2 v = __ldcg(reinterpret_cast<const float2*>(src));
-                acc[0] = fmaf(wk, v.x, acc[0]);
-                acc[1] = fmaf(wk, v.y, acc[1]);
-              }
-            }
-          }
-#pragma unroll
-          for (int e = 0; e < DP / 32; ++e) {
-            const int d = lane * (DP / 32) + e;
-            if (d < p.dv) kva_store(p.out, ((int64_t)b * p.heads + head0 + h) * p.dv + d, p.bf16, l == 0.f ? 0.f : acc[e] / l);
-          }
-        }
+        kva_join_parts<DP, H>(p, (int64_t)b * p.heads + head0, nh, c0, c1);
         if (tid == 0) p.tickets[c0] = 0;
       }
     }
