@@ -4,9 +4,9 @@
 // softmax_scale log2(e).  q . (c - 8) is exact integer arithmetic on the tensor cores: four codes are the bytes of one AND, q is
 // rounded to 2^-19 of its largest channel or less and split into three signed base-128 digits, and mma.sync m16n8k32 (u8 x s8) sums
 // digit times code for each.  A packed word costs three instructions, all a half-rate pipe's, against five of that pipe and four of
-// the other one as two fp16 pairs: what bounds the arithmetic is that pipe (LOP3, PRMT, shifts: two cycles each).
-// (e4m3, where a code is its own subnormal number,
-// runs as conversions and fp16 products on this part.)  Scale and zero enter once per token in fp32.
+// the other one as two fp16 pairs: what bounds the arithmetic is that pipe (LOP3, PRMT, shifts: two cycles each).  (e4m3, where a
+// code is its own subnormal number, runs as conversions and fp16 products on this part.)  Scale and zero enter once per token in
+// fp32.
 // The value side folds its scale into the exponent: with y_t = x_t + log2 s'_t, M a running bound of y and w_t = 2^(y_t - M),
 //     out = (sum w_t (c'_t - 8) + sum (w_t / s'_t) m'_t) / sum (w_t / s'_t),
 // so that w is the one operand that is rounded (fp16, 2^-12 relative above 6e-5; it is at most 2^8, see below), next to exact
@@ -23,12 +23,17 @@
 // (174 us at the measured copy rate), the loads alone take 180 us, the arithmetic alone 195 (as fp16 products), both 222.  Each
 // warp keeps a ring of kStages steps of 32 tokens in flight with cp.async.
 //
-// Split: the 32-token steps of all requests form one list (a step: one request, one kv head), cut into equal ranges, one per
-// CTA; lengths are read on the device.  Every list begins with kOpen places that stand for what a CTA pays to open it (queries,
-// first loads, the join), so that ranges with several lists hold fewer steps (64 ragged requests: 57 us without, 50 with 16).  A
-// CTA whose range covers only a part of a request's list stores an fp32 partial (sums, M), and the last CTA of that request to
-// arrive joins the parts in order: deterministic.  Short contexts are bound by that chain of dependent steps: 1000 tokens of one
-// request take 9 us in the kernel, of which the step itself is 0.8.
+// Split: lengths are read on the device, and every CTA works out the same cut from them.  A step is 32 tokens of one request and kv
+// head, a list the steps of one request and head.
+//  - Little work (below kShort steps a CTA): lists are cut into equal parts of about 8 to 32 steps, one a CTA, as long as all
+//    are resident at once.  A list that is one part is finished where it is read: joining parts costs 3.5 us of dependent trips
+//    to L2, as much as 32 steps.  (us, parts / ranges of at least 4 steps: 250 tokens of 1 request 8.3 / 9.9, of 32 requests
+//    12.1 / 14.0, 4000 tokens of 1 request 13.6 / 17.5, 16000 of 1 20.0 / 27.0; 1000 of 1 11.4 / 11.2.)
+//  - More: the steps form one long list, cut into equal ranges, one per CTA.  Every list begins with kOpen places that stand for
+//    what a CTA pays to open it (queries, first loads, the join), so that ranges with several lists hold fewer steps (64 ragged
+//    requests: 57 us without, 50 with 16).
+// A CTA that has only a part of a list stores an fp32 partial (sums, M), and the last CTA of that list to arrive joins the parts
+// in order: deterministic.
 #include "common.cuh"
 #include "kv_cache.cuh"
 #include "tma.cuh"
@@ -42,7 +47,10 @@ constexpr int kWarps = 4, kThreads = kWarps * 32;
 constexpr int kStages = 3;
 constexpr int kStep = 32;                       // tokens of a step: one warp, one turn of its ring
 constexpr int kOpen = 16;                       // what opening a list costs a CTA, in steps: places of the list that hold no tokens
-constexpr int kMinSteps = kWarps;               // steps a CTA gets at least, while there are fewer than the GPU could hold
+constexpr int kShort = 24;                      // below so many steps a CTA lists are cut into whole parts
+// steps of a part, and how many parts a list may have: joining takes longer the more there are
+__host__ __device__ constexpr int part_steps(int k) { return k == 0 ? 8 : k == 1 ? 12 : k == 2 ? 24 : 32; }
+__host__ __device__ constexpr int most_parts(int k) { return k < 2 ? 12 : 24; }
 constexpr float kFloor = -1e30f;                // M before the first token
 constexpr int kMaxCtas = 2048;
 constexpr int per_sm(int nt) { return nt == 1 ? 3 : 2; }        // resident CTAs (NT 1: 237 us with 3, 245 with 2, 251 with 4 at 8 x 131072)
@@ -196,6 +204,7 @@ __global__ void __launch_bounds__(kva::kThreads, kva::per_sm(NT)) kv4_attention_
   constexpr int PSTR = DP + 4;                  // floats of one head's partial: sums, M, L
   extern __shared__ __align__(16) unsigned char smem[];
   __shared__ long long s_wide[kWarps];
+  __shared__ unsigned s_count[kWarps][6];
   __shared__ float s_m[kWarps][H], s_l[kWarps][H], s_z[kWarps][H];
   __shared__ int s_find;
   __shared__ long long s_before;
@@ -206,11 +215,55 @@ __global__ void __launch_bounds__(kva::kThreads, kva::per_sm(NT)) kv4_attention_
   const int cap = min((int64_t)p.max_blocks << p.page_shift, (int64_t)kMaxTokens);
   const int lists = p.kv_heads * p.hgroups;     // lists of a request
   auto length = [&](int b) { return min(max(p.lens[b], 0), cap); };
-  auto places = [](int len) { return len > 0 ? (len + kStep - 1) / kStep + kOpen : 0; };
 
-  // ---- this CTA's range of the list of all steps
+  // ---- how the lists are cut
   const int per = (p.batch + kThreads - 1) / kThreads;
   const int b0 = min(tid * per, p.batch), b1 = min(b0 + per, p.batch);
+  {
+    unsigned work = 0, longest = 0, parts[4] = {0, 0, 0, 0};    // what is too large for the whole cut anyway is counted short
+    for (int b = b0; b < b1; ++b) {
+      const unsigned steps = min((unsigned)(length(b) + kStep - 1) / kStep, 1u << 14);
+      work += steps;
+      longest = max(longest, steps);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) parts[k] += (steps + part_steps(k) - 1) / part_steps(k);
+    }
+    work = __reduce_add_sync(~0u, work);
+    longest = __reduce_max_sync(~0u, longest);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) parts[k] = __reduce_add_sync(~0u, parts[k]);
+    if (lane == 0) {
+      s_count[warp][0] = work;
+      s_count[warp][1] = longest;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) s_count[warp][2 + k] = parts[k];
+    }
+  }
+  __syncthreads();
+  int unit = 0;                                 // steps of a part; 0: the ranges of one long list
+  {
+    unsigned work = 0, longest = 0;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      work += s_count[w][0];
+      longest = max(longest, s_count[w][1]);
+    }
+    if ((long long)work * lists < (long long)kShort * gridDim.x)
+#pragma unroll
+      for (int k = 3; k >= 0; --k) {
+        unsigned parts = 0;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) parts += s_count[w][2 + k];
+        if ((long long)parts * lists <= gridDim.x && longest <= part_steps(k) * most_parts(k)) unit = part_steps(k);
+      }
+  }
+  // a list's places: its parts, or its steps and what stands for the opening
+  auto places = [&](int len) {
+    const int steps = (len + kStep - 1) / kStep;
+    return len <= 0 ? 0 : unit ? (steps + unit - 1) / unit : steps + kOpen;
+  };
+
+  // ---- this CTA's range of the list of all places
   long long mine = 0;
   for (int b = b0; b < b1; ++b) mine += places(length(b));
   long long incl = mine;
@@ -228,7 +281,7 @@ __global__ void __launch_bounds__(kva::kThreads, kva::per_sm(NT)) kv4_attention_
     total += s_wide[w];
   }
   const long long N = total * lists;            // below 2^48, times the CTAs below 2^59
-  const long long ctas = min((long long)gridDim.x, (N + kMinSteps - 1) / kMinSteps);
+  const long long ctas = min((long long)gridDim.x, N);          // N: one part each
   const long long begin = blockIdx.x < ctas ? N * blockIdx.x / ctas : 0;
   const long long end = blockIdx.x < ctas ? N * (blockIdx.x + 1) / ctas : 0;
   // idle rows of the batch
@@ -273,11 +326,18 @@ __global__ void __launch_bounds__(kva::kThreads, kva::per_sm(NT)) kv4_attention_
     }
     const int list = (int)((cur - req_begin) / size);
     const long long list_begin = req_begin + (long long)list * size;
-    const int steps = size - kOpen;
-    const int t0 = max((int)(cur - list_begin) - kOpen, 0);
-    const int t1 = (int)min((long long)size, end - list_begin) - kOpen;
-    cur = list_begin + min((long long)size, end - list_begin);
-    if (t1 <= t0) continue;                                     // only places that stand for the opening
+    const int at = (int)(cur - list_begin), steps = (len + kStep - 1) / kStep;
+    int t0, t1;                                                 // steps of this list
+    if (unit) {
+      t0 = steps * at / size;
+      t1 = steps * (at + 1) / size;
+      ++cur;
+    } else {
+      t0 = max(at - kOpen, 0);
+      t1 = (int)min((long long)size, end - list_begin) - kOpen;
+      cur = list_begin + min((long long)size, end - list_begin);
+      if (t1 <= t0) continue;                                   // only places that stand for the opening
+    }
     const int kvh = list / p.hgroups, hg = list - kvh * p.hgroups;
     const int head0 = kvh * p.group + hg * H;                   // first query head of this list
     const int nh = min(H, p.group - hg * H);
@@ -641,7 +701,7 @@ __global__ void __launch_bounds__(kva::kThreads, kva::per_sm(NT)) kv4_attention_
     }
     if (!whole) {
       // CTAs of this list: the ones whose ranges hold its first and its last step
-      const int c0 = (int)(((list_begin + kOpen + 1) * ctas - 1) / N), c1 = (int)(((list_begin + size) * ctas - 1) / N);
+      const int c0 = (int)(((list_begin + (unit ? 0 : kOpen) + 1) * ctas - 1) / N), c1 = (int)(((list_begin + size) * ctas - 1) / N);
       __syncthreads();
       if (tid == 0) {                           // behind the barrier its fence speaks for the whole CTA
         __threadfence();
