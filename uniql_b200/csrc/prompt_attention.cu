@@ -10,16 +10,21 @@
 //   P (16-bit, on the first 64 of S's columns) -- four softmax warps, one row a thread
 //   O (tensor memory) += P V, P read from tensor memory, V as an MN-major operand straight from its row-major tile
 // While the softmax of one unit runs the tensor cores work on the other:  warps 0-3 and 4-7 softmax of unit 0 and 1 (they also
-// rescale and store O), warp 8 issues the MMAs, warp 9 the TMA loads (no multicast).
+// rescale and store O), warp 8 issues the MMAs, warp 9 the TMA loads (no multicast), warp 10 hands out the items.
+//
+// Items.  A CTA stays on its SM and takes one pair of units after the other, by cluster launch control (the grid names every item;
+// a running CTA asks for the place of one that has not begun).  The next item's queries, keys and first scores then run under
+// the end of the one before, and the items even out over the SMs: 16 packed prompts 515 us against 562 as one CTA an item, and
+// 548 when every CTA takes every 148th (9.6 % uneven there).
 //
 // Masked places: keys behind a request's last are set to -inf in S, and the rows of V behind it in its last tile, which belong
 // to another request, are cleared in shared memory before they are multiplied by the zeros of P.
 // Bound: 128 keys of both units cost 2048 cycles of MMA, 2048 of shared memory traffic (Q and K are both read from there) and 2048
 // of exponentials (16 a clock and SM); they take 3135, the rest being the hops S -> softmax -> P -> O of a unit that the other
 // unit's work does not cover, at the 1.6 GHz that the part's power limit leaves (16384 tokens, 32 heads of 128, fp16, causal: 1.8 ms
-// in a short burst, 2.0 ms back to back = 1.1 PFLOP/s).  Tried without gain: S in two 64-key buffers a unit (Q is read twice as
+// in a short burst, 1.93 ms back to back = 1.14 PFLOP/s).  Tried without gain: S in two 64-key buffers a unit (Q is read twice as
 // often: 2.07 ms against 1.79), P handed over in quarters (1.83 to 2.0), a quarter of the exponentials as polynomials on the FMA
-// pipe (1.75 to 1.96), waits polled without a suspend time (2.00 against 2.05 back to back).
+// pipe (1.75 to 1.96), waits polled without a suspend time (2.00 against 2.05 back to back).  These were measured with one CTA an item.
 // Every wait is bounded; a wait that gives up sets UNIQL_STATUS_WAIT_TIMEOUT and the kernel drains.
 #include "common.cuh"
 #include "kv_cache.cuh"
@@ -28,8 +33,8 @@
 namespace uniql {
 
 namespace pa {
-constexpr int kMmaWarp = 8, kLoadWarp = 9;   // warps 0-7: softmax
-constexpr int kThreads = 384;                   // three warpgroups; the third has two idle warps
+constexpr int kMmaWarp = 8, kLoadWarp = 9, kPlanWarp = 10;        // warps 0-7: softmax
+constexpr int kThreads = 384;                   // three warpgroups; the third has an idle warp
 constexpr int kSoftmaxRegs = 208, kOtherRegs = 80;      // 2 * 208 + 80 <= 3 * 168, what the block is launched with
 constexpr int kRows = 128, kKeys = 128;
 constexpr int kTmemCols = 512;                  // S0, S1, O0, O1: 128 columns each
@@ -39,11 +44,41 @@ struct Cfg {
   static constexpr int kStages = 5;
   static constexpr int kOffKv = 2 * kTileBytes;
   static constexpr int kOffBar = kOffKv + kStages * kTileBytes;
-  static constexpr int kBars = 1 + 2 * kStages + 8 + 1;
+  static constexpr int kBars = 2 + 2 * kStages + 2 + 4 + 2 + 2 + 1 + 4 + 2;
   static constexpr int kSmem = kOffBar + kBars * 8 + 16 + 1024;
   static_assert(kSmem <= 227 * 1024, "shared memory");
 };
 }  // namespace pa
+
+// Cluster launch control: ask for the place of a CTA of this grid that has not begun, and read the answer (16 bytes, behind `bar`).
+__device__ __forceinline__ void pa_ask_next(uint32_t answer, uint32_t bar) {
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  tc_mbar_expect_tx(bar, 16);
+  asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(answer), "r"(bar)
+               : "memory");
+}
+__device__ __forceinline__ bool pa_next(uint32_t answer, long long& x) {
+  uint32_t ok, at = 0;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b128 h;\n\t"
+      "ld.shared.b128 h, [%2];\n\t"
+      "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, h;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t"
+      "mov.u32 %1, 0;\n\t"
+      "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, h;\n\t}"
+      : "=r"(ok), "=r"(at)
+      : "r"(answer)
+      : "memory");
+  x = at;
+  return ok != 0;
+}
+
+// What a CTA works on at a time: two units of a request and kv head.
+struct PaItem {
+  int kvh;                                      // -1: no more
+  int q0, nq, k0, nk;                           // the request's rows
+  int row[2], head[2], n[2];                    // of each unit: first query row, query head (-1: none), tiles of keys
+};
 
 struct PaParams {
   const int32_t* cu_q;
@@ -134,12 +169,13 @@ prompt_attention_kernel(const __grid_constant__ PaParams p, const __grid_constan
   using C = Cfg<DP>;
   constexpr int SUB = 128 * 128;                // bytes of a sub-tile of 128 rows x 64 channels
   extern __shared__ uint8_t smem_unaligned[];
-  __shared__ int s_work[4];                     // request, pair, valid
-  __shared__ long long s_wide[kThreads / 32];
+  __shared__ PaItem s_item[2];
+  __shared__ __align__(16) uint4 s_next[2];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_unaligned) + 1023) & ~(uintptr_t)1023);
   const uint32_t sbase = tc_smem_addr(smem);
   const uint32_t bar_q = sbase + C::kOffBar, bar_full = bar_q + 8, bar_empty = bar_full + 8 * C::kStages;
   const uint32_t bar_s = bar_empty + 8 * C::kStages, bar_p = bar_s + 16, bar_o = bar_p + 32, bar_clean = bar_o + 16;
+  const uint32_t bar_qfree = bar_clean + 8, bar_ofree = bar_qfree + 8, bar_item = bar_ofree + 16, bar_taken = bar_item + 16, bar_next = bar_taken + 16, bar_loaded = bar_next + 8;
   volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(smem + C::kOffBar + C::kBars * 8);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
@@ -165,122 +201,181 @@ prompt_attention_kernel(const __grid_constant__ PaParams p, const __grid_constan
       tc_mbar_init(bar_o + 8 * t, 1);
     }
     tc_mbar_init(bar_clean, 1);
+    tc_mbar_init(bar_qfree, 1);
+    tc_mbar_init(bar_next, 1);
+    tc_mbar_init(bar_loaded, 1);
+    for (int t = 0; t < 2; ++t) {
+      tc_mbar_init(bar_ofree + 8 * t, 4);
+      tc_mbar_init(bar_item + 8 * t, 1);
+      tc_mbar_init(bar_taken + 8 * t, 2 + kMmaWarp);           // load warp, MMA thread, softmax warps
+    }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
   pdl_wait();
   pdl_launch_dependents();
 
-  // ---- which request and which two units: pairs of units of all requests in order, kv head fastest, the last row blocks (the
-  // ones with the most keys) of a request first
-  const int pair = blockIdx.x / p.kv_heads, kvh = blockIdx.x - pair * p.kv_heads;
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
   auto begin_q = [&](int b) { return min(max(p.cu_q[b], 0), p.total_q); };
   auto begin_k = [&](int b) { return min(max(p.cu_k[b], 0), p.total_k); };
-  auto pairs_of = [&](int b) {
-    const int n = max(begin_q(b + 1) - begin_q(b), 0);
-    return (long long)(((n + kRows - 1) / kRows) * (long long)p.group + 1) / 2;
-  };
-  {
-    const int per = (p.batch + kThreads - 1) / kThreads;
-    const int b0 = min(tid * per, p.batch), b1 = min(b0 + per, p.batch);
-    long long mine = 0;
-    for (int b = b0; b < b1; ++b) mine += pairs_of(b);
-    long long incl = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const long long v = __shfl_up_sync(~0u, incl, o);
-      if (lane >= o) incl += v;
-    }
-    if (lane == 31) s_wide[warp] = incl;
-    if (tid == 0) s_work[0] = -1;
-    tc_fence_before();
-    __syncthreads();
-    tc_fence_after();
-    long long before = incl - mine;
-    for (int w = 0; w < warp; ++w) before += s_wide[w];
-    if (before <= pair && pair < before + mine) {
-      for (int b = b0; b < b1; ++b) {
-        const long long n = pairs_of(b);
-        if (pair < before + n) {
-          s_work[0] = b;
-          s_work[1] = (int)(n - 1 - (pair - before));
-          break;
-        }
-        before += n;
-      }
-    }
-    __syncthreads();
-  }
-  // rows that no request owns
-  {
-    const int lo = p.batch > 0 ? begin_q(0) : p.total_q, hi = p.batch > 0 ? begin_q(p.batch) : p.total_q;
-    const size_t rowb = (size_t)p.heads * p.dv * 2;
-    for (int r = blockIdx.x; r < lo + p.total_q - hi; r += gridDim.x) {
-      uint4* dst = reinterpret_cast<uint4*>(p.out + (size_t)(r < lo ? r : r - lo + hi) * rowb);
-      for (int i = tid; i < (int)(rowb / 16); i += kThreads) dst[i] = make_uint4(0, 0, 0, 0);
-    }
-  }
   const uint32_t tmem = *tmem_slot;
-  const int req = s_work[0];
   bool timed_out = false;
-  if (req >= 0) {
-    const int q0 = begin_q(req), nq = begin_q(req + 1) - q0;
-    const int k0 = begin_k(req), nk = max(begin_k(req + 1) - k0, 0);
-    const int units = ((nq + kRows - 1) / kRows) * p.group, u0 = 2 * s_work[1];
-    const int shift = p.causal ? nk - nq : 0;   // query i sees the keys below i + 1 + shift
-    int row[2], head[2], n[2];
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      const int u = u0 + t;
-      row[t] = u / p.group * kRows;
-      head[t] = kvh * p.group + u % p.group;
-      int seen = nk;
-      if (p.causal) seen = min(nk, max(min(row[t] + kRows, nq) + shift, 0));
-      n[t] = u < units ? (seen + kKeys - 1) / kKeys : 0;
-    }
-    const int nmax = max(n[0], n[1]);
-    const bool dirty = nmax * kKeys > nk;       // the last tile of V reaches behind the request
+  // The items of a CTA, one behind the other: every role walks them by itself.  item(k): the k-th one, false behind the last or when a
+  // wait of the role has given up; a warp decides that together.
+  auto item = [&](int k, PaItem& w, bool whole_warp) {
+    if (!timed_out && !tc_mbar_wait(bar_item + 8 * (k & 1), (k >> 1) & 1)) timed_out = true;
+    if (whole_warp) timed_out = __any_sync(~0u, timed_out);
+    if (timed_out) return false;
+    w = s_item[k & 1];
+    return w.kvh >= 0;
+  };
 
-    if (warp >= kMmaWarp) {
-      asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
-    if (warp == kLoadWarp) {
-      // ------------------------------------------------------------------ loads: Q, then K 0, V 0, K 1, V 1, ...
-      if (tc_elect() && nmax > 0) {
-        tc_mbar_expect_tx(bar_q, ((n[0] > 0) + (n[1] > 0)) * C::kTileBytes);
+  if (warp >= kMmaWarp) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
+    if (warp == kPlanWarp) {
+      // ------------------------------------------------------------------ items: pairs of units of all requests in order, kv head
+      // fastest, the last row blocks (the ones with the most keys) of a request first.  The grid has a CTA for every item; one
+      // that runs takes the places of others that have not begun (cluster launch control), so that the next item's loads and
+      // products start while the last one's results are written, and whoever is free first takes the next item.
+      auto pairs_of = [&](int b) {
+        const int n = max(begin_q(b + 1) - begin_q(b), 0);
+        return (long long)(((n + kRows - 1) / kRows) * (long long)p.group + 1) / 2;
+      };
+      const int per = (p.batch + 31) / 32;
+      const int b0 = min(lane * per, p.batch), b1 = min(b0 + per, p.batch);
+      long long mine = 0;
+      for (int b = b0; b < b1; ++b) mine += pairs_of(b);
+      long long incl = mine;
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
-          if (n[t] > 0)
-            for (int i = 0; i < DP / 64; ++i)
-              pa_tma_3d(sbase + t * C::kTileBytes + i * SUB, &qmap, 64 * i, head[t], q0 + row[t], bar_q);
-        for (int it = 0; it < 2 * nmax; ++it) {
-          const int s = it % C::kStages;
-          if (!timed_out && !tc_mbar_wait(bar_empty + 8 * s, ((it / C::kStages) & 1) ^ 1)) timed_out = true;
-          if (timed_out) break;
-          tc_mbar_expect_tx(bar_full + 8 * s, C::kTileBytes);
-          for (int i = 0; i < DP / 64; ++i)
-            pa_tma_3d(sbase + C::kOffKv + s * C::kTileBytes + i * SUB, (it & 1) ? &vmap : &kmap, 64 * i, kvh,
-                      k0 + (it >> 1) * kKeys, bar_full + 8 * s);
-        }
+      for (int o = 1; o < 32; o <<= 1) {
+        const long long v = __shfl_up_sync(~0u, incl, o);
+        if (lane >= o) incl += v;
       }
-      timed_out = __shfl_sync(~0u, (int)(__any_sync(~0u, timed_out)), 0);
-      if (dirty && nmax > 0 && !timed_out) {
-        const int it = 2 * nmax - 1, s = it % C::kStages;
-        if (!tc_mbar_wait(bar_full + 8 * s, (it / C::kStages) & 1)) timed_out = true;
-        if (!timed_out) {
-          const int r0 = nk - (nmax - 1) * kKeys;               // first row of another request
-          const uint32_t tile = sbase + C::kOffKv + s * C::kTileBytes;
-          for (int i = lane; i < (kKeys - r0) * 8 * (DP / 64); i += 32) {
-            const int sub = i / ((kKeys - r0) * 8), x = i - sub * ((kKeys - r0) * 8);
-            asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(tile + sub * SUB + r0 * 128 + x * 16), "r"(0) : "memory");
+      const long long before = incl - mine, total = __shfl_sync(~0u, incl, 31) * p.kv_heads;
+      const int low = p.batch > 0 ? begin_q(0) : p.total_q, high = p.batch > 0 ? begin_q(p.batch) : p.total_q;
+      long long x = blockIdx.x;
+      bool more = true;
+      for (int k = 0;; ++k) {
+        if (more)                               // rows that no request owns: cleared by the way
+          for (long long r = x; r < low + p.total_q - high; r += gridDim.x) {
+            uint4* dst = reinterpret_cast<uint4*>(p.out + (size_t)(r < low ? r : r - low + high) * p.heads * p.dv * 2);
+            for (int i = lane; i < p.heads * p.dv / 8; i += 32) dst[i] = make_uint4(0, 0, 0, 0);
           }
-          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        if (k >= 2 && !timed_out && !tc_mbar_wait(bar_taken + 8 * (k & 1), ((k >> 1) & 1) ^ 1)) timed_out = true;
+        timed_out = __any_sync(~0u, timed_out);
+        if (timed_out) break;                   // the others give up by themselves
+        const long long pair = x / p.kv_heads;
+        PaItem w;
+        if (more && x < total) {
+          // the lane whose requests hold the pair works the item out
+          const bool hit = before <= pair && pair < before + mine;
+          if (hit) {
+            long long at = before, n = 0;
+            int b = b0;
+            for (; b < b1; ++b) {
+              n = pairs_of(b);
+              if (pair < at + n) break;
+              at += n;
+            }
+            w.kvh = (int)(x - pair * p.kv_heads);
+            w.q0 = begin_q(b);
+            w.nq = begin_q(b + 1) - w.q0;
+            w.k0 = begin_k(b);
+            w.nk = max(begin_k(b + 1) - w.k0, 0);
+            const int units = ((w.nq + kRows - 1) / kRows) * p.group, u0 = 2 * (int)(n - 1 - (pair - at));
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+              const int u = u0 + t;
+              const int row = u / p.group * kRows;
+              int seen = w.nk;                  // query i sees the keys below i + 1 + nk - nq
+              if (p.causal) seen = min(w.nk, max(min(row + kRows, w.nq) + w.nk - w.nq, 0));
+              w.row[t] = row;
+              w.head[t] = u < units ? w.kvh * p.group + u % p.group : -1;
+              w.n[t] = u < units ? (seen + kKeys - 1) / kKeys : 0;
+            }
+            s_item[k & 1] = w;
+          }
+        } else if (lane == 0) {                 // none behind this one, or a place of the grid that is no item
+          s_item[k & 1].kvh = more ? 0 : -1;
+          s_item[k & 1].n[0] = s_item[k & 1].n[1] = 0;
+          s_item[k & 1].head[0] = s_item[k & 1].head[1] = -1;
         }
         __syncwarp();
-        if (lane == 0) tc_mbar_arrive(bar_clean);
+        if (lane == 0) tc_mbar_arrive(bar_item + 8 * (k & 1));
+        if (!more) break;
+        // the next one is asked for when this one's loads have all been issued: earlier, it could be another CTA's sooner
+        if (!tc_mbar_wait(bar_loaded, k & 1)) timed_out = true;
+        timed_out = __any_sync(~0u, timed_out);
+        if (timed_out) break;
+        if (lane == 0) pa_ask_next(tc_smem_addr(&s_next[k & 1]), bar_next);
+        if (!tc_mbar_wait(bar_next, k & 1)) timed_out = true;
+        timed_out = __any_sync(~0u, timed_out);
+        if (timed_out) break;
+        more = pa_next(tc_smem_addr(&s_next[k & 1]), x);
       }
+    }
+    if (warp == kLoadWarp) {
+      // ------------------------------------------------------------------ loads: Q, then K 0, V 0, K 1, V 1, ... of every item
+      PaItem w;
+      int it0 = 0, qs = 0;                      // tiles and items loaded so far
+      for (int k = 0; item(k, w, true); ++k) {
+        __syncwarp();
+        if (lane == 0) tc_mbar_arrive(bar_taken + 8 * (k & 1));
+        const int nmax = max(w.n[0], w.n[1]);
+        if (nmax == 0) {
+          if (lane == 0) tc_mbar_arrive(bar_loaded);
+          continue;
+        }
+        if (tc_elect()) {
+          if (qs > 0 && !tc_mbar_wait(bar_qfree, (qs - 1) & 1)) timed_out = true;
+          if (!timed_out) {
+            tc_mbar_expect_tx(bar_q, ((w.n[0] > 0) + (w.n[1] > 0)) * C::kTileBytes);
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+              if (w.n[t] > 0)
+                for (int i = 0; i < DP / 64; ++i)
+                  pa_tma_3d(sbase + t * C::kTileBytes + i * SUB, &qmap, 64 * i, w.head[t], w.q0 + w.row[t], bar_q);
+          }
+          for (int i2 = 0; i2 < 2 * nmax && !timed_out; ++i2) {
+            const int it = it0 + i2, s = it % C::kStages;
+            if (!tc_mbar_wait(bar_empty + 8 * s, ((it / C::kStages) & 1) ^ 1)) {
+              timed_out = true;
+              break;
+            }
+            tc_mbar_expect_tx(bar_full + 8 * s, C::kTileBytes);
+            for (int i = 0; i < DP / 64; ++i)
+              pa_tma_3d(sbase + C::kOffKv + s * C::kTileBytes + i * SUB, (i2 & 1) ? &vmap : &kmap, 64 * i, w.kvh,
+                        w.k0 + (i2 >> 1) * kKeys, bar_full + 8 * s);
+          }
+        }
+        timed_out = __any_sync(~0u, timed_out);
+        if (lane == 0) tc_mbar_arrive(bar_loaded);
+        it0 += 2 * nmax;
+        ++qs;
+        if (nmax * kKeys > w.nk) {              // the last tile of V reaches behind the request: clear those rows
+          const int it = it0 - 1, s = it % C::kStages;
+          if (!timed_out && !tc_mbar_wait(bar_full + 8 * s, (it / C::kStages) & 1)) timed_out = true;
+          if (!timed_out) {
+            const int r0 = w.nk - (nmax - 1) * kKeys;           // first row of another request
+            const uint32_t tile = sbase + C::kOffKv + s * C::kTileBytes;
+            for (int i = lane; i < (kKeys - r0) * 8 * (DP / 64); i += 32) {
+              const int sub = i / ((kKeys - r0) * 8), x = i - sub * ((kKeys - r0) * 8);
+              asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(tile + sub * SUB + r0 * 128 + x * 16), "r"(0) : "memory");
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          }
+          timed_out = __any_sync(~0u, timed_out);
+          if (lane == 0) tc_mbar_arrive(bar_clean);
+        }
+      }
+      // given up: what has been asked for arrives before the CTA leaves (each tile's wait is bounded, too)
+      if (timed_out && lane == 0)
+        for (int it = max(it0 - C::kStages, 0); it < it0; ++it) tc_mbar_wait(bar_full + 8 * (it % C::kStages), (it / C::kStages) & 1);
     } else if (warp == kMmaWarp) {
       // ------------------------------------------------------------------ MMAs
-      if (tc_elect() && nmax > 0) {
+      if (tc_elect()) {
         constexpr uint32_t kType = BF16 ? (1u << 7) | (1u << 10) : 0u;
         const uint32_t idesc_s = (1u << 4) | kType | ((uint32_t)(kKeys >> 3) << 17) | (8u << 24);
         const int nv = (p.dv + 15) / 16 * 16, ks = (p.dk + 15) / 16;
@@ -311,24 +406,46 @@ prompt_attention_kernel(const __grid_constant__ PaParams p, const __grid_constan
           }
           tc_commit(bar_o + 8 * t);
         };
-        wait(bar_q, 0);
-        wait(bar_full, 0);
+        PaItem w;
+        int it0 = 0, qs = 0, cleans = 0, steps[2] = {0, 0}, outs[2] = {0, 0};     // tiles, items, .. so far; steps and results of a unit
+        for (int k = 0; item(k, w, false); ++k) {
+          tc_mbar_arrive(bar_taken + 8 * (k & 1));
+          const int nmax = max(w.n[0], w.n[1]);
+          if (nmax == 0) continue;
+          const bool dirty = nmax * kKeys > w.nk;
+          wait(bar_q, qs & 1);
+          wait(bar_full + 8 * (it0 % C::kStages), (it0 / C::kStages) & 1);
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
-          if (n[t] > 0) scores(t, 0);
-        tc_commit(bar_empty);
-        for (int j = 0; j < nmax; ++j) {
-          const int iv = 2 * j + 1, ik = 2 * j + 2, sv = iv % C::kStages, sk = ik % C::kStages;
-          wait(bar_full + 8 * sv, (iv / C::kStages) & 1);
-          if (j + 1 < nmax) wait(bar_full + 8 * sk, (ik / C::kStages) & 1);
-          else if (dirty) wait(bar_clean, 0);
+          for (int t = 0; t < 2; ++t)
+            if (w.n[t] > 0) scores(t, it0);
+          tc_commit(bar_empty + 8 * (it0 % C::kStages));
+          if (nmax == 1) tc_commit(bar_qfree);
+          for (int j = 0; j < nmax; ++j) {
+            const int iv = it0 + 2 * j + 1, ik = iv + 1, sv = iv % C::kStages, sk = ik % C::kStages;
+            wait(bar_full + 8 * sv, (iv / C::kStages) & 1);
+            if (j + 1 < nmax) wait(bar_full + 8 * sk, (ik / C::kStages) & 1);
+            else if (dirty) wait(bar_clean, cleans & 1);
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+              if (j < w.n[t]) {
+                // the first values of an item overwrite the unit's result before it: that has to have been read
+                if (j == 0 && outs[t] > 0) wait(bar_ofree + 8 * t, (outs[t] - 1) & 1);
+                values(t, iv, j > 0, (steps[t] + j) & 1);
+              }
+              if (t == 1) tc_commit(bar_empty + 8 * sv);
+              if (j + 1 < w.n[t]) scores(t, ik);
+            }
+            if (j + 1 < nmax) tc_commit(bar_empty + 8 * sk);
+            if (j + 2 == nmax) tc_commit(bar_qfree);            // the item's last Q K^T
+          }
+          it0 += 2 * nmax;
+          ++qs;
+          cleans += dirty;
 #pragma unroll
           for (int t = 0; t < 2; ++t) {
-            if (j < n[t]) values(t, iv, j > 0, j & 1);
-            if (t == 1) tc_commit(bar_empty + 8 * sv);
-            if (j + 1 < n[t]) scores(t, ik);
+            steps[t] += w.n[t];
+            outs[t] += w.n[t] > 0;
           }
-          if (j + 1 < nmax) tc_commit(bar_empty + 8 * sk);
         }
       }
     }
@@ -336,15 +453,21 @@ prompt_attention_kernel(const __grid_constant__ PaParams p, const __grid_constan
       // ------------------------------------------------------------------ softmax, one query row a thread
       asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
       const int t = warp >> 2;
-      const int nt = t ? n[1] : n[0], row0 = t ? row[1] : row[0], i = row0 + (warp & 3) * 32 + lane;
-      const int limit = p.causal ? min(nk, max(i + 1 + shift, 0)) : nk;
-      const int full = p.causal ? min(nk, max(row0 + 1 + shift, 0)) : nk;       // keys that every row of the unit sees
       const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
       const uint32_t ts = tmem + t * 128 + lanes, to = tmem + 256 + t * 128 + lanes;
       const float f = p.scale_log2;
+      PaItem w;
+      int steps = 0;                            // of this unit in the items before
+      for (int k = 0; item(k, w, true); ++k) {
+      __syncwarp();
+      if (lane == 0) tc_mbar_arrive(bar_taken + 8 * (k & 1));
+      const int nt = t ? w.n[1] : w.n[0], row0 = t ? w.row[1] : w.row[0], head = t ? w.head[1] : w.head[0];
+      const int nq = w.nq, nk = w.nk, shift = nk - nq, i = row0 + (warp & 3) * 32 + lane;
+      const int limit = p.causal ? min(nk, max(i + 1 + shift, 0)) : nk;
+      const int full = p.causal ? min(nk, max(row0 + 1 + shift, 0)) : nk;       // keys that every row of the unit sees
       float m = -INFINITY, l = 0.f;
       for (int j = 0; j < nt; ++j) {
-        if (!timed_out && !tc_mbar_wait(bar_s + 8 * t, j & 1)) timed_out = true;
+        if (!timed_out && !tc_mbar_wait(bar_s + 8 * t, (steps + j) & 1)) timed_out = true;
         tc_fence_after();
         float s[128];
 #pragma unroll
@@ -366,11 +489,11 @@ prompt_attention_kernel(const __grid_constant__ PaParams p, const __grid_constan
         if (top != top) m = top;                // a NaN among the scores: all of the row is
         if (__any_sync(~0u, top > m + 8.f)) {
           const float mn = fmaxf(m, top);
-          const float k = m == m ? (mn == -INFINITY ? 1.f : pa_exp2(m - mn)) : m;
+          const float down = m == m ? (mn == -INFINITY ? 1.f : pa_exp2(m - mn)) : m;
           m = m == m ? mn : m;
-          l *= k;
+          l *= down;
           if (j > 0) {
-            if (!timed_out && !tc_mbar_wait(bar_o + 8 * t, (j - 1) & 1)) timed_out = true;
+            if (!timed_out && !tc_mbar_wait(bar_o + 8 * t, (steps + j - 1) & 1)) timed_out = true;
             tc_fence_after();
 #pragma unroll 1
             for (int c = 0; c < DP; c += 32) {
@@ -378,7 +501,7 @@ prompt_attention_kernel(const __grid_constant__ PaParams p, const __grid_constan
               pa_ld32(to + c, o);
               pa_wait_ld();
 #pragma unroll
-              for (int e = 0; e < 32; ++e) o[e] *= k;
+              for (int e = 0; e < 32; ++e) o[e] *= down;
               pa_st32(to + c, reinterpret_cast<const uint32_t*>(o));
             }
           }
@@ -388,15 +511,15 @@ prompt_attention_kernel(const __grid_constant__ PaParams p, const __grid_constan
         uint64_t sum[2] = {0, 0};
 #pragma unroll
         for (int q = 0; q < 4; ++q) {           // P = 2^(f S - m), 32 columns at a time
-          uint32_t w[16];
+          uint32_t y[16];
 #pragma unroll
           for (int c = 0; c < 16; ++c) {
             const float2 x = split2(fma2(two(s[32 * q + 2 * c], s[32 * q + 2 * c + 1]), ff, nb));
             const float2 e = make_float2(pa_exp2(x.x), pa_exp2(x.y));
             sum[c & 1] = add2(sum[c & 1], two(e.x, e.y));
-            w[c] = pa_pack<BF16>(e.x, e.y);
+            y[c] = pa_pack<BF16>(e.x, e.y);
           }
-          pa_st16(ts + 16 * q, w);
+          pa_st16(ts + 16 * q, y);
           if (q & 1) {
             pa_wait_st();
             tc_fence_before();
@@ -408,39 +531,45 @@ prompt_attention_kernel(const __grid_constant__ PaParams p, const __grid_constan
         l += (s0.x + s0.y) + (s1.x + s1.y);
       }
       // ---- O / l
-      if (u0 + t < units) {
+      if (head >= 0) {
         if (nt > 0) {
-          if (!timed_out && !tc_mbar_wait(bar_o + 8 * t, (nt - 1) & 1)) timed_out = true;
+          if (!timed_out && !tc_mbar_wait(bar_o + 8 * t, (steps + nt - 1) & 1)) timed_out = true;
           tc_fence_after();
         }
         const float inv = l == 0.f ? 0.f : 1.f / l;
-        unsigned char* dst = p.out + ((size_t)(q0 + i) * p.heads + (t ? head[1] : head[0])) * p.dv * 2;
+        unsigned char* dst = p.out + ((size_t)(w.q0 + i) * p.heads + head) * p.dv * 2;
 #pragma unroll 1
         for (int c = 0; c < DP; c += 32) {
           float o[32];
           if (nt > 0) {
             pa_ld32(to + c, o);
             pa_wait_ld();
+            if (c + 32 == DP) {                 // O may be overwritten
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) tc_mbar_arrive(bar_ofree + 8 * t);
+            }
           } else {
 #pragma unroll
             for (int e = 0; e < 32; ++e) o[e] = 0.f;
           }
-          if (i < nq) {
+          if (i < nq && !timed_out) {
 #pragma unroll
             for (int v = 0; v < 4; ++v)
               if (c + 8 * v < p.dv) {
-                uint32_t w[4];
+                uint32_t x[4];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                   const float a = l == 0.f ? 0.f : o[8 * v + 2 * e] * inv, b = l == 0.f ? 0.f : o[8 * v + 2 * e + 1] * inv;
-                  w[e] = pa_pack<BF16>(a, b);
+                  x[e] = pa_pack<BF16>(a, b);
                 }
-                *reinterpret_cast<uint4*>(dst + (c + 8 * v) * 2) = make_uint4(w[0], w[1], w[2], w[3]);
+                *reinterpret_cast<uint4*>(dst + (c + 8 * v) * 2) = make_uint4(x[0], x[1], x[2], x[3]);
               }
           }
         }
       }
-    }
+      steps += nt;
+      }
   }
   if (timed_out && p.status_word) atomicOr(p.status_word, UNIQL_STATUS_WAIT_TIMEOUT);
   tc_fence_before();
@@ -524,7 +653,9 @@ extern "C" int uniql_prompt_attention(const void* q, int64_t q_token_stride, int
   // at most this many pairs of units: every request rounds its row blocks and its pairs up
   const int64_t blocks = total_q / pa::kRows + (batch < total_q ? batch : total_q);
   const int64_t pairs = (blocks * p.group + 1) / 2 + batch;
-  const int64_t ctas = pairs > 0 ? pairs * kv_heads : 1;     // at least one: rows that nobody owns are cleared
+  const int64_t sms = device_info().sm_count;
+  int64_t ctas = pairs * kv_heads;
+  if (ctas < sms) ctas = total_q < sms ? (ctas > total_q ? ctas : total_q) : sms;       // rows that nobody owns are cleared by all
   if (ctas > ((int64_t)1 << 31) - 1) return UNIQL_ESHAPE;
   cudaStream_t s = (cudaStream_t)stream;
   if (dk > 64 || dv > 64)
