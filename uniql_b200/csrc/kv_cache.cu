@@ -154,7 +154,7 @@ __global__ void __launch_bounds__(kPlanThreads) kv_page_plan_kernel(const __grid
 // reads, 4 bytes a channel against 0.5 written, if the instructions are few: the packed minimum carries NaN along, the codes
 // are rounded by adding 1.5 * 2^23 and joined as the low bits of those sums, and sixteen channels a lane share what a row costs
 // (eight: 50 us for 14760 tokens of 8 heads, 60 MB read; sixteen: 34; with K's and V's rows in one turn and packed
-// arithmetic: 30).  (hi - lo) / 15 is the quotient by the reciprocal and one
+// arithmetic: 27).  (hi - lo) / 15 is the quotient by the reciprocal and one
 // residual step (Markstein), equal to the division for every mantissa.
 //
 // Codes are taken from a quotient in fp32.  Where that leaves the side of a half-way point open, the two sides are compared
@@ -181,7 +181,7 @@ struct AppendParams {
   int d[2], page_shift;
 };
 
-constexpr int kAppendThreads = 256, kAppendCtas = 6;      // CTAs an SM holds: one wave
+constexpr int kAppendThreads = 256, kAppendCtas = 6;      // CTAs an SM holds
 
 template <bool BF16>
 struct Pair16 {
@@ -518,7 +518,7 @@ extern "C" int uniql_kv4_append(const void* k, int64_t k_token_stride, int64_t k
   const bool bf16 = dtype == UNIQL_BF16;
   auto kernel = dp == 128 ? (bf16 ? kv4_append_kernel<128, true> : kv4_append_kernel<128, false>)
                           : (bf16 ? kv4_append_kernel<64, true> : kv4_append_kernel<64, false>);
-  const int64_t per = kAppendThreads / (dp / 16), cap = kAppendCtas * (int64_t)device_info().sm_count;
+  const int64_t per = kAppendThreads / (dp / 16), cap = 4 * kAppendCtas * (int64_t)device_info().sm_count;     // four waves even out: 26.7 us against 30.2 of one
   const int64_t slab = ((int64_t)1 << 30) / kv_heads;                   // tokens of a launch: rows stay below 2^31
   for (int64_t t0 = 0; t0 < tokens; t0 += slab) {
     const int64_t n = tokens - t0 < slab ? tokens - t0 : slab;
