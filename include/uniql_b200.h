@@ -370,8 +370,9 @@ int uniql_w4a16_swap_plan_check(void);
  *
  * uniql_kv4_attention: one query token per request over its first lens[i] cached tokens (grouped heads: query head h reads kv head
  *   h / (heads / kv_heads)): out[i, h] = softmax(softmax_scale * q k^T) v in fp32, rounded once.  A V scale of 0 (a row that was
- *   never written) and a page outside the cache are absent tokens; without any token the result is zeros.  The tokens are split evenly over the GPU whatever the lengths are, and the parts of a request are
- *   joined in a fixed order.
+ *   never written) and a page outside the cache are absent tokens; without any token the result is zeros.  The work is split
+ *   over the GPU whatever the lengths are, and the parts of a request are joined in a fixed order: the same call gives the
+ *   same bits.
  *   scratch  uniql_kv4_attention_scratch_bytes(...) bytes, rules as for uniql_w4a16_linear
  *
  * uniql_prompt_attention: packed prompts.  Request i owns rows cu_q[i] .. cu_q[i + 1] - 1 of q [total_q, heads, dk] and out
@@ -379,7 +380,8 @@ int uniql_w4a16_swap_plan_check(void);
  *   queries), so that the last query sees them all; a query that sees none gives zeros, and so do rows of `out` that no
  *   request owns.  k and v of tokens that other requests own never reach a request, whatever they hold; within a request a
  *   non-finite v may reach queries in front of it that share its 128-row tile.
- *   Rows must be 16-byte aligned (strides multiples of 8).  P is rounded to the input type in front of the second product.
+ *   Rows must be 16-byte aligned (strides multiples of 8).  P is rounded to the input type in front of the second product.  At
+ *   most 2^26 keys.
  */
 #define UNIQL_KV_MAX_BATCH 16384
 int uniql_kv_page_plan(const int32_t* lens, const int32_t* new_lens, int64_t batch, int32_t* block_table, int64_t ld_table,

@@ -68,7 +68,7 @@ EINVAL, ESHAPE, ESCRATCH, EDTYPE = -1, -3, -4, -6
     (_decode, dict(codes=None), EINVAL), (_decode, dict(batch=16385), ESHAPE), (_decode, dict(batch=0), 0),
     (_prompt, dict(total_q=-1), EINVAL), (_prompt, dict(heads=7), ESHAPE), (_prompt, dict(dk=136), ESHAPE), (_prompt, dict(dv=12), ESHAPE), (_prompt, dict(dtype=2), EDTYPE),
     (_prompt, dict(scale=-1.0), EINVAL), (_prompt, dict(qt=1023), EINVAL), (_prompt, dict(kh=-128), EINVAL), (_prompt, dict(q=P + 2), EINVAL),
-    (_prompt, dict(k=None), EINVAL), (_prompt, dict(cu_k=None), EINVAL), (_prompt, dict(out=None), EINVAL), (_prompt, dict(batch=16385), ESHAPE),
+    (_prompt, dict(k=None), EINVAL), (_prompt, dict(cu_k=None), EINVAL), (_prompt, dict(out=None), EINVAL), (_prompt, dict(batch=16385), ESHAPE), (_prompt, dict(total_k=(1 << 26) + 1), ESHAPE),
     (_prompt, dict(total_q=0), 0)])
 def test_refusals(built_lib, call, kw, code):
     assert call(**kw) == code

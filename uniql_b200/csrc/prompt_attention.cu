@@ -629,7 +629,8 @@ extern "C" int uniql_prompt_attention(const void* q, int64_t q_token_stride, int
   if (batch < 0 || total_q < 0 || total_k < 0 || heads <= 0 || kv_heads <= 0 || dk <= 0 || dv <= 0) return UNIQL_EINVAL;
   if (dtype != UNIQL_F16 && dtype != UNIQL_BF16) return UNIQL_EDTYPE;
   if (dk % 8 || dv % 8 || dk > 128 || dv > 128 || heads % kv_heads || heads > 16384 || kv_heads > 1024) return UNIQL_ESHAPE;
-  if (batch > UNIQL_KV_MAX_BATCH || total_q > kMaxTokens || total_k > kMaxTokens) return UNIQL_ESHAPE;
+  // 2^26 keys are 2^19 tiles, 0.8 s of one item: well inside the bound of every wait
+  if (batch > UNIQL_KV_MAX_BATCH || total_q > kMaxTokens || total_k > (int64_t)1 << 26) return UNIQL_ESHAPE;
   if (!(softmax_scale > 0.f) || softmax_scale > 1e30f) return UNIQL_EINVAL;
   if ((q_token_stride | q_head_stride | k_token_stride | k_head_stride | v_token_stride | v_head_stride) & 7) return UNIQL_EINVAL;
   if (q_token_stride < 0 || q_head_stride < 0 || k_token_stride < 0 || k_head_stride < 0 || v_token_stride < 0 || v_head_stride < 0)
