@@ -326,6 +326,21 @@ def test_decode_is_deterministic_and_independent_of_the_batch():
         assert (alone - first[i]).abs().max() < 2 * (2 ** -11 + 2 ** -11 * 4)
 
 
+@pytest.mark.parametrize("lens,kv", [
+    ([128] * 32, 1), ([129] * 33, 1), ([0] * 31 + [257], 2), ([0] * 32 + [257], 2), ([256, 255, 1, 0, 1536, 1537], 1), ([1535] * 9, 6),
+    ([384 * 12 + 1], 8), ([768 * 24], 4), ([768 * 24 + 1, 5], 4), ([32 * 4 * 12 + 1, 256], 3), ([1] * 131, 4), ([2000, 0, 33] * 43, 1)])
+def test_decode_cuts(lens, kv):
+    """Where the way that lists are cut changes: parts of every size, the longest lists that get them, batches of 32 and 33."""
+    from uniql_b200 import ops
+    g = _gen(len(lens) * 7 + kv)
+    codes, scales, table = _filled(g, lens, 64, kv, 64, 64)
+    q = _rows(g, len(lens), 2 * kv, 64, F16)
+    args = q.cuda(), codes.cuda(), scales.cuda(), table.cuda(), torch.tensor(lens, dtype=torch.int32).cuda()
+    got = ops.kv4_attention(*args)
+    _decode_check(got.cpu(), q, codes, scales, table, lens, 64, 64, 1 / 8)
+    assert torch.equal(got, ops.kv4_attention(*args))
+
+
 def test_decode_bad_pages_and_lengths(route):
     """Pages outside the cache are absent tokens; lengths beyond the table and below zero are cut."""
     from uniql_b200 import ops

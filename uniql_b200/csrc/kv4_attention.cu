@@ -27,8 +27,8 @@
 // head, a list the steps of one request and head.
 //  - Little work (below kShort steps a CTA): lists are cut into equal parts of about 8 to 32 steps, one a CTA, as long as all
 //    are resident at once.  A list that is one part is finished where it is read: joining parts costs 3.5 us of dependent trips
-//    to L2, as much as 32 steps.  (us, parts / ranges of at least 4 steps: 250 tokens of 1 request 8.3 / 9.9, of 32 requests
-//    12.1 / 14.0, 4000 tokens of 1 request 13.6 / 17.5, 16000 of 1 20.0 / 27.0; 1000 of 1 11.4 / 11.2.)
+//    to L2, as much as 32 steps.  (us, parts / ranges: 250 tokens of 1 request 8.4 / 10.1, of 32 requests 11.8 / 13.9, 4000
+//    tokens of 1 request 13.0 / 18.2, 16000 of 1 20.3 / 27.0; 1000 of 1 11.1 / 11.3.)
 //  - More: the steps form one long list, cut into equal ranges, one per CTA.  Every list begins with kOpen places that stand for
 //    what a CTA pays to open it (queries, first loads, the join), so that ranges with several lists hold fewer steps (64 ragged
 //    requests: 57 us without, 50 with 16).
@@ -217,12 +217,55 @@ __global__ void __launch_bounds__(kva::kThreads, kva::per_sm(NT)) kv4_attention_
   auto length = [&](int b) { return min(max(p.lens[b], 0), cap); };
 
   // ---- how the lists are cut
-  const int per = (p.batch + kThreads - 1) / kThreads;
-  const int b0 = min(tid * per, p.batch), b1 = min(b0 + per, p.batch);
-  {
+  int unit = 0;                                 // steps of a part; 0: the ranges of one long list
+  auto cut = [&](unsigned work, unsigned longest, const unsigned (&parts)[4]) {
+    if ((long long)work * lists >= (long long)kShort * gridDim.x) return;
+#pragma unroll
+    for (int k = 3; k >= 0; --k)
+      if ((long long)parts[k] * lists <= gridDim.x && longest <= part_steps(k) * most_parts(k)) unit = part_steps(k);
+    // lists that are joined anyway: a step a warp
+    if (unit == part_steps(0) && longest > part_steps(0) && longest <= kWarps * most_parts(0) && 2ll * parts[0] * lists <= gridDim.x) unit = kWarps;
+  };
+  // a list's places: its parts, or its steps and what stands for the opening
+  auto places = [&](int len) {
+    const int steps = (len + kStep - 1) / kStep;
+    return len <= 0 ? 0 : unit ? (steps + unit - 1) / unit : steps + kOpen;
+  };
+  long long begin = 0, end = 0, N;              // this CTA's range of the list of all places
+  long long ctas;
+  auto range = [&](long long total) {
+    N = total * lists;                          // below 2^48, times the CTAs below 2^59
+    ctas = min((long long)gridDim.x, N);
+    if (blockIdx.x >= ctas) return;
+    begin = N * blockIdx.x / ctas;              // parts: one each
+    end = N * (blockIdx.x + 1) / ctas;
+  };
+  int b;
+  long long req_begin;
+  if (p.batch <= 32) {                          // every warp by itself, a request a lane: no barrier on the way to the first load
+    const int len = lane < p.batch ? length(lane) : 0;
+    const unsigned steps = (unsigned)(len + kStep - 1) / kStep, few = min(steps, 1u << 14);
+    unsigned parts[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) parts[k] = __reduce_add_sync(~0u, (few + part_steps(k) - 1) / part_steps(k));
+    cut(__reduce_add_sync(~0u, few), __reduce_max_sync(~0u, few), parts);
+    const unsigned mine = places(len);          // below 2^24, 32 of them below 2^29
+    unsigned incl = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const unsigned v = __shfl_up_sync(~0u, incl, o);
+      if (lane >= o) incl += v;
+    }
+    range(__shfl_sync(~0u, incl, 31));
+    const unsigned has = __ballot_sync(~0u, mine && (long long)(incl - mine) * lists <= begin && begin < (long long)incl * lists);
+    b = has ? __ffs(has) - 1 : 0;
+    req_begin = (long long)__shfl_sync(~0u, incl - mine, b) * lists;
+  } else {
+    const int per = (p.batch + kThreads - 1) / kThreads;
+    const int b0 = min(tid * per, p.batch), b1 = min(b0 + per, p.batch);
     unsigned work = 0, longest = 0, parts[4] = {0, 0, 0, 0};    // what is too large for the whole cut anyway is counted short
-    for (int b = b0; b < b1; ++b) {
-      const unsigned steps = min((unsigned)(length(b) + kStep - 1) / kStep, 1u << 14);
+    for (int i = b0; i < b1; ++i) {
+      const unsigned steps = min((unsigned)(length(i) + kStep - 1) / kStep, 1u << 14);
       work += steps;
       longest = max(longest, steps);
 #pragma unroll
@@ -238,72 +281,56 @@ __global__ void __launch_bounds__(kva::kThreads, kva::per_sm(NT)) kv4_attention_
 #pragma unroll
       for (int k = 0; k < 4; ++k) s_count[warp][2 + k] = parts[k];
     }
-  }
-  __syncthreads();
-  int unit = 0;                                 // steps of a part; 0: the ranges of one long list
-  {
-    unsigned work = 0, longest = 0;
+    __syncthreads();
+    work = longest = 0;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) parts[k] = 0;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
       work += s_count[w][0];
       longest = max(longest, s_count[w][1]);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) parts[k] += s_count[w][2 + k];
     }
-    if ((long long)work * lists < (long long)kShort * gridDim.x)
+    cut(work, longest, parts);
+    long long mine = 0;
+    for (int i = b0; i < b1; ++i) mine += places(length(i));
+    long long incl = mine;
 #pragma unroll
-      for (int k = 3; k >= 0; --k) {
-        unsigned parts = 0;
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long v = __shfl_up_sync(~0u, incl, o);
+      if (lane >= o) incl += v;
+    }
+    if (lane == 31) s_wide[warp] = incl;
+    __syncthreads();
+    long long total = 0, before = incl - mine;
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w) parts += s_count[w][2 + k];
-        if ((long long)parts * lists <= gridDim.x && longest <= part_steps(k) * most_parts(k)) unit = part_steps(k);
+    for (int w = 0; w < kWarps; ++w) {
+      if (w < warp) before += s_wide[w];
+      total += s_wide[w];
+    }
+    range(total);
+    if (mine && before * lists <= begin && begin < (before + mine) * lists) {
+      long long at = before;
+      for (int i = b0; i < b1; ++i) {
+        const int t = places(length(i));
+        if (begin < (at + t) * lists) {
+          s_find = i;
+          s_before = at * lists;
+          break;
+        }
+        at += t;
       }
+    }
+    __syncthreads();
+    b = s_find;                                 // of a CTA with places
+    req_begin = s_before;
   }
-  // a list's places: its parts, or its steps and what stands for the opening
-  auto places = [&](int len) {
-    const int steps = (len + kStep - 1) / kStep;
-    return len <= 0 ? 0 : unit ? (steps + unit - 1) / unit : steps + kOpen;
-  };
-
-  // ---- this CTA's range of the list of all places
-  long long mine = 0;
-  for (int b = b0; b < b1; ++b) mine += places(length(b));
-  long long incl = mine;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const long long v = __shfl_up_sync(~0u, incl, o);
-    if (lane >= o) incl += v;
-  }
-  if (lane == 31) s_wide[warp] = incl;
-  __syncthreads();
-  long long total = 0, before = incl - mine;
-#pragma unroll
-  for (int w = 0; w < kWarps; ++w) {
-    if (w < warp) before += s_wide[w];
-    total += s_wide[w];
-  }
-  const long long N = total * lists;            // below 2^48, times the CTAs below 2^59
-  const long long ctas = min((long long)gridDim.x, N);          // N: one part each
-  const long long begin = blockIdx.x < ctas ? N * blockIdx.x / ctas : 0;
-  const long long end = blockIdx.x < ctas ? N * (blockIdx.x + 1) / ctas : 0;
   // idle rows of the batch
   for (int b = blockIdx.x; b < p.batch; b += gridDim.x)
     if (length(b) == 0)
       for (int i = tid; i < p.heads * p.dv; i += kThreads) kva_store(p.out, (int64_t)b * p.heads * p.dv + i, p.bf16, 0.f);
   if (begin == end) return;
-  if (mine && before * lists <= begin && begin < (before + mine) * lists) {
-    long long at = before;
-    for (int b = b0; b < b1; ++b) {
-      const int t = places(length(b));
-      if (begin < (at + t) * lists) {
-        s_find = b;
-        s_before = at * lists;
-        break;
-      }
-      at += t;
-    }
-  }
-  __syncthreads();
-  int b = s_find;
-  long long req_begin = s_before;
 
   const uint32_t ring = smem_addr(smem) + warp * WARPB, meta = ring + RINGB;
   const int tok_a = kva_token(g);               // rows g and g + 8 of the first product: tokens tok_a and 8 + tok_a
