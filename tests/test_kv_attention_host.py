@@ -103,3 +103,17 @@ def test_reference_quantiser_is_within_half_a_step():
     back = zero.double()[..., None] + scale.double()[..., None] * code
     # 15 steps of a scale that is off by at most 2^-11 of itself
     assert ((back - x.double()).abs() <= scale.double()[..., None] * (0.5 + 15 * 2.0 ** -11)).all()
+
+
+def test_cache_moves_and_releases_rows():
+    from uniql_b200.kv_cache import PagedKV4Cache
+    cache = PagedKV4Cache(1, 5, 1, 64, page_size=16, requests=3, max_tokens=64, device="cpu")
+    cache.block_table[0, :2], cache.lens[0] = torch.tensor([4, 3], dtype=torch.int32), 20
+    cache.block_table[2, :1], cache.lens[2] = torch.tensor([2], dtype=torch.int32), 7
+    cache.free_count -= 3
+    cache.move(2, 2)                                              # onto itself: nothing changes
+    assert cache.block_table[2].tolist() == [2, -1, -1, -1] and cache.lens.tolist() == [20, 0, 7]
+    cache.move(2, 1)
+    assert cache.block_table[1].tolist() == [2, -1, -1, -1] and cache.lens.tolist() == [20, 7, 0] and (cache.block_table[2] == -1).all()
+    cache.release([0, 0])                                         # the second time there is nothing to give back
+    assert cache.free_count.item() == 4 and cache.free_pages[:4].tolist() == [4, 3, 4, 3] and cache.lens.tolist() == [0, 7, 0]

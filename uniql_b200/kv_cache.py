@@ -94,7 +94,9 @@ class PagedKV4Cache:
             self.lens[r] = 0
 
     def move(self, src, dst) -> None:
-        """Make the request of row src the one of the (released) row dst."""
+        """Make the request of row src the one of the (released) row dst: what dst still holds is not given back."""
+        if src == dst:
+            return
         self.block_table[dst] = self.block_table[src]
         self.lens[dst] = self.lens[src]
         self.block_table[src] = -1
