@@ -451,6 +451,31 @@ def test_prompt_requests_do_not_see_each_other():
     assert torch.equal(got[:399], clean[:399]) and got[399:460].isnan().all()
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("nq,nk,heads,kv,dk,dv,causal", [
+    ([300, 1, 0, 40], [300, 1, 0, 700], 42, 6, 64, 64, True), ([5, 130, 64], [133, 130, 1000], 49, 7, 64, 40, True), ([148], [148], 75, 75, 64, 64, True),
+    ([129], [400], 75, 25, 128, 112, False), ([200, 90], [70, 90], 40, 8, 128, 128, True)])
+def test_prompt_two_units_an_item(route, dtype, nq, nk, heads, kv, dk, dv, causal):
+    """More row blocks and heads than the GPU has SMs."""
+    test_prompt(route, dtype, nq, nk, heads, kv, dk, dv, causal)
+
+
+@pytest.mark.parametrize("heads", [4, 80])
+def test_prompt_padding(heads):
+    """Rows behind the last request: NaN there reaches nothing, and their results are zeros."""
+    from uniql_b200 import ops
+    g = _gen(23)
+    n = [100, 61]
+    q, k, v = (_rows(g, 200, h, 64, F16) for h in (heads, heads // 2, heads // 2))
+    cu = _cu(n).cuda()
+    clean = ops.prompt_attention(q[:161].cuda(), k[:161].cuda(), v[:161].cuda(), cu)
+    _prompt_check(clean.cpu(), q[:161], k[:161], v[:161], n, n, True, 1 / 8)
+    for t in (q, k, v):
+        t[161:] = math.nan
+    got = ops.prompt_attention(q.cuda(), k.cuda(), v.cuda(), cu)
+    assert torch.equal(got[:161], clean) and (got[161:] == 0).all()
+
+
 def test_prompt_views(route):
     from uniql_b200 import ops
     g = _gen(22)

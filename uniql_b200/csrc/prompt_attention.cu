@@ -11,11 +11,15 @@
 //   O (tensor memory) += P V, P read from tensor memory, V as an MN-major operand straight from its row-major tile
 // While the softmax of one unit runs the tensor cores work on the other:  warps 0-3 and 4-7 softmax of unit 0 and 1 (they also
 // rescale and store O), warp 8 issues the MMAs, warp 9 the TMA loads (no multicast), warp 10 hands out the items.
+// Few units (at most one an SM) are items of their own: 256 tokens of 28 heads 8.8 us, 12.6 as pairs on half of the SMs.
+//
+// A thread stores 32 bytes of its row at a time: every store instruction touches 32 rows, which takes the load/store unit 32
+// cycles whatever their width (16 packed prompts: 497 us with 16 bytes at a time, 480 with 32).
 //
 // Items.  A CTA stays on its SM and takes one pair of units after the other, by cluster launch control (the grid names every item;
 // a running CTA asks for the place of one that has not begun).  The next item's queries, keys and first scores then run under
 // the end of the one before, and the items even out over the SMs: 16 packed prompts 515 us against 562 as one CTA an item, and
-// 548 when every CTA takes every 148th (9.6 % uneven there).
+// 548 when every CTA takes every 148th (9.6 % uneven there; all three with stores of 16 bytes).
 //
 // Masked places: keys behind a request's last are set to -inf in S, and the rows of V behind it in its last tile, which belong
 // to another request, are cleared in shared memory before they are multiplied by the zeros of P.
@@ -86,6 +90,8 @@ struct PaParams {
   unsigned char* out;
   int* status_word;
   int batch, total_q, total_k, heads, kv_heads, group, dk, dv, causal;
+  int units;                                    // of an item: 2, or 1
+  int wide;                                     // rows of the result are 32-byte aligned
   float scale_log2;
 };
 
@@ -145,6 +151,11 @@ __device__ __forceinline__ void pa_st16(uint32_t taddr, const uint32_t* u) {
       ::"r"(taddr), "r"(u[0]), "r"(u[1]), "r"(u[2]), "r"(u[3]), "r"(u[4]), "r"(u[5]), "r"(u[6]), "r"(u[7]), "r"(u[8]),
         "r"(u[9]), "r"(u[10]), "r"(u[11]), "r"(u[12]), "r"(u[13]), "r"(u[14]), "r"(u[15])
       : "memory");
+}
+__device__ __forceinline__ void pa_store32(void* at, const uint32_t* x) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(at), "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]),
+               "r"(x[4]), "r"(x[5]), "r"(x[6]), "r"(x[7])
+               : "memory");
 }
 __device__ __forceinline__ float pa_max3(float a, float b, float c) {   // NaN if any is
   float r;
@@ -220,6 +231,8 @@ prompt_attention_kernel(const __grid_constant__ PaParams p, const __grid_constan
   tc_fence_after();
   auto begin_q = [&](int b) { return min(max(p.cu_q[b], 0), p.total_q); };
   auto begin_k = [&](int b) { return min(max(p.cu_k[b], 0), p.total_k); };
+  // behind the last key of all the loads fill in zeros by themselves
+  auto dirty = [&](const PaItem& w, int tiles) { return tiles * kKeys > w.nk && w.k0 + w.nk < p.total_k; };
   const uint32_t tmem = *tmem_slot;
   bool timed_out = false;
   // The items of a CTA, one behind the other: every role walks them by itself.  item(k): the k-th one, false behind the last or when a
@@ -241,7 +254,7 @@ prompt_attention_kernel(const __grid_constant__ PaParams p, const __grid_constan
       // products start while the last one's results are written, and whoever is free first takes the next item.
       auto pairs_of = [&](int b) {
         const int n = max(begin_q(b + 1) - begin_q(b), 0);
-        return (long long)(((n + kRows - 1) / kRows) * (long long)p.group + 1) / 2;
+        return (long long)(((n + kRows - 1) / kRows) * (long long)p.group + p.units - 1) / p.units;
       };
       const int per = (p.batch + 31) / 32;
       const int b0 = min(lane * per, p.batch), b1 = min(b0 + per, p.batch);
@@ -284,10 +297,10 @@ prompt_attention_kernel(const __grid_constant__ PaParams p, const __grid_constan
             w.nq = begin_q(b + 1) - w.q0;
             w.k0 = begin_k(b);
             w.nk = max(begin_k(b + 1) - w.k0, 0);
-            const int units = ((w.nq + kRows - 1) / kRows) * p.group, u0 = 2 * (int)(n - 1 - (pair - at));
+            const int units = ((w.nq + kRows - 1) / kRows) * p.group, u0 = p.units * (int)(n - 1 - (pair - at));
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
-              const int u = u0 + t;
+              const int u = t < p.units ? u0 + t : units;
               const int row = u / p.group * kRows;
               int seen = w.nk;                  // query i sees the keys below i + 1 + nk - nq
               if (p.causal) seen = min(w.nk, max(min(row + kRows, w.nq) + w.nk - w.nq, 0));
@@ -354,7 +367,7 @@ prompt_attention_kernel(const __grid_constant__ PaParams p, const __grid_constan
         if (lane == 0) tc_mbar_arrive(bar_loaded);
         it0 += 2 * nmax;
         ++qs;
-        if (nmax * kKeys > w.nk) {              // the last tile of V reaches behind the request: clear those rows
+        if (dirty(w, nmax)) {                   // the last tile of V reaches into another request: clear those rows
           const int it = it0 - 1, s = it % C::kStages;
           if (!timed_out && !tc_mbar_wait(bar_full + 8 * s, (it / C::kStages) & 1)) timed_out = true;
           if (!timed_out) {
@@ -412,7 +425,7 @@ prompt_attention_kernel(const __grid_constant__ PaParams p, const __grid_constan
           tc_mbar_arrive(bar_taken + 8 * (k & 1));
           const int nmax = max(w.n[0], w.n[1]);
           if (nmax == 0) continue;
-          const bool dirty = nmax * kKeys > w.nk;
+          const bool unclean = dirty(w, nmax);
           wait(bar_q, qs & 1);
           wait(bar_full + 8 * (it0 % C::kStages), (it0 / C::kStages) & 1);
 #pragma unroll
@@ -424,7 +437,7 @@ prompt_attention_kernel(const __grid_constant__ PaParams p, const __grid_constan
             const int iv = it0 + 2 * j + 1, ik = iv + 1, sv = iv % C::kStages, sk = ik % C::kStages;
             wait(bar_full + 8 * sv, (iv / C::kStages) & 1);
             if (j + 1 < nmax) wait(bar_full + 8 * sk, (ik / C::kStages) & 1);
-            else if (dirty) wait(bar_clean, cleans & 1);
+            else if (unclean) wait(bar_clean, cleans & 1);
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
               if (j < w.n[t]) {
@@ -440,7 +453,7 @@ prompt_attention_kernel(const __grid_constant__ PaParams p, const __grid_constan
           }
           it0 += 2 * nmax;
           ++qs;
-          cleans += dirty;
+          cleans += unclean;
 #pragma unroll
           for (int t = 0; t < 2; ++t) {
             steps[t] += w.n[t];
@@ -554,17 +567,19 @@ prompt_attention_kernel(const __grid_constant__ PaParams p, const __grid_constan
             for (int e = 0; e < 32; ++e) o[e] = 0.f;
           }
           if (i < nq && !timed_out) {
+            uint32_t x[16];
 #pragma unroll
-            for (int v = 0; v < 4; ++v)
-              if (c + 8 * v < p.dv) {
-                uint32_t x[4];
+            for (int e = 0; e < 16; ++e) x[e] = l == 0.f ? 0u : pa_pack<BF16>(o[2 * e] * inv, o[2 * e + 1] * inv);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                  const float a = l == 0.f ? 0.f : o[8 * v + 2 * e] * inv, b = l == 0.f ? 0.f : o[8 * v + 2 * e + 1] * inv;
-                  x[e] = pa_pack<BF16>(a, b);
-                }
-                *reinterpret_cast<uint4*>(dst + (c + 8 * v) * 2) = make_uint4(x[0], x[1], x[2], x[3]);
+            for (int v = 0; v < 2; ++v) {       // a store instruction touches 32 rows: the fewer, the better
+              unsigned char* at = dst + (c + 16 * v) * 2;
+              if (p.wide) {
+                if (c + 16 * v < p.dv) pa_store32(at, x + 8 * v);
+              } else {
+                if (c + 16 * v < p.dv) *reinterpret_cast<uint4*>(at) = make_uint4(x[8 * v], x[8 * v + 1], x[8 * v + 2], x[8 * v + 3]);
+                if (c + 16 * v + 8 < p.dv) *reinterpret_cast<uint4*>(at + 16) = make_uint4(x[8 * v + 4], x[8 * v + 5], x[8 * v + 6], x[8 * v + 7]);
               }
+            }
           }
         }
       }
@@ -653,9 +668,12 @@ extern "C" int uniql_prompt_attention(const void* q, int64_t q_token_stride, int
   if (st != UNIQL_OK) return st;
   // at most this many pairs of units: every request rounds its row blocks and its pairs up
   const int64_t blocks = total_q / pa::kRows + (batch < total_q ? batch : total_q);
-  const int64_t pairs = (blocks * p.group + 1) / 2 + batch;
   const int64_t sms = device_info().sm_count;
-  int64_t ctas = pairs * kv_heads;
+  // two units share an SM and their keys only when there are not SMs enough for one each
+  p.units = blocks * heads <= sms ? 1 : 2;
+  p.wide = dv % 16 == 0 && !(reinterpret_cast<uintptr_t>(out) & 31);
+  const int64_t items = p.units == 1 ? blocks * p.group : (blocks * p.group + 1) / 2 + batch;
+  int64_t ctas = items * kv_heads;
   if (ctas < sms) ctas = total_q < sms ? (ctas > total_q ? ctas : total_q) : sms;       // rows that nobody owns are cleared by all
   if (ctas > ((int64_t)1 << 31) - 1) return UNIQL_ESHAPE;
   cudaStream_t s = (cudaStream_t)stream;
