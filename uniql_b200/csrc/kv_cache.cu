@@ -321,7 +321,7 @@ __global__ void __launch_bounds__(kAppendThreads, kAppendCtas) kv4_append_kernel
 
 // ------------------------------------------------------------------------------------------------ gather
 // zero + scale * code, fused so that it is rounded once, from the packed rows of a token range.  HBM-bound by the writes.
-// A CTA owns kGatherTokens packed places: one thread per place finds request, page and row (bisection over cu, the batch's last
+// A CTA owns 4, 8 or 16 packed places: one thread per place finds request, page and row (bisection over cu, the batch's last
 // narrowing in shared memory), then all walk the places' rows, DP / 8 lanes a row, one word in and 16 bytes out each.
 constexpr int kGatherThreads = 256, kGatherTokens = 16, kGatherRows = 4, kGatherCu = 1024;
 
@@ -336,6 +336,7 @@ struct GatherParams {
   int64_t ld_table, num_pages, total;
   FastDiv heads;
   int batch, max_blocks, d[2], page_shift;
+  int tokens;                                   // places of a CTA, at most kGatherTokens
 };
 
 template <int DP, bool BF16>
@@ -345,13 +346,13 @@ __global__ void __launch_bounds__(kGatherThreads) kv4_gather_kernel(const __grid
   __shared__ int s_cu[kGatherCu + 1];
   pdl_wait();
   pdl_launch_dependents();
-  const int64_t t0 = (int64_t)blockIdx.x * kGatherTokens;
+  const int64_t t0 = (int64_t)blockIdx.x * p.tokens;
   const int heads = p.heads.d;
   const bool local = p.batch <= kGatherCu;
   if (local)
     for (int i = threadIdx.x; i <= p.batch; i += kGatherThreads) s_cu[i] = p.cu[i];
   __syncthreads();
-  if (threadIdx.x < kGatherTokens) {
+  if (threadIdx.x < p.tokens) {
     const int32_t* cu = local ? s_cu : p.cu;
     const int64_t t = t0 + threadIdx.x;
     int64_t row = -1;
@@ -371,7 +372,7 @@ __global__ void __launch_bounds__(kGatherThreads) kv4_gather_kernel(const __grid
     s_row[threadIdx.x] = row;
   }
   __syncthreads();
-  const uint32_t n = (uint32_t)(p.total - t0 < kGatherTokens ? p.total - t0 : kGatherTokens);
+  const uint32_t n = (uint32_t)(p.total - t0 < p.tokens ? p.total - t0 : p.tokens);
   const uint32_t sub = threadIdx.x % W;
 #pragma unroll
   for (int kv = 0; kv < 2; ++kv) {
@@ -553,7 +554,11 @@ extern "C" int uniql_kv4_gather(const void* codes, const void* scales, int64_t n
   p.out[0] = (unsigned char*)k_out; p.out[1] = (unsigned char*)v_out; p.status_word = status_word;
   p.ld_table = ld_table; p.num_pages = num_pages; p.total = total; p.batch = (int)batch; p.max_blocks = (int)max_blocks;
   p.heads = FastDiv((uint32_t)kv_heads); p.d[0] = (int)dk; p.d[1] = (int)dv; p.page_shift = page_shift_of(page_size);
-  const unsigned ctas = (unsigned)((total + kGatherTokens - 1) / kGatherTokens);
+  const int64_t sms = device_info().sm_count;
+  // Few tokens: fewer a CTA, so that fewer rows follow one another, up to three CTAs an SM (us with 4 / 8 / 16, 8 heads: 64 tokens
+  // 2.5 / - / 4.3, 1000 2.9 / - / 4.5, 2000 4.5 / 3.8 / 4.5, 3200 - / 4.5 / 5.5, 4000 5.6 / 6.5 / 5.6).
+  p.tokens = total <= 12 * sms ? 4 : total <= 24 * sms ? 8 : kGatherTokens;
+  const unsigned ctas = (unsigned)((total + p.tokens - 1) / p.tokens);
   const bool bf16 = dtype == UNIQL_BF16;
   auto kernel = dp == 128 ? (bf16 ? kv4_gather_kernel<128, true> : kv4_gather_kernel<128, false>)
                           : (bf16 ? kv4_gather_kernel<64, true> : kv4_gather_kernel<64, false>);
