@@ -154,7 +154,8 @@ __global__ void __launch_bounds__(kPlanThreads) kv_page_plan_kernel(const __grid
 // reads, 4 bytes a channel against 0.5 written, if the instructions are few: the packed minimum carries NaN along, the codes
 // are rounded by adding 1.5 * 2^23 and joined as the low bits of those sums, and sixteen channels a lane share what a row costs
 // (eight: 50 us for 14760 tokens of 8 heads, 60 MB read; sixteen: 34; with K's and V's rows in one turn and packed
-// arithmetic: 27).  (hi - lo) / 15 is the quotient by the reciprocal and one
+// arithmetic: 27; exact comparisons for the channels near a half-way point alone, not for their whole word: 24).
+// (hi - lo) / 15 is the quotient by the reciprocal and one
 // residual step (Markstein), equal to the division for every mantissa.
 //
 // Codes are taken from a quotient in fp32.  Where that leaves the side of a half-way point open, the two sides are compared
@@ -301,6 +302,11 @@ __global__ void __launch_bounds__(kAppendThreads, kAppendCtas) kv4_append_kernel
           const uint32_t ue = (e >> 1) == 0 ? u[0] : (e >> 1) == 1 ? u[1] : (e >> 1) == 2 ? u[2] : u[3];
           float xe = BF16 ? __uint_as_float((e & 1) ? ue & 0xffff0000u : ue << 16)
                           : __half2float(__ushort_as_half((unsigned short)(ue >> (16 * (e & 1)))));
+          const float y = fmaf(xe, inv, zi), n = rintf(y);
+          if (!odd && fabsf(y - n) <= 0.49998f) {
+            w |= (uint32_t)(int)n << (4 * e);
+            continue;
+          }
           xe = fminf(fmaxf(xe, -65504.f), 65504.f);
           w |= kv4_exact_code(xe, z, s, (xe - z) * inv) << (4 * e);
         }
@@ -519,7 +525,7 @@ extern "C" int uniql_kv4_append(const void* k, int64_t k_token_stride, int64_t k
   const bool bf16 = dtype == UNIQL_BF16;
   auto kernel = dp == 128 ? (bf16 ? kv4_append_kernel<128, true> : kv4_append_kernel<128, false>)
                           : (bf16 ? kv4_append_kernel<64, true> : kv4_append_kernel<64, false>);
-  const int64_t per = kAppendThreads / (dp / 16), cap = 4 * kAppendCtas * (int64_t)device_info().sm_count;     // four waves even out: 26.7 us against 30.2 of one
+  const int64_t per = kAppendThreads / (dp / 16), cap = 4 * kAppendCtas * (int64_t)device_info().sm_count;     // four waves even out: 27 us against 30 of one
   const int64_t slab = ((int64_t)1 << 30) / kv_heads;                   // tokens of a launch: rows stay below 2^31
   for (int64_t t0 = 0; t0 < tokens; t0 += slab) {
     const int64_t n = tokens - t0 < slab ? tokens - t0 : slab;
