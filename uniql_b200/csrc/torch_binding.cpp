@@ -3,9 +3,11 @@
 // their forward: shape checks, output allocation, scratch and the C-ABI call cost a few microseconds here instead of the
 // tens of microseconds the same steps cost in Python over ctypes.  Nothing is computed in this file; every function ends
 // in a call of libuniql_b200.so with raw pointers and the current stream.
+
 #include <torch/extension.h>
 
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 
 #include <mutex>
@@ -295,6 +297,11 @@ int64_t stride_of(const at::Tensor& x, int64_t dim) {          // of a dimension
   return x.size(dim) > 1 ? x.stride(dim) : (dim == 0 ? x.size(1) * x.size(2) : x.size(2));
 }
 
+// A new tensor, straight from the allocator: half of what at::empty costs through the dispatcher.
+at::Tensor new_tensor(at::IntArrayRef sizes, at::ScalarType type, at::Device device) {
+  return at::Tensor(at::detail::empty_cuda(sizes, type, device, std::nullopt));
+}
+
 struct CacheView {
   int64_t pages, heads, page, dp;
 };
@@ -336,7 +343,7 @@ std::vector<at::Tensor> kv_page_plan(const at::Tensor& lens, const at::Tensor& n
   const c10::cuda::CUDAGuard guard(lens.device());
   const int dev = lens.device().index();
   const int64_t longs = 16 * total_new, ints = 4 * (batch + 1);
-  at::Tensor buf = at::empty({longs + 2 * ints + 4}, lens.options().dtype(at::kByte));
+  at::Tensor buf = new_tensor({longs + 2 * ints + 4}, at::kByte, lens.device());
   at::Tensor slots = part_of(buf, 0, total_new, at::kLong), positions = part_of(buf, 8 * total_new, total_new, at::kLong);
   at::Tensor cu = part_of(buf, longs, batch + 1, at::kInt);
   at::Tensor lens_out = in_place ? lens : part_of(buf, longs + ints, batch, at::kInt);
@@ -390,8 +397,8 @@ std::vector<at::Tensor> kv4_gather(const at::Tensor& codes, const at::Tensor& sc
   TORCH_CHECK(total >= 0 && dk > 0 && dv > 0, "total, head_dim_k and head_dim_v must not be negative");
   const c10::cuda::CUDAGuard guard(codes.device());
   const int dev = codes.device().index();
-  const auto opt = scales.options().dtype(bf16 ? at::kBFloat16 : at::kHalf);
-  at::Tensor k = at::empty({total, cv.heads, dk}, opt), v = at::empty({total, cv.heads, dv}, opt);
+  const auto type = bf16 ? at::kBFloat16 : at::kHalf;
+  at::Tensor k = new_tensor({total, cv.heads, dk}, type, codes.device()), v = new_tensor({total, cv.heads, dv}, type, codes.device());
   at::Tensor status = status_tensor(dev);
   const int code = uniql_kv4_gather(codes.data_ptr(), scales.data_ptr(), cv.pages, cv.page, cv.dp, cv.heads,
                                     (const int32_t*)block_table.data_ptr(), batch > 1 ? block_table.stride(0) : width, width, batch,
@@ -418,7 +425,7 @@ at::Tensor kv4_attention(const at::Tensor& q, const at::Tensor& codes, const at:
   const c10::cuda::CUDAGuard guard(q.device());
   const int dev = q.device().index();
   const at::Tensor q3 = q.stride(2) == 1 || q.size(2) == 1 ? q : q.contiguous();
-  at::Tensor out = at::empty({batch, q.size(1), dv}, q.options());
+  at::Tensor out = new_tensor({batch, q.size(1), dv}, q.scalar_type(), q.device());
   if (batch == 0) return out;
   cudaStream_t stream = at::cuda::getCurrentCUDAStream(dev).stream();
   const size_t need = uniql_kv4_attention_scratch_bytes(batch, q.size(1), cv.heads, cv.dp);
@@ -450,7 +457,7 @@ at::Tensor prompt_attention(const at::Tensor& q, const at::Tensor& k, const at::
   const c10::cuda::CUDAGuard guard(q.device());
   const int dev = q.device().index();
   const at::Tensor q3 = head_rows(q), k3 = head_rows(k), v3 = head_rows(v);
-  at::Tensor out = at::empty({q.size(0), q.size(1), v.size(2)}, q.options());
+  at::Tensor out = new_tensor({q.size(0), q.size(1), v.size(2)}, q.scalar_type(), q.device());
   at::Tensor status = status_tensor(dev);
   const int code = uniql_prompt_attention(q3.data_ptr(), stride_of(q3, 0), stride_of(q3, 1), k3.data_ptr(), stride_of(k3, 0),
                                           stride_of(k3, 1), v3.data_ptr(), stride_of(v3, 0), stride_of(v3, 1),
