@@ -460,6 +460,16 @@ def test_prompt_two_units_an_item(route, dtype, nq, nk, heads, kv, dk, dv, causa
     test_prompt(route, dtype, nq, nk, heads, kv, dk, dv, causal)
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("nq,nk,heads,kv,dk,dv,causal", [
+    ([1] * 9, [3] * 9, 128, 1, 64, 64, True), ([2, 0, 5], [200, 7, 5], 130, 1, 64, 64, True), ([3, 1], [3, 129], 65, 1, 128, 128, True),
+    ([18, 19, 17, 1], [18, 190, 17, 0], 14, 2, 128, 128, True), ([43, 42], [43, 300], 9, 3, 128, 72, True), ([1] * 150, [1] * 150, 10, 2, 64, 64, True),
+    ([33] * 20, [40] * 20, 64, 16, 112, 112, False), ([64, 65, 63], [64, 65, 200], 4, 2, 128, 128, True)])
+def test_prompt_short_requests(route, dtype, nq, nk, heads, kv, dk, dv, causal):
+    """A group's heads share a row block: groups that divide it, that do not, that fill it and that are larger."""
+    test_prompt(route, dtype, nq, nk, heads, kv, dk, dv, causal)
+
+
 @pytest.mark.parametrize("heads", [4, 80])
 def test_prompt_padding(heads):
     """Rows behind the last request: NaN there reaches nothing, and their results are zeros."""

@@ -91,6 +91,8 @@ struct PaParams {
   int* status_word;
   int batch, total_q, total_k, heads, kv_heads, group, dk, dv, causal;
   int units;                                    // of an item: 2, or 1
+  int pack, tokens;                             // of a unit: query heads (1, or the whole group) and tokens (128 / pack)
+  int parts;                                    // group / pack: units of a row block and kv head
   int wide;                                     // rows of the result are 32-byte aligned
   float scale_log2;
 };
@@ -254,7 +256,7 @@ prompt_attention_kernel(const __grid_constant__ PaParams p, const __grid_constan
       // products start while the last one's results are written, and whoever is free first takes the next item.
       auto pairs_of = [&](int b) {
         const int n = max(begin_q(b + 1) - begin_q(b), 0);
-        return (long long)(((n + kRows - 1) / kRows) * (long long)p.group + p.units - 1) / p.units;
+        return (long long)(((n + p.tokens - 1) / p.tokens) * (long long)p.parts + p.units - 1) / p.units;
       };
       const int per = (p.batch + 31) / 32;
       const int b0 = min(lane * per, p.batch), b1 = min(b0 + per, p.batch);
@@ -297,15 +299,15 @@ prompt_attention_kernel(const __grid_constant__ PaParams p, const __grid_constan
             w.nq = begin_q(b + 1) - w.q0;
             w.k0 = begin_k(b);
             w.nk = max(begin_k(b + 1) - w.k0, 0);
-            const int units = ((w.nq + kRows - 1) / kRows) * p.group, u0 = p.units * (int)(n - 1 - (pair - at));
+            const int units = ((w.nq + p.tokens - 1) / p.tokens) * p.parts, u0 = p.units * (int)(n - 1 - (pair - at));
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
               const int u = t < p.units ? u0 + t : units;
-              const int row = u / p.group * kRows;
+              const int row = u / p.parts * p.tokens;
               int seen = w.nk;                  // query i sees the keys below i + 1 + nk - nq
-              if (p.causal) seen = min(w.nk, max(min(row + kRows, w.nq) + w.nk - w.nq, 0));
+              if (p.causal) seen = min(w.nk, max(min(row + p.tokens, w.nq) + w.nk - w.nq, 0));
               w.row[t] = row;
-              w.head[t] = u < units ? w.kvh * p.group + u % p.group : -1;
+              w.head[t] = u < units ? w.kvh * p.group + u % p.parts * p.pack : -1;
               w.n[t] = u < units ? (seen + kKeys - 1) / kKeys : 0;
             }
             s_item[k & 1] = w;
@@ -344,7 +346,7 @@ prompt_attention_kernel(const __grid_constant__ PaParams p, const __grid_constan
         if (tc_elect()) {
           if (qs > 0 && !tc_mbar_wait(bar_qfree, (qs - 1) & 1)) timed_out = true;
           if (!timed_out) {
-            tc_mbar_expect_tx(bar_q, ((w.n[0] > 0) + (w.n[1] > 0)) * C::kTileBytes);
+            tc_mbar_expect_tx(bar_q, ((w.n[0] > 0) + (w.n[1] > 0)) * p.tokens * p.pack * DP * 2);
 #pragma unroll
             for (int t = 0; t < 2; ++t)
               if (w.n[t] > 0)
@@ -469,13 +471,15 @@ prompt_attention_kernel(const __grid_constant__ PaParams p, const __grid_constan
       const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
       const uint32_t ts = tmem + t * 128 + lanes, to = tmem + 256 + t * 128 + lanes;
       const float f = p.scale_log2;
+      const int r = (warp & 3) * 32 + lane, my_token = r / p.pack, my_head = r - my_token * p.pack;
+      const int tokens = p.tokens;
       PaItem w;
       int steps = 0;                            // of this unit in the items before
       for (int k = 0; item(k, w, true); ++k) {
       __syncwarp();
       if (lane == 0) tc_mbar_arrive(bar_taken + 8 * (k & 1));
       const int nt = t ? w.n[1] : w.n[0], row0 = t ? w.row[1] : w.row[0], head = t ? w.head[1] : w.head[0];
-      const int nq = w.nq, nk = w.nk, shift = nk - nq, i = row0 + (warp & 3) * 32 + lane;
+      const int nq = w.nq, nk = w.nk, shift = nk - nq, i = row0 + my_token;
       const int limit = p.causal ? min(nk, max(i + 1 + shift, 0)) : nk;
       const int full = p.causal ? min(nk, max(row0 + 1 + shift, 0)) : nk;       // keys that every row of the unit sees
       float m = -INFINITY, l = 0.f;
@@ -498,7 +502,7 @@ prompt_attention_kernel(const __grid_constant__ PaParams p, const __grid_constan
 #pragma unroll
           for (int e = 0; e < 4; ++e) top4[e] = pa_max3(top4[e], s[c + e], s[c + 4 + e]);
         float top = pa_max3(pa_max3(top4[0], top4[1], top4[2]), pa_max3(top4[3], s[124], s[125]), pa_max3(s[126], s[127], s[127]));
-        top = i < nq ? top * f : -INFINITY;     // rows of another request have no say in when m is raised
+        top = i < nq && my_token < tokens ? top * f : -INFINITY;        // rows of another request, or of none, have no say in when m is raised
         if (top != top) m = top;                // a NaN among the scores: all of the row is
         if (__any_sync(~0u, top > m + 8.f)) {
           const float mn = fmaxf(m, top);
@@ -550,7 +554,7 @@ prompt_attention_kernel(const __grid_constant__ PaParams p, const __grid_constan
           tc_fence_after();
         }
         const float inv = l == 0.f ? 0.f : 1.f / l;
-        unsigned char* dst = p.out + ((size_t)(w.q0 + i) * p.heads + head) * p.dv * 2;
+        unsigned char* dst = p.out + ((size_t)(w.q0 + i) * p.heads + head + my_head) * p.dv * 2;
 #pragma unroll 1
         for (int c = 0; c < DP; c += 32) {
           float o[32];
@@ -566,7 +570,7 @@ prompt_attention_kernel(const __grid_constant__ PaParams p, const __grid_constan
 #pragma unroll
             for (int e = 0; e < 32; ++e) o[e] = 0.f;
           }
-          if (i < nq && !timed_out) {
+          if (i < nq && my_token < tokens && !timed_out) {
             uint32_t x[16];
 #pragma unroll
             for (int e = 0; e < 16; ++e) x[e] = l == 0.f ? 0u : pa_pack<BF16>(o[2 * e] * inv, o[2 * e + 1] * inv);
@@ -595,14 +599,14 @@ prompt_attention_kernel(const __grid_constant__ PaParams p, const __grid_constan
   }
 }
 
-// rows [tokens, heads, d] as a 3-D tensor, boxes of 64 channels x 1 head x 128 tokens; what lies outside reads as zero
+// rows [tokens, heads, d] as a 3-D tensor, boxes of 64 channels x box_heads x box_tokens; what lies outside reads as zero
 static int pa_map(CUtensorMap* map, const void* x, int64_t tokens, int64_t heads, int64_t d, int64_t token_stride,
-                  int64_t head_stride, bool bf16) {
+                  int64_t head_stride, bool bf16, int box_heads = 1, int box_tokens = 128) {
   EncodeTiledFn enc = encode_tiled_fn();
   if (!enc) return cuda_fail(cudaErrorNotSupported);
   cuuint64_t dims[3] = {(cuuint64_t)d, (cuuint64_t)heads, (cuuint64_t)tokens};
   cuuint64_t strides[2] = {(cuuint64_t)head_stride * 2, (cuuint64_t)token_stride * 2};
-  cuuint32_t box[3] = {64, 1, 128}, estr[3] = {1, 1, 1};
+  cuuint32_t box[3] = {64, (cuuint32_t)box_heads, (cuuint32_t)box_tokens}, estr[3] = {1, 1, 1};
   if (enc(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void*>(x), dims, strides,
           box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
@@ -660,19 +664,26 @@ extern "C" int uniql_prompt_attention(const void* q, int64_t q_token_stride, int
   p.group = (int)(heads / kv_heads); p.dk = (int)dk; p.dv = (int)dv; p.causal = causal != 0;
   p.scale_log2 = softmax_scale * 1.44269504088896340736f;
   const bool bf16 = dtype == UNIQL_BF16;
+  // Rows of a unit: 128 tokens of one query head, or, where that leaves fewer units (short requests), fewer tokens of the whole
+  // group, a token's heads side by side.  At most this many units: every request rounds its row blocks up.
+  const int64_t sms = device_info().sm_count, some = batch < total_q ? batch : total_q;
+  p.pack = 1;
+  if (p.group > 1 && p.group <= pa::kRows) {
+    const int64_t apart = (total_q / pa::kRows + some) * p.group, packed = total_q / (pa::kRows / p.group) + some;
+    if (packed * 8 <= apart * 7) p.pack = p.group;
+  }
+  p.tokens = pa::kRows / p.pack; p.parts = p.group / p.pack;
   CUtensorMap qm, km, vm;
-  int st = pa_map(&qm, q, total_q, heads, dk, q_token_stride, q_head_stride, bf16);
+  int st = pa_map(&qm, q, total_q, heads, dk, q_token_stride, q_head_stride, bf16, p.pack, p.tokens);
   // without keys no tile of K or V is ever loaded: the maps only have to be valid
   if (st == UNIQL_OK) st = total_k ? pa_map(&km, k, total_k, kv_heads, dk, k_token_stride, k_head_stride, bf16) : (km = qm, UNIQL_OK);
   if (st == UNIQL_OK) st = total_k ? pa_map(&vm, v, total_k, kv_heads, dv, v_token_stride, v_head_stride, bf16) : (vm = qm, UNIQL_OK);
   if (st != UNIQL_OK) return st;
-  // at most this many pairs of units: every request rounds its row blocks and its pairs up
-  const int64_t blocks = total_q / pa::kRows + (batch < total_q ? batch : total_q);
-  const int64_t sms = device_info().sm_count;
+  const int64_t blocks = total_q / p.tokens + some;
   // two units share an SM and their keys only when there are not SMs enough for one each
-  p.units = blocks * heads <= sms ? 1 : 2;
+  p.units = blocks * p.parts * kv_heads <= sms ? 1 : 2;
   p.wide = dv % 16 == 0 && !(reinterpret_cast<uintptr_t>(out) & 31);
-  const int64_t items = p.units == 1 ? blocks * p.group : (blocks * p.group + 1) / 2 + batch;
+  const int64_t items = p.units == 1 ? blocks * p.parts : (blocks * p.parts + 1) / 2 + batch;
   int64_t ctas = items * kv_heads;
   if (ctas < sms) ctas = total_q < sms ? (ctas > total_q ? ctas : total_q) : sms;       // rows that nobody owns are cleared by all
   if (ctas > ((int64_t)1 << 31) - 1) return UNIQL_ESHAPE;
