@@ -43,13 +43,17 @@ constexpr int kThreads = 384;                   // three warpgroups; the third h
 constexpr int kSoftmaxRegs = 208, kOtherRegs = 80;      // 2 * 208 + 80 <= 3 * 168, what the block is launched with
 constexpr int kRows = 128, kKeys = 128;
 constexpr int kTmemCols = 512;                  // S0, S1, O0, O1: 128 columns each
+// Barriers that say "rows of other requests cleared", taken in turn.  One would not do: the load warp may clear the next item's last
+// tile before the MMA thread has seen this one's phase, whose parity would then never come.  With two, clearing c + 2 waits for the
+// queries of the item behind that of clearing c (bar_qfree), which the MMA thread frees only behind its wait for clearing c.
+constexpr int kCleans = 2;
 template <int DP>
 struct Cfg {
   static constexpr int kTileBytes = 128 * DP * 2;
   static constexpr int kStages = 5;
   static constexpr int kOffKv = 2 * kTileBytes;
   static constexpr int kOffBar = kOffKv + kStages * kTileBytes;
-  static constexpr int kBars = 2 + 2 * kStages + 2 + 4 + 2 + 2 + 1 + 4 + 2;
+  static constexpr int kBars = 1 + 2 * kStages + 2 + 4 + 2 + kCleans + 1 + 2 + 2 + 2 + 1 + 1;
   static constexpr int kSmem = kOffBar + kBars * 8 + 16 + 1024;
   static_assert(kSmem <= 227 * 1024, "shared memory");
 };
@@ -189,7 +193,7 @@ prompt_attention_kernel(const __grid_constant__ PaParams p, const __grid_constan
   const uint32_t sbase = tc_smem_addr(smem);
   const uint32_t bar_q = sbase + C::kOffBar, bar_full = bar_q + 8, bar_empty = bar_full + 8 * C::kStages;
   const uint32_t bar_s = bar_empty + 8 * C::kStages, bar_p = bar_s + 16, bar_o = bar_p + 32, bar_clean = bar_o + 16;
-  const uint32_t bar_qfree = bar_clean + 8, bar_ofree = bar_qfree + 8, bar_item = bar_ofree + 16, bar_taken = bar_item + 16, bar_next = bar_taken + 16, bar_loaded = bar_next + 8;
+  const uint32_t bar_qfree = bar_clean + 8 * kCleans, bar_ofree = bar_qfree + 8, bar_item = bar_ofree + 16, bar_taken = bar_item + 16, bar_next = bar_taken + 16, bar_loaded = bar_next + 8;
   volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(smem + C::kOffBar + C::kBars * 8);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
@@ -214,7 +218,7 @@ prompt_attention_kernel(const __grid_constant__ PaParams p, const __grid_constan
       tc_mbar_init(bar_p + 16 * t + 8, 4);
       tc_mbar_init(bar_o + 8 * t, 1);
     }
-    tc_mbar_init(bar_clean, 1);
+    for (int t = 0; t < kCleans; ++t) tc_mbar_init(bar_clean + 8 * t, 1);
     tc_mbar_init(bar_qfree, 1);
     tc_mbar_init(bar_next, 1);
     tc_mbar_init(bar_loaded, 1);
@@ -335,7 +339,7 @@ prompt_attention_kernel(const __grid_constant__ PaParams p, const __grid_constan
     if (warp == kLoadWarp) {
       // ------------------------------------------------------------------ loads: Q, then K 0, V 0, K 1, V 1, ... of every item
       PaItem w;
-      int it0 = 0, qs = 0;                      // tiles and items loaded so far
+      int it0 = 0, qs = 0, cleans = 0;          // tiles and items loaded, tiles cleared so far
       for (int k = 0; item(k, w, true); ++k) {
         __syncwarp();
         if (lane == 0) tc_mbar_arrive(bar_taken + 8 * (k & 1));
@@ -383,7 +387,8 @@ prompt_attention_kernel(const __grid_constant__ PaParams p, const __grid_constan
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
           }
           timed_out = __any_sync(~0u, timed_out);
-          if (lane == 0) tc_mbar_arrive(bar_clean);
+          if (lane == 0) tc_mbar_arrive(bar_clean + 8 * (cleans % kCleans));
+          ++cleans;
         }
       }
       // given up: what has been asked for arrives before the CTA leaves (each tile's wait is bounded, too)
@@ -440,7 +445,7 @@ prompt_attention_kernel(const __grid_constant__ PaParams p, const __grid_constan
             const int iv = it0 + 2 * j + 1, ik = iv + 1, sv = iv % C::kStages, sk = ik % C::kStages;
             wait(bar_full + 8 * sv, (iv / C::kStages) & 1);
             if (j + 1 < nmax) wait(bar_full + 8 * sk, (ik / C::kStages) & 1);
-            else if (unclean) wait(bar_clean, cleans & 1);
+            else if (unclean) wait(bar_clean + 8 * (cleans % kCleans), (cleans / kCleans) & 1);
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
               if (j < w.n[t]) {
