@@ -34,3 +34,21 @@ def test_prompt_many_items_with_foreign_rows(lens, heads, kv):
         assert torch.equal(ops.prompt_attention(*args), first)
     _prompt_check(first.cpu(), q, k, v, lens, lens, True, 1 / 8)
     assert ops.read_and_clear_status("cuda") == 0
+
+
+@pytest.mark.parametrize("batch", [4050, 4051, 4095, 4096, 16384])
+def test_plan_large_batches(batch):
+    """Around the size at which the plan's tables no longer fit the shared memory that a kernel gets by default, and the largest."""
+    from uniql_b200 import ops
+    g = _gen(batch)
+    lens, new = torch.randint(0, 40, (batch,), generator=g), torch.randint(0, 4, (batch,), generator=g)
+    table = torch.full((batch, 3), -1, dtype=torch.int32)
+    for i, n in enumerate(lens.tolist()):
+        table[i, :-(-n // 16)] = i % 7
+    free = torch.randperm(batch * 3, generator=g).int()
+    total = int(new.sum()) + 2
+    want = ref.plan(lens, new, table, free, free.numel(), 16, total)
+    d_table = table.cuda()
+    got = ops.kv_page_plan(lens.int().cuda(), new.int().cuda(), d_table, free.cuda(), torch.tensor([free.numel()], dtype=torch.int32).cuda(), 16, total)
+    assert torch.equal(d_table.cpu(), want[0]) and got[0].tolist() == want[1] and got[1].tolist() == want[2]
+    assert got[2].tolist() == want[3] and got[3].tolist() == want[4] and got[4].tolist() == [want[5]]

@@ -466,15 +466,14 @@ extern "C" int uniql_kv_page_plan(const int32_t* lens, const int32_t* new_lens, 
   p.cu_new = cu_new; p.lens_out = lens_out; p.free_count_out = free_count_out; p.status_word = status_word;
   p.total_new = total_new; p.batch = (int)batch; p.max_blocks = (int)max_blocks; p.free_cap = (int)free_cap; p.page_shift = shift;
   const size_t smem = (3 * (size_t)batch + 2) * sizeof(int);
-  if (smem > 48 * 1024) {
-    static thread_local bool attr_set[64] = {};
-    int dev = 0;
-    cudaGetDevice(&dev);
-    if (dev < 0 || dev >= 64 || !attr_set[dev]) {
-      UNIQL_CUDA_TRY(cudaFuncSetAttribute(kv_page_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                          (3 * UNIQL_KV_MAX_BATCH + 2) * (int)sizeof(int)));
-      if (dev >= 0 && dev < 64) attr_set[dev] = true;
-    }
+  // raised for every size: what a kernel gets by default counts its static shared memory too
+  static thread_local bool attr_set[64] = {};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= 64 || !attr_set[dev]) {
+    UNIQL_CUDA_TRY(cudaFuncSetAttribute(kv_page_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                        (3 * UNIQL_KV_MAX_BATCH + 2) * (int)sizeof(int)));
+    if (dev >= 0 && dev < 64) attr_set[dev] = true;
   }
   const int64_t ctas = (total_new + kPlanThreads - 1) / kPlanThreads;
   auto launch = [&](int64_t grid, int cluster, int lists, int totals) {
