@@ -43,7 +43,8 @@ enum {
   UNIQL_STATUS_WAIT_TIMEOUT = 2,  /* a bounded wait (asynchronous copy, or words another GPU has to write) gave up;
                                      the output is invalid */
   UNIQL_STATUS_BAD_INDEX = 4,     /* a slicing index pointed outside the source layer; that column / row was written as zeros.
-                                     KV cache: a slot or page number outside the cache; that token was skipped / read as absent */
+                                     KV cache: a slot or page number outside the cache; that token was skipped / read as absent.  Packed rows: bounds
+                                     that leave the rows or descend */
   UNIQL_STATUS_NO_PAGE = 8        /* uniql_kv_page_plan: the free stack or a row of the block table was too short */
 };
 
@@ -366,7 +367,8 @@ int uniql_w4a16_swap_plan_check(void);
  *
  * uniql_kv4_gather: rows of tokens starts[i] .. starts[i] + (cu[i + 1] - cu[i]) - 1 of every request i (starts NULL: from 0),
  *   packed: k_out [total, kv_heads, dk], v_out [total, kv_heads, dv], each value rounded once.  Places that no request
- *   covers, and tokens on a page outside the cache, are zeros.
+ *   covers, and tokens on a page outside the cache, are zeros.  Tokens behind the last place are left out
+ *   (UNIQL_STATUS_BAD_INDEX).
  *
  * uniql_kv4_attention: one query token per request over its first lens[i] cached tokens (grouped heads: query head h reads kv head
  *   h / (heads / kv_heads)): out[i, h] = softmax(softmax_scale * q k^T) v in fp32, rounded once.  A V scale of 0 (a row that was
@@ -378,8 +380,10 @@ int uniql_w4a16_swap_plan_check(void);
  * uniql_prompt_attention: packed prompts.  Request i owns rows cu_q[i] .. cu_q[i + 1] - 1 of q [total_q, heads, dk] and out
  *   [total_q, heads, dv] and rows cu_k[i] .. of k, v [total_k, kv_heads, dk / dv].  causal: query j sees the keys up to j + (keys -
  *   queries), so that the last query sees them all; a query that sees none gives zeros, and so do rows of `out` that no
- *   request owns.  k and v of tokens that other requests own never reach a request, whatever they hold; within a request a
- *   non-finite v may reach queries in front of it that share its 128-row tile.
+ *   request owns.  A request whose rows of q, k and v do not all exist, or whose bounds descend, has no keys
+ *   (UNIQL_STATUS_BAD_INDEX); where cu_q descends, rows of `out` may be left unwritten.  k and v of tokens that other requests
+ *   own never reach a request, whatever they hold; within a request a non-finite v may reach queries in front of it that share
+ *   its 128-row tile.
  *   Rows must be 16-byte aligned (strides multiples of 8).  P is rounded to the input type in front of the second product.  At
  *   most 2^26 keys.
  */

@@ -358,6 +358,10 @@ __global__ void __launch_bounds__(kGatherThreads) kv4_gather_kernel(const __grid
   if (local)
     for (int i = threadIdx.x; i <= p.batch; i += kGatherThreads) s_cu[i] = p.cu[i];
   __syncthreads();
+  if (blockIdx.x == 0 && threadIdx.x == 0 && p.batch > 0 && p.status_word) {
+    const int32_t* cu = local ? s_cu : p.cu;
+    if (cu[0] < 0 || cu[p.batch] > p.total) atomicOr(p.status_word, UNIQL_STATUS_BAD_INDEX);       // tokens that have no place
+  }
   if (threadIdx.x < p.tokens) {
     const int32_t* cu = local ? s_cu : p.cu;
     const int64_t t = t0 + threadIdx.x;

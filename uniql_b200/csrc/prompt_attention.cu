@@ -11,7 +11,8 @@
 //   P (16-bit, on the first 64 of S's columns) -- four softmax warps, one row a thread
 //   O (tensor memory) += P V, P read from tensor memory, V as an MN-major operand straight from its row-major tile
 // While the softmax of one unit runs the tensor cores work on the other:  warps 0-3 and 4-7 softmax of unit 0 and 1 (they also
-// rescale and store O), warp 8 issues the MMAs, warp 9 the TMA loads (no multicast), warp 10 hands out the items.
+// rescale and store O), warp 8 issues the MMAs, warp 9 the TMA loads (no multicast), warp 10 hands out the items,
+// warp 11 looks the requests' bounds over.
 // Few units (at most one an SM) are items of their own: 256 tokens of 28 heads 8.8 us, 12.6 as pairs on half of the SMs.
 //
 // A thread stores 32 bytes of its row at a time: every store instruction touches 32 rows, which takes the load/store unit 32
@@ -38,8 +39,8 @@
 namespace uniql {
 
 namespace pa {
-constexpr int kMmaWarp = 8, kLoadWarp = 9, kPlanWarp = 10;        // warps 0-7: softmax
-constexpr int kThreads = 384;                   // three warpgroups; the third has an idle warp
+constexpr int kMmaWarp = 8, kLoadWarp = 9, kPlanWarp = 10, kCheckWarp = 11;       // warps 0-7: softmax
+constexpr int kThreads = 384;                   // three warpgroups
 constexpr int kSoftmaxRegs = 208, kOtherRegs = 80;      // 2 * 208 + 80 <= 3 * 168, what the block is launched with
 constexpr int kRows = 128, kKeys = 128;
 constexpr int kTmemCols = 512;                  // S0, S1, O0, O1: 128 columns each
@@ -238,6 +239,11 @@ prompt_attention_kernel(const __grid_constant__ PaParams p, const __grid_constan
   tc_fence_after();
   auto begin_q = [&](int b) { return min(max(p.cu_q[b], 0), p.total_q); };
   auto begin_k = [&](int b) { return min(max(p.cu_k[b], 0), p.total_k); };
+  // a request whose rows all exist; one that is not has no keys: with some of its rows cut off its queries would see the wrong ones
+  auto sound = [&](int b) {
+    const int q0 = p.cu_q[b], q1 = p.cu_q[b + 1], k0 = p.cu_k[b], k1 = p.cu_k[b + 1];
+    return 0 <= q0 && q0 <= q1 && q1 <= p.total_q && 0 <= k0 && k0 <= k1 && k1 <= p.total_k;
+  };
   // behind the last key of all the loads fill in zeros by themselves
   auto dirty = [&](const PaItem& w, int tiles) { return tiles * kKeys > w.nk && w.k0 + w.nk < p.total_k; };
   const uint32_t tmem = *tmem_slot;
@@ -303,7 +309,7 @@ prompt_attention_kernel(const __grid_constant__ PaParams p, const __grid_constan
             w.q0 = begin_q(b);
             w.nq = begin_q(b + 1) - w.q0;
             w.k0 = begin_k(b);
-            w.nk = max(begin_k(b + 1) - w.k0, 0);
+            w.nk = sound(b) ? begin_k(b + 1) - w.k0 : 0;
             const int units = ((w.nq + p.tokens - 1) / p.tokens) * p.parts, u0 = p.units * (int)(n - 1 - (pair - at));
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
@@ -335,6 +341,11 @@ prompt_attention_kernel(const __grid_constant__ PaParams p, const __grid_constan
         if (timed_out) break;
         more = pa_next(tc_smem_addr(&s_next[k & 1]), x);
       }
+    }
+    if (warp == kCheckWarp) {                   // nobody waits for it: the bounds of all requests, over all CTAs
+      bool all = true;
+      for (long long b = blockIdx.x * 32ll + lane; b < p.batch; b += gridDim.x * 32ll) all &= sound((int)b);
+      if (!all && p.status_word) atomicOr(p.status_word, UNIQL_STATUS_BAD_INDEX);
     }
     if (warp == kLoadWarp) {
       // ------------------------------------------------------------------ loads: Q, then K 0, V 0, K 1, V 1, ... of every item

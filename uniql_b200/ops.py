@@ -35,8 +35,8 @@ def status_word(device: torch.device) -> torch.Tensor:
 
 def read_and_clear_status(device) -> int:
     """Synchronising read of the kernel diagnostics word (bit 0: an embedding id was out of range; bit 1: a bounded
-    wait gave up; bit 2: a slicing index was outside the source layer, or a slot or page outside the KV cache; bit 3: a page
-    plan ran out of free pages or of columns of the block table)."""
+    wait gave up; bit 2: a slicing index was outside the source layer, or a slot or page outside the KV cache, or bounds of
+    packed rows named rows that do not exist; bit 3: a page plan ran out of free pages or of columns of the block table)."""
     t = status_word(torch.device(device))
     v = int(t.item())
     t.zero_()
@@ -524,7 +524,7 @@ def kv4_gather(codes: torch.Tensor, scales: torch.Tensor, block_table: torch.Ten
                head_dim_v: int | None = None, dtype: torch.dtype = torch.float16, starts: torch.Tensor | None = None):
     """The cached rows of a token range of every request, dequantised and packed: request i gives cu[i + 1] - cu[i] tokens from
     starts[i] on (None: from its first).  Returns k [total, kv_heads, head_dim_k] and v [total, kv_heads, head_dim_v]; places behind
-    cu[-1] are zeros."""
+    cu[-1] are zeros; tokens behind the last place are left out (status bit 2)."""
     dv = head_dim_k if head_dim_v is None else head_dim_v
     if dtype not in (torch.float16, torch.bfloat16):
         raise RuntimeError("dtype must be float16 or bfloat16")
@@ -605,7 +605,8 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: to
     """Attention of packed prompts of different lengths: q [tokens, heads, channels], k and v [key tokens, kv_heads, channels] (fp16
     or bf16; views of a fused q/k/v result are fine), request i owning rows cu_q[i] .. cu_q[i + 1] - 1 of q and cu_k[i] .. of k and
     v (cu_k None: the same).  With causal the last query of a request sees all its keys, the one before it all but the last.
-    Returns [tokens, heads, channels of v]; queries that see no key, and rows that no request owns, give zeros."""
+    Returns [tokens, heads, channels of v]; queries that see no key, and rows that no request owns, give zeros.
+    A request whose rows do not all exist (cu ends behind the tensors) gives zeros, too, and raises status bit 2."""
     if q.dim() != 3:
         raise RuntimeError("q must be a [tokens, heads, channels] CUDA tensor")
     scale = 1.0 / math.sqrt(max(q.shape[2], 1)) if softmax_scale is None else float(softmax_scale)
