@@ -100,3 +100,27 @@ def test_too_few_keys_for_a_chunk():
     cut = cache.attend(0, q, k, v, step._replace(max_keys=125))
     assert ops.read_and_clear_status("cuda") == 4
     assert torch.equal(cut[:7], out[:7]) and (cut[7:] == 0).all()
+
+
+@pytest.mark.parametrize("kind", ["decode", "chunk"])
+def test_a_step_keeps_its_lengths(kind):
+    """The next step may be planned before the layers of this one have run: a step attends to the keys that it was planned with."""
+    from uniql_b200.kv_cache import PagedKV4Cache
+    g = _gen(42)
+    caches = [PagedKV4Cache(1, 30, 2, 64, page_size=16, requests=3, max_tokens=160) for _ in range(2)]
+    new = [30, 47, 16]
+    rows = [_rows(g, sum(new), h, 64, F16).cuda() for h in (4, 2, 2)]
+    more = [1, 1, 1] if kind == "decode" else [5, 20, 1]
+    rows2 = [_rows(g, sum(more), h, 64, F16).cuda() for h in (4, 2, 2)]
+    outs = []
+    for ahead, cache in enumerate(caches):
+        step = cache.plan(torch.tensor(new, dtype=torch.int32).cuda(), sum(new), fresh=True)
+        cache.append(0, *rows[1:], step)
+        cache.codes[0][cache.block_table.max() + 1:] = 0x33333333     # what pages of ended requests hold
+        cache.scales[0][cache.block_table.max() + 1:] = 1.0
+        step = cache.plan_decode(3) if kind == "decode" else cache.plan(torch.tensor(more, dtype=torch.int32).cuda(), sum(more))
+        if ahead:
+            cache.plan(torch.tensor([9, 30, 2], dtype=torch.int32).cuda(), 41)
+        cache.append(0, *rows2[1:], step)
+        outs.append(cache.attend(0, *rows2, step))
+    assert torch.equal(*outs)

@@ -18,7 +18,8 @@ from . import fused, ops
 
 
 class KVStep(NamedTuple):
-    """One step's tokens, packed request after request."""
+    """One step's tokens, packed request after request, and the keys they attend to: another step may be planned before the layers of
+    this one have run.  `release` and `move` change the block table that all steps read: they come behind the layers."""
     rows: int                    # requests 0 .. rows - 1 take part
     single: bool                 # one new token for each of them: a decode step
     fresh: bool                  # no request had cached tokens before: keys and values of the step are all there is
@@ -26,6 +27,7 @@ class KVStep(NamedTuple):
     positions: torch.Tensor      # int64 [total]
     cu: torch.Tensor             # int32 [rows + 1]: first token of each request
     max_keys: int                # bound of the keys of all requests together, for a step that is neither single nor fresh
+    lens: torch.Tensor           # int32 [rows]: keys of each request, the step's own included
 
 
 class PagedKV4Cache:
@@ -56,10 +58,10 @@ class PagedKV4Cache:
         n = new_lens.shape[0]
         if n > self.block_table.shape[0]:
             raise RuntimeError(f"the cache has room for {self.block_table.shape[0]} requests")
-        slots, positions, cu, _, _ = ops.kv_page_plan(self.lens[:n], new_lens, self.block_table[:n], self.free_pages, self.free_count,
+        slots, positions, cu, lens, _ = ops.kv_page_plan(self.lens[:n], new_lens, self.block_table[:n], self.free_pages, self.free_count,
                                                       self.page_size, total, in_place=True)
         bound = min(n * self.block_table.shape[1], self.num_pages) * self.page_size
-        return KVStep(n, False, fresh, slots, positions, cu, bound if max_keys is None else min(bound, max_keys))
+        return KVStep(n, False, fresh, slots, positions, cu, bound if max_keys is None else min(bound, max_keys), lens.clone())
 
     def plan_decode(self, n) -> KVStep:
         """One new token for each of requests 0 .. n - 1."""
@@ -72,7 +74,7 @@ class PagedKV4Cache:
         """Attention of the step's queries q [total, heads, channels]; k and v are the step's own rows, already appended.  Decode
         steps read the cache in 4 bits, fresh prompts their own keys and values, later chunks of a prompt the cached rows of
         their requests, gathered."""
-        codes, scales, table, lens = self.codes[layer], self.scales[layer], self.block_table[:step.rows], self.lens[:step.rows]
+        codes, scales, table, lens = self.codes[layer], self.scales[layer], self.block_table[:step.rows], step.lens
         if step.single:
             return ops.kv4_attention(q, codes, scales, table, lens, self.head_dim_v, softmax_scale)
         if step.fresh:
