@@ -45,7 +45,7 @@ enum {
   UNIQL_STATUS_BAD_INDEX = 4,     /* a slicing index pointed outside the source layer; that column / row was written as zeros.
                                      KV cache: a slot or page number outside the cache; that token was skipped / read as absent.  Packed rows: bounds
                                      that leave the rows or descend */
-  UNIQL_STATUS_NO_PAGE = 8        /* uniql_kv_page_plan: the free stack or a row of the block table was too short */
+  UNIQL_STATUS_NO_PAGE = 8        /* uniql_kv_page_plan, uniql_kv_step_plan: the free stack or a row of the block table was too short */
 };
 
 int uniql_abi_version(void);
@@ -360,6 +360,14 @@ int uniql_w4a16_swap_plan_check(void);
  *   lens_out         int32 [batch] = len + new, free_count_out int32 [1] = what is left; either may be its input
  *   batch up to UNIQL_KV_MAX_BATCH.
  *
+ * uniql_kv_step_plan: the same for steps whose requests are served whole.  A request that cannot have all its pages, table columns and
+ *   places is left out: its length and its row of the table stay as they are, its slots are -1, UNIQL_STATUS_NO_PAGE is raised, and a
+ *   later step may ask for the same again.  Requests are served in order: what cannot be met by all free pages or the table's width is
+ *   left out by itself; of the others, once one does not fit, the ones behind it that need a page (or a place) are left out too.
+ *   lens_out is len + new of the served ones; cu_new stops at total_new.
+ *   key_lens         int32 [batch]: keys of each request in this step, len + new; 0 for one that is left out
+ *   cu_keys          int32 [batch + 1]: their exclusive sums (at most 2^30)
+ *
  * uniql_kv4_append: quantises the rows k[t], v[t] (t < tokens; [kv_heads, head] each, unit channel stride) and stores them at slots[t].
  *   zero = fp16(min), scale = fp16((max - min) / 15) but at least 2^-24, code = the nearest to (x - zero) / scale, ties to even,
  *   within 0..15.  Values beyond +-65504 are clamped to them first; a row that holds a NaN reads back as NaN.  A slot of -1
@@ -392,6 +400,11 @@ int uniql_kv_page_plan(const int32_t* lens, const int32_t* new_lens, int64_t bat
                        int64_t max_blocks, const int32_t* free_pages, int64_t free_cap, const int32_t* free_count,
                        int64_t page_size, int64_t total_new, int64_t* slots, int64_t* positions, int32_t* cu_new,
                        int32_t* lens_out, int32_t* free_count_out, int* status_word, void* stream);
+int uniql_kv_step_plan(const int32_t* lens, const int32_t* new_lens, int64_t batch, int32_t* block_table, int64_t ld_table,
+                       int64_t max_blocks, const int32_t* free_pages, int64_t free_cap, const int32_t* free_count,
+                       int64_t page_size, int64_t total_new, int64_t* slots, int64_t* positions, int32_t* cu_new,
+                       int32_t* lens_out, int32_t* free_count_out, int32_t* key_lens, int32_t* cu_keys, int* status_word,
+                       void* stream);
 int uniql_kv4_append(const void* k, int64_t k_token_stride, int64_t k_head_stride, const void* v, int64_t v_token_stride,
                      int64_t v_head_stride, int dtype, int64_t tokens, int64_t kv_heads, int64_t dk, int64_t dv,
                      const int64_t* slots, void* codes, void* scales, int64_t num_pages, int64_t page_size, int64_t dp,

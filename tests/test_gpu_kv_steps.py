@@ -124,3 +124,137 @@ def test_a_step_keeps_its_lengths(kind):
         cache.append(0, *rows2[1:], step)
         outs.append(cache.attend(0, *rows2, step))
     assert torch.equal(*outs)
+
+
+def _whole(lens, new, table, count, page, width, total):
+    """Which requests a step serves: those whose pages, columns and places all fit, in order; an impossible one stands in nobody's way."""
+    left, at, stop, served = count, 0, False, []
+    for n, add in zip(lens, new):
+        need = -(-(n + add) // page) - -(-n // page)
+        at += add
+        if (add and -(-(n + add) // page) > width) or need > count:
+            served.append(False)
+            continue
+        left -= need
+        served.append(not (add and at > total) and not (need and left < 0))
+    return served
+
+
+@pytest.mark.parametrize("new,total,served", [
+    ([320, 10, 3], 333, [False, True, True]),                     # more pages than there are: the others are served
+    ([64, 70, 8], 142, [True, False, True]),                      # what the first leaves is too little for the second; the third needs none
+    ([96, 0, 0], 96, [True, True, True]), ([1, 1, 1], 3, [True, True, True]),
+    ([10, 10, 400], 420, [True, True, False]),                    # more columns than the table has
+    ([10, 10, 4], 22, [True, True, False]),                       # fewer rows in the step than tokens
+    ([0, 700, 0], 700, [True, False, True])])
+def test_shortage_leaves_whole_requests_out(route, new, total, served):
+    """A request that cannot have all its pages keeps its length and pages, gives zeros, and is served once there are pages again; the
+    others of the step are not touched by it."""
+    from uniql_b200 import ops
+    from uniql_b200.kv_cache import PagedKV4Cache
+    g = _gen(sum(new))
+    d, heads, kv = 64, 4, 2
+    cache = PagedKV4Cache(1, 10, kv, d, page_size=16, requests=3, max_tokens=320)
+    old = [0, 48, 5]
+    step = cache.plan(torch.tensor(old, dtype=torch.int32).cuda(), 53, fresh=True)
+    cache.append(0, *(_rows(g, 53, kv, d, F16).cuda() for _ in range(2)), step)
+    before = cache.block_table.clone(), cache.free_pages.clone()
+    assert cache.free_count.item() == 6 and ops.read_and_clear_status("cuda") == 0
+    assert _whole(old, new, None, 6, 16, 20, total) == served
+
+    step = cache.plan(torch.tensor(new, dtype=torch.int32).cuda(), total)
+    held = [o + n * s for o, n, s in zip(old, new, served)]
+    taken = sum(-(-h // 16) - -(-o // 16) for h, o in zip(held, old))
+    assert ops.read_and_clear_status("cuda") == (0 if all(served) else 8)
+    assert cache.lens.tolist() == held and cache.free_count.item() == 6 - taken
+    q, k, v = (_rows(g, total, h, d, F16) for h in (heads, kv, kv))
+    cache.append(0, k.cuda(), v.cuda(), step)
+    out = cache.attend(0, q.cuda(), k.cuda(), v.cuda(), step).cpu()
+    assert ops.read_and_clear_status("cuda") == 0                 # what is left out is no key of anybody
+    codes, scales, table = cache.codes[0].cpu(), cache.scales[0].cpu(), cache.block_table.cpu()
+    at = 0
+    for r, (o, n, s) in enumerate(zip(old, new, served)):
+        rows = slice(at, min(at + n, total))
+        at += n
+        slots = step.slots.cpu()[rows]
+        if not s:
+            assert torch.equal(table[r], before[0].cpu()[r]) and (slots == -1).all() and (out[rows] == 0).all()
+            continue
+        t = torch.arange(o, o + n)
+        assert torch.equal(slots, table[r].long()[t // 16] * 16 + t % 16)
+        assert (table[r, :-(-held[r] // 16)] >= 0).all() and (table[r, -(-held[r] // 16):] == -1).all()
+        keys, vals = (ref.cached(codes, scales, table[r], i, d, o + n)[0].to(F16) for i in (0, 1))
+        _prompt_check(out[rows], q[rows], keys, vals, [n], [o + n], True, 1 / math.sqrt(d))
+    # every page is free or in the table, once
+    pages = cache.free_pages[:cache.free_count.item()].tolist() + table[table >= 0].tolist()
+    assert sorted(pages) == list(range(10))
+    # with a request gone its pages serve the one that was left out
+    if served == [True, False, True] and total == 142:
+        cache.release([0])
+        step = cache.plan(torch.tensor([0, 70, 0], dtype=torch.int32).cuda(), 70)
+        assert cache.lens.tolist() == [0, 118, 13] and (step.slots >= 0).all() and ops.read_and_clear_status("cuda") == 0
+
+
+def test_decode_without_a_page_for_one_request(route):
+    from uniql_b200 import ops
+    from uniql_b200.kv_cache import PagedKV4Cache
+    g = _gen(43)
+    cache = PagedKV4Cache(1, 4, 2, 64, page_size=16, requests=3, max_tokens=64)
+    old = [16, 20, 3]                                             # the first needs a page, and there is none
+    step = cache.plan(torch.tensor(old, dtype=torch.int32).cuda(), 39, fresh=True)
+    cache.append(0, *(_rows(g, 39, 2, 64, F16).cuda() for _ in range(2)), step)
+    q, k, v = (_rows(g, 3, h, 64, F16).cuda() for h in (4, 2, 2))
+    step = cache.plan_decode(3)
+    cache.append(0, k, v, step)
+    out = cache.attend(0, q, k, v, step)
+    assert ops.read_and_clear_status("cuda") == 8
+    assert cache.lens.tolist() == [16, 21, 4] and step.slots.tolist()[0] == -1 and (out[0] == 0).all()
+    args = cache.codes[0], cache.scales[0], cache.block_table
+    assert torch.equal(out[1:], ops.kv4_attention(q[1:], *args[:2], cache.block_table[1:], cache.lens[1:])) and (out[1:] != 0).any()
+    cache.release([2])
+    step = cache.plan_decode(2)
+    cache.append(0, k[:2], v[:2], step)
+    cache.attend(0, q[:2], k[:2], v[:2], step)
+    assert cache.lens.tolist() == [17, 22, 0] and ops.read_and_clear_status("cuda") == 0
+
+
+@pytest.mark.parametrize("seed", range(4))
+def test_whole_requests_step_after_step(route, seed):
+    """Many ragged requests over few pages, in place, above and below the size at which a plan becomes two launches."""
+    from uniql_b200 import ops
+    g = _gen(100 + seed)
+    batch, page, width, most = ((7, 16, 9, 40), (300, 16, 12, 90), (1100, 32, 9, 30), (40, 256, 5, 700))[seed]
+    pages = batch * 2
+    lens, table = [0] * batch, torch.full((batch, width), -1, dtype=torch.int32)
+    free, count = torch.randperm(pages, generator=g).int(), pages
+    d = [torch.tensor(lens, dtype=torch.int32).cuda(), table.cuda(), free.cuda(), torch.tensor([count], dtype=torch.int32).cuda()]
+    some = False
+    for step in range(6):
+        new = torch.randint(0, most, (batch,), generator=g)
+        new[torch.rand(batch, generator=g) < 0.2] = 0
+        total = int(new.sum()) - (3 if step == 4 else -5)
+        served = _whole(lens, new.tolist(), None, count, page, width, total)
+        some |= not all(served)
+        got = ops.kv_page_plan(d[0], new.int().cuda(), d[1], d[2], d[3], page, total, in_place=True, whole=True)
+        slots, at = [], 0
+        for r, (n, add, s) in enumerate(zip(list(lens), new.tolist(), served)):
+            if s:
+                for b in range(-(-n // page), -(-(n + add) // page)):
+                    count -= 1
+                    table[r, b] = free[count]
+                lens[r] = n + add
+            slots += [int(table[r, t // page]) * page + t % page if s else -1 for t in range(n, n + add)]
+        slots = (slots + [-1] * total)[:total]
+        assert torch.equal(d[1].cpu(), table) and got[0].tolist() == slots and d[0].tolist() == lens and d[3].item() == count
+        keys = [n if s else 0 for n, s in zip(lens, served)]
+        assert got[2].tolist() == _cu(new.tolist()).clamp(max=total).tolist() and got[5].tolist() == keys and got[6].tolist() == _cu(keys).tolist()
+        assert ops.read_and_clear_status("cuda") == (0 if all(served) else 8)
+        if step == 2:                                             # half of the requests end: their pages go back
+            for r in range(0, batch, 2):
+                back = table[r][table[r] >= 0]
+                free[count:count + back.numel()] = back
+                count += back.numel()
+                table[r], lens[r] = -1, 0
+            for t, x in zip(d, (torch.tensor(lens, dtype=torch.int32), table, free, torch.tensor([count], dtype=torch.int32))):
+                t.copy_(x)
+    assert some

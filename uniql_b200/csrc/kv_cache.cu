@@ -13,6 +13,11 @@ namespace uniql {
 // more than thousands of single ones.  lens and free_count may be overwritten in place, so what goes there waits for every CTA's
 // reads: up to 8 CTAs are one cluster with a barrier; a step of more tokens than those have threads for takes a grid over the
 // GPU and a second launch of one CTA (257328 tokens of 1024 requests: 35 us in one cluster, 9.5 as grid and second launch).
+//
+// A step's plan (cu_keys given) serves whole requests: one that cannot have all its pages, columns and places keeps its length and
+// takes nothing.  What is impossible by itself does not count for the others; of the rest, the ones whose inclusive sums stay within
+// the stack and the places are served.  A later request that needs a page sums to more than an earlier one that was left out, so the
+// served ones' pages are the first of the list and s_first holds for them as it is.  s_len of a request left out is ~len.
 constexpr int kPlanThreads = 1024, kPlanCap = 1 << 30;
 
 struct PlanParams {
@@ -28,6 +33,8 @@ struct PlanParams {
   int32_t* lens_out;
   int32_t* free_count_out;
   int* status_word;
+  int32_t* key_lens;                            // of a step's plan: keys of each request, and their exclusive sums
+  int32_t* cu_keys;
   int64_t total_new;
   int batch, max_blocks, free_cap, page_shift;
   int lists, totals;                            // what this launch does: pages and tokens; lengths, starts and count
@@ -49,29 +56,37 @@ __global__ void __launch_bounds__(kPlanThreads) kv_page_plan_kernel(const __grid
   int* s_cu = s_len + p.batch;                  // [batch + 1]
   int* s_first = s_cu + p.batch + 1;            // [batch + 1]
   __shared__ long long warp_new[32], warp_need[32];
-  __shared__ long long carry_new, carry_need;
-  __shared__ int s_count;
+  __shared__ long long carry_new, carry_need, carry_keys;
+  __shared__ int s_count, s_taken;
   pdl_wait();
   pdl_launch_dependents();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int pmask = (1 << p.page_shift) - 1;
   if (tid == 0) {
-    carry_new = carry_need = 0;
+    carry_new = carry_need = carry_keys = 0;
+    s_taken = 0;
     s_cu[0] = s_first[0] = 0;                   // all there is of them when the batch is empty
     s_count = min(max(p.free_count[0], 0), p.free_cap);
   }
+  const bool whole = p.cu_keys != nullptr, sums = whole && p.totals && blockIdx.x == 0;
   bool short_table = false;
   __syncthreads();
   for (int i0 = 0; i0 < p.batch; i0 += kPlanThreads) {
     const int i = i0 + tid;
     int len = 0, add = 0, need = 0;
+    bool out = false;                           // not served by a step's plan
     if (i < p.batch) {
       len = min(max(p.lens[i], 0), kMaxTokens);
       add = min(max(p.new_lens[i], 0), kMaxTokens);
       const int had = (len + pmask) >> p.page_shift, has = (len + add + pmask) >> p.page_shift;
       need = max(min(has, p.max_blocks) - had, 0);
-      short_table |= has > p.max_blocks && add > 0;
-      s_len[i] = len;
+      if (whole) {
+        out = (has > p.max_blocks && add > 0) || need > s_count;
+        if (out) need = 0;
+      } else {
+        short_table |= has > p.max_blocks && add > 0;
+        s_len[i] = len;
+      }
     }
     long long xn = add, xb = need;              // inclusive sums over the warp, then over the block
 #pragma unroll
@@ -98,7 +113,36 @@ __global__ void __launch_bounds__(kPlanThreads) kv_page_plan_kernel(const __grid
       s_cu[i] = (int)min(bn + xn - add, (long long)kPlanCap);
       s_first[i] = (int)min(bb + xb - need, (long long)kPlanCap);
     }
+    if (whole && i < p.batch) {
+      out |= (add > 0 && bn + xn > p.total_new) || (need > 0 && bb + xb > s_count);
+      if (!out && need > 0) atomicMax(&s_taken, (int)(bb + xb));
+      short_table |= out;
+      s_len[i] = out ? ~len : len;
+    }
     __syncthreads();
+    if (sums) {
+      const int keys = i < p.batch && !out ? len + add : 0;
+      long long xk = keys;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const long long v = __shfl_up_sync(~0u, xk, o);
+        if (lane >= o) xk += v;
+      }
+      // bn and bb of this round have been taken: the warps' sums may go
+      if (lane == 31) warp_need[warp] = xk;
+      __syncthreads();
+      long long bk = lane < warp ? warp_need[lane] : 0;
+#pragma unroll
+      for (int o = 16; o; o >>= 1) bk += __shfl_xor_sync(~0u, bk, o);
+      bk += carry_keys;
+      if (i < p.batch) {
+        p.key_lens[i] = keys;
+        p.cu_keys[i] = (int)min(bk + xk - keys, (long long)kPlanCap);
+        if (i == p.batch - 1) p.cu_keys[p.batch] = (int)min(bk + xk, (long long)kPlanCap);
+      }
+      __syncthreads();
+      if (tid == kPlanThreads - 1) carry_keys = bk + xk;
+    }
     if (tid == kPlanThreads - 1) {
       carry_new = bn + xn;
       carry_need = bb + xb;
@@ -107,11 +151,12 @@ __global__ void __launch_bounds__(kPlanThreads) kv_page_plan_kernel(const __grid
     }
     __syncthreads();
   }
-  const int tokens = s_cu[p.batch], pages = s_first[p.batch], count = s_count;
+  if (sums && p.batch == 0 && tid == 0) p.cu_keys[0] = 0;
+  const int tokens = s_cu[p.batch], count = s_count, pages = whole ? s_taken : s_first[p.batch];
   const int rank = blockIdx.x, ranks = gridDim.x, step = ranks * kPlanThreads;
   if (p.lists) {
   for (int x = rank * kPlanThreads + tid; x < pages; x += step) {
-    const int i = plan_find(s_first, p.batch, x);
+    const int i = plan_find(s_first, p.batch, x);       // a served one: theirs are the first places
     const int had = (s_len[i] + pmask) >> p.page_shift;
     p.table[(size_t)i * p.ld_table + had + (x - s_first[i])] = x < count ? p.free_pages[count - 1 - x] : -1;
   }
@@ -119,10 +164,10 @@ __global__ void __launch_bounds__(kPlanThreads) kv_page_plan_kernel(const __grid
     int64_t slot = -1, pos = 0;
     if (x < tokens) {
       const int i = plan_find(s_cu, p.batch, (int)x);
-      const int len = s_len[i], at = len + ((int)x - s_cu[i]), had = (len + pmask) >> p.page_shift;
-      const int block = at >> p.page_shift;
+      const int held = s_len[i], len = held < 0 ? ~held : held, at = len + ((int)x - s_cu[i]);
+      const int had = (len + pmask) >> p.page_shift, block = at >> p.page_shift;
       int page = -1;
-      if (block < p.max_blocks) {
+      if (held >= 0 && block < p.max_blocks) {
         const int r = s_first[i] + block - had;
         if (block < had) page = p.table[(size_t)i * p.ld_table + block];
         else if (r < count) page = p.free_pages[count - 1 - r];
@@ -141,8 +186,8 @@ __global__ void __launch_bounds__(kPlanThreads) kv_page_plan_kernel(const __grid
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
   if (rank == 0) {
     for (int i = tid; i <= p.batch; i += kPlanThreads) {
-      p.cu_new[i] = s_cu[i];
-      if (i < p.batch) p.lens_out[i] = s_len[i] + min(max(p.new_lens[i], 0), kMaxTokens);
+      p.cu_new[i] = whole ? (int)min((int64_t)s_cu[i], p.total_new) : s_cu[i];
+      if (i < p.batch) p.lens_out[i] = s_len[i] < 0 ? ~s_len[i] : s_len[i] + min(max(p.new_lens[i], 0), kMaxTokens);
     }
     if (tid == 0) p.free_count_out[0] = max(count - pages, 0);
   }
@@ -451,11 +496,10 @@ __global__ void __launch_bounds__(kGatherThreads) kv4_gather_kernel(const __grid
 }  // namespace uniql
 
 // ------------------------------------------------------------------------------------------------ C ABI
-extern "C" int uniql_kv_page_plan(const int32_t* lens, const int32_t* new_lens, int64_t batch, int32_t* block_table,
-                                  int64_t ld_table, int64_t max_blocks, const int32_t* free_pages, int64_t free_cap,
-                                  const int32_t* free_count, int64_t page_size, int64_t total_new, int64_t* slots,
-                                  int64_t* positions, int32_t* cu_new, int32_t* lens_out, int32_t* free_count_out,
-                                  int* status_word, void* stream) {
+static int kv_plan(const int32_t* lens, const int32_t* new_lens, int64_t batch, int32_t* block_table, int64_t ld_table,
+                   int64_t max_blocks, const int32_t* free_pages, int64_t free_cap, const int32_t* free_count, int64_t page_size,
+                   int64_t total_new, int64_t* slots, int64_t* positions, int32_t* cu_new, int32_t* lens_out,
+                   int32_t* free_count_out, int32_t* key_lens, int32_t* cu_keys, int* status_word, void* stream) {
   using namespace uniql;
   if (batch < 0 || total_new < 0 || max_blocks < 0 || free_cap < 0 || ld_table < max_blocks) return UNIQL_EINVAL;
   const int shift = page_shift_of(page_size);
@@ -468,6 +512,7 @@ extern "C" int uniql_kv_page_plan(const int32_t* lens, const int32_t* new_lens, 
   p.lens = lens; p.new_lens = new_lens; p.table = block_table; p.ld_table = ld_table;
   p.free_pages = free_pages; p.free_count = free_count; p.slots = slots; p.positions = positions;
   p.cu_new = cu_new; p.lens_out = lens_out; p.free_count_out = free_count_out; p.status_word = status_word;
+  p.key_lens = key_lens; p.cu_keys = cu_keys;
   p.total_new = total_new; p.batch = (int)batch; p.max_blocks = (int)max_blocks; p.free_cap = (int)free_cap; p.page_shift = shift;
   const size_t smem = (3 * (size_t)batch + 2) * sizeof(int);
   // raised for every size: what a kernel gets by default counts its static shared memory too
@@ -503,6 +548,25 @@ extern "C" int uniql_kv_page_plan(const int32_t* lens, const int32_t* new_lens, 
   const int64_t sms = device_info().sm_count;
   const int st = launch(ctas < sms ? ctas : sms, 1, 1, 0);
   return st != UNIQL_OK ? st : launch(1, 1, 0, 1);
+}
+
+extern "C" int uniql_kv_page_plan(const int32_t* lens, const int32_t* new_lens, int64_t batch, int32_t* block_table,
+                                  int64_t ld_table, int64_t max_blocks, const int32_t* free_pages, int64_t free_cap,
+                                  const int32_t* free_count, int64_t page_size, int64_t total_new, int64_t* slots,
+                                  int64_t* positions, int32_t* cu_new, int32_t* lens_out, int32_t* free_count_out,
+                                  int* status_word, void* stream) {
+  return kv_plan(lens, new_lens, batch, block_table, ld_table, max_blocks, free_pages, free_cap, free_count, page_size, total_new,
+                 slots, positions, cu_new, lens_out, free_count_out, nullptr, nullptr, status_word, stream);
+}
+
+extern "C" int uniql_kv_step_plan(const int32_t* lens, const int32_t* new_lens, int64_t batch, int32_t* block_table,
+                                  int64_t ld_table, int64_t max_blocks, const int32_t* free_pages, int64_t free_cap,
+                                  const int32_t* free_count, int64_t page_size, int64_t total_new, int64_t* slots,
+                                  int64_t* positions, int32_t* cu_new, int32_t* lens_out, int32_t* free_count_out,
+                                  int32_t* key_lens, int32_t* cu_keys, int* status_word, void* stream) {
+  if (!cu_keys || (batch > 0 && !key_lens)) return UNIQL_EINVAL;
+  return kv_plan(lens, new_lens, batch, block_table, ld_table, max_blocks, free_pages, free_cap, free_count, page_size, total_new,
+                 slots, positions, cu_new, lens_out, free_count_out, key_lens, cu_keys, status_word, stream);
 }
 
 extern "C" int uniql_kv4_append(const void* k, int64_t k_token_stride, int64_t k_head_stride, const void* v,

@@ -329,7 +329,7 @@ at::Tensor part_of(const at::Tensor& bytes, int64_t offset, int64_t n, at::Scala
 
 std::vector<at::Tensor> kv_page_plan(const at::Tensor& lens, const at::Tensor& new_lens, const at::Tensor& block_table,
                                      const at::Tensor& free_pages, const at::Tensor& free_count, int64_t page_size,
-                                     int64_t total_new, bool in_place) {
+                                     int64_t total_new, bool in_place, bool whole) {
   check_ints(lens, lens, 1, "lens");
   check_ints(new_lens, lens, 1, "new_lens");
   check_ints(block_table, lens, 2, "block_table");
@@ -343,20 +343,26 @@ std::vector<at::Tensor> kv_page_plan(const at::Tensor& lens, const at::Tensor& n
   const c10::cuda::CUDAGuard guard(lens.device());
   const int dev = lens.device().index();
   const int64_t longs = 16 * total_new, ints = 4 * (batch + 1);
-  at::Tensor buf = new_tensor({longs + 2 * ints + 4}, at::kByte, lens.device());
+  at::Tensor buf = new_tensor({longs + (whole ? 4 : 2) * ints + 4}, at::kByte, lens.device());
   at::Tensor slots = part_of(buf, 0, total_new, at::kLong), positions = part_of(buf, 8 * total_new, total_new, at::kLong);
   at::Tensor cu = part_of(buf, longs, batch + 1, at::kInt);
   at::Tensor lens_out = in_place ? lens : part_of(buf, longs + ints, batch, at::kInt);
   at::Tensor count_out = in_place ? free_count : part_of(buf, longs + 2 * ints, 1, at::kInt);
   at::Tensor status = status_tensor(dev);
-  const int code = uniql_kv_page_plan(
-      (const int32_t*)lens.data_ptr(), (const int32_t*)new_lens.data_ptr(), batch, (int32_t*)block_table.data_ptr(),
-      batch > 1 ? block_table.stride(0) : width, width, (const int32_t*)free_pages.data_ptr(), free_pages.size(0),
-      (const int32_t*)free_count.data_ptr(), page_size, total_new, (int64_t*)slots.data_ptr(), (int64_t*)positions.data_ptr(),
-      (int32_t*)cu.data_ptr(), (int32_t*)lens_out.data_ptr(), (int32_t*)count_out.data_ptr(), (int*)status.data_ptr(),
-      at::cuda::getCurrentCUDAStream(dev).stream());
-  check_code(code, "uniql_kv_page_plan");
-  return {slots, positions, cu, lens_out, count_out};
+  auto plan = [&](auto fn, auto... keys) {
+    return fn((const int32_t*)lens.data_ptr(), (const int32_t*)new_lens.data_ptr(), batch, (int32_t*)block_table.data_ptr(),
+              batch > 1 ? block_table.stride(0) : width, width, (const int32_t*)free_pages.data_ptr(), free_pages.size(0),
+              (const int32_t*)free_count.data_ptr(), page_size, total_new, (int64_t*)slots.data_ptr(),
+              (int64_t*)positions.data_ptr(), (int32_t*)cu.data_ptr(), (int32_t*)lens_out.data_ptr(),
+              (int32_t*)count_out.data_ptr(), keys..., (int*)status.data_ptr(), at::cuda::getCurrentCUDAStream(dev).stream());
+  };
+  if (!whole) {
+    check_code(plan(uniql_kv_page_plan), "uniql_kv_page_plan");
+    return {slots, positions, cu, lens_out, count_out};
+  }
+  at::Tensor key_lens = part_of(buf, longs + 2 * ints + 4, batch, at::kInt), cu_keys = part_of(buf, longs + 3 * ints + 4, batch + 1, at::kInt);
+  check_code(plan(uniql_kv_step_plan, (int32_t*)key_lens.data_ptr(), (int32_t*)cu_keys.data_ptr()), "uniql_kv_step_plan");
+  return {slots, positions, cu, lens_out, count_out, key_lens, cu_keys};
 }
 
 void kv4_append(const at::Tensor& k, const at::Tensor& v, const at::Tensor& slots, const at::Tensor& codes, const at::Tensor& scales) {

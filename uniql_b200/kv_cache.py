@@ -27,7 +27,8 @@ class KVStep(NamedTuple):
     positions: torch.Tensor      # int64 [total]
     cu: torch.Tensor             # int32 [rows + 1]: first token of each request
     max_keys: int                # bound of the keys of all requests together, for a step that is neither single nor fresh
-    lens: torch.Tensor           # int32 [rows]: keys of each request, the step's own included
+    lens: torch.Tensor           # int32 [rows]: keys of each request, the step's own included (0: left out of the step)
+    cu_keys: torch.Tensor        # int32 [rows + 1]: their exclusive sums
 
 
 class PagedKV4Cache:
@@ -54,14 +55,19 @@ class PagedKV4Cache:
         """Take pages for new_lens[i] (int32, CUDA) tokens of requests 0 .. len(new_lens) - 1, `total` rows of tokens in all (rows
         behind the last token are padding), and move their lengths on.  fresh: the caller knows that all of them were empty.
         max_keys: bound of the requests' keys together after the step, where they are known to be fewer than their tables can
-        hold (a prompt step behind a prefix gathers that many rows)."""
+        hold (a prompt step behind a prefix gathers that many rows); requests that do not fit into it give zeros and raise
+        status bit 2.
+
+        A request that cannot have all its pages, within `total` rows and the table, is left out (status bit 3): it keeps its
+        length and pages, nothing of it is stored, and its rows of a decode step or of a chunk come out as zeros (a fresh step
+        works out its rows, but the cache does not hold them).  It may be planned again once `release` has given pages back."""
         n = new_lens.shape[0]
         if n > self.block_table.shape[0]:
             raise RuntimeError(f"the cache has room for {self.block_table.shape[0]} requests")
-        slots, positions, cu, lens, _ = ops.kv_page_plan(self.lens[:n], new_lens, self.block_table[:n], self.free_pages, self.free_count,
-                                                      self.page_size, total, in_place=True)
+        slots, positions, cu, _, _, lens, cu_keys = ops.kv_page_plan(self.lens[:n], new_lens, self.block_table[:n], self.free_pages,
+                                                                     self.free_count, self.page_size, total, in_place=True, whole=True)
         bound = min(n * self.block_table.shape[1], self.num_pages) * self.page_size
-        return KVStep(n, False, fresh, slots, positions, cu, bound if max_keys is None else min(bound, max_keys), lens.clone())
+        return KVStep(n, False, fresh, slots, positions, cu, bound if max_keys is None else min(bound, max_keys), lens, cu_keys)
 
     def plan_decode(self, n) -> KVStep:
         """One new token for each of requests 0 .. n - 1."""
@@ -79,10 +85,8 @@ class PagedKV4Cache:
             return ops.kv4_attention(q, codes, scales, table, lens, self.head_dim_v, softmax_scale)
         if step.fresh:
             return ops.prompt_attention(q, k, v, step.cu, None, True, softmax_scale)
-        cu_k = torch.zeros(step.rows + 1, dtype=torch.int32, device=lens.device)
-        torch.cumsum(lens, 0, dtype=torch.int32, out=cu_k[1:])
-        kk, vv = ops.kv4_gather(codes, scales, table, cu_k, step.max_keys, self.head_dim_k, self.head_dim_v, q.dtype)
-        return ops.prompt_attention(q, kk, vv, step.cu, cu_k, True, softmax_scale)
+        kk, vv = ops.kv4_gather(codes, scales, table, step.cu_keys, step.max_keys, self.head_dim_k, self.head_dim_v, q.dtype)
+        return ops.prompt_attention(q, kk, vv, step.cu, step.cu_keys, True, softmax_scale)
 
     def release(self, rows) -> None:
         """Give the pages of finished requests back.  Synchronises with the host: not for the inside of a captured step.  The rows

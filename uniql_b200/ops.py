@@ -460,15 +460,18 @@ def kv4_cache(num_pages: int, kv_heads: int, page_size: int, head_dim: int, devi
 
 
 def kv_page_plan(lens: torch.Tensor, new_lens: torch.Tensor, block_table: torch.Tensor, free_pages: torch.Tensor,
-                 free_count: torch.Tensor, page_size: int, total_new: int, in_place: bool = False):
+                 free_count: torch.Tensor, page_size: int, total_new: int, in_place: bool = False, whole: bool = False):
     """What a step's new tokens need, worked out on the GPU from the requests' lengths: pages from the top of the stack
     `free_pages` (free_count[0] of them are left) go into `block_table` in place.  Returns (slots int64 [total_new], positions
     int64 [total_new], cu_new int32 [batch + 1], lens after the step, free_count after the step); with in_place the last two are
     `lens` and `free_count` themselves.  total_new: places to fill (the rows of the step's tensors; those behind the last
-    token get slot -1).  A shortage of pages or of table columns gives slots of -1 and status bit 3."""
+    token get slot -1).  A shortage of pages or of table columns gives slots of -1 and status bit 3.  With `whole` a request that
+    cannot have all its pages, columns and places is left out of the step (its length and table row stay, its slots are -1), and two
+    more results say what the step attends to: its requests' keys (int32 [batch], 0 for one left out) and their exclusive sums
+    (int32 [batch + 1]).  The results may share one storage."""
     ext = torch_ext()
     if ext is not None:
-        return tuple(ext.kv_page_plan(lens, new_lens, block_table, free_pages, free_count, page_size, total_new, in_place))
+        return tuple(ext.kv_page_plan(lens, new_lens, block_table, free_pages, free_count, page_size, total_new, in_place, whole))
     for t, dim, name in ((lens, 1, "lens"), (new_lens, 1, "new_lens"), (block_table, 2, "block_table"), (free_pages, 1, "free_pages"),
                          (free_count, 1, "free_count")):
         _ints(t, lens, dim, name)
@@ -483,13 +486,15 @@ def kv_page_plan(lens: torch.Tensor, new_lens: torch.Tensor, block_table: torch.
     cu = torch.empty(batch + 1, dtype=torch.int32, device=dev)
     lens_out = lens if in_place else torch.empty_like(lens)
     count_out = free_count if in_place else torch.empty_like(free_count)
+    keys = (torch.empty(batch, dtype=torch.int32, device=dev), torch.empty_like(cu)) if whole else ()
+    name = "uniql_kv_step_plan" if whole else "uniql_kv_page_plan"
     with torch.cuda.device(dev):
-        code = lib().uniql_kv_page_plan(lens.data_ptr(), new_lens.data_ptr(), batch, block_table.data_ptr(), ld, block_table.shape[1],
-                                        free_pages.data_ptr(), free_pages.shape[0], free_count.data_ptr(), page_size, total_new,
-                                        slots.data_ptr(), positions.data_ptr(), cu.data_ptr(), lens_out.data_ptr(),
-                                        count_out.data_ptr(), status_word(dev).data_ptr(), _stream_handle(dev))
-    check(code, "uniql_kv_page_plan")
-    return slots, positions, cu, lens_out, count_out
+        code = getattr(lib(), name)(lens.data_ptr(), new_lens.data_ptr(), batch, block_table.data_ptr(), ld, block_table.shape[1],
+                                    free_pages.data_ptr(), free_pages.shape[0], free_count.data_ptr(), page_size, total_new,
+                                    slots.data_ptr(), positions.data_ptr(), cu.data_ptr(), lens_out.data_ptr(), count_out.data_ptr(),
+                                    *(t.data_ptr() for t in keys), status_word(dev).data_ptr(), _stream_handle(dev))
+    check(code, name)
+    return slots, positions, cu, lens_out, count_out, *keys
 
 
 def kv4_append(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor) -> None:
