@@ -258,3 +258,103 @@ def test_whole_requests_step_after_step(route, seed):
             for t, x in zip(d, (torch.tensor(lens, dtype=torch.int32), table, free, torch.tensor([count], dtype=torch.int32))):
                 t.copy_(x)
     assert some
+
+
+# ------------------------------------------------------------------------------------------------ branches of large calls
+@pytest.mark.parametrize("short", [False, True])
+def test_plan_in_place_as_two_launches(route, short):
+    """More than 8192 new tokens of many ragged requests, in place, step after step; in the last one pages run out."""
+    from uniql_b200 import ops
+    g = _gen(50)
+    batch, page, width = 1200, 16, 12
+    free = torch.randperm(6 * batch, generator=g).int()
+    count = free.numel() if not short else 3 * batch
+    lens, table = torch.zeros(batch, dtype=torch.int32), torch.full((batch, width), -1, dtype=torch.int32)
+    d = [t.cuda() for t in (lens, table, free, torch.tensor([count], dtype=torch.int32))]
+    for step in range(4):
+        new = torch.randint(0, 30, (batch,), generator=g).int()
+        total = int(new.sum()) + 7
+        assert total > 8192
+        want = ref.plan(lens, new, table, free, count, page, total)
+        got = ops.kv_page_plan(d[0], new.cuda(), d[1], d[2], d[3], page, total, in_place=True)
+        table, lens, count = want[0], torch.tensor(want[4], dtype=torch.int32), want[5]
+        assert got[0].tolist() == want[1] and got[1].tolist() == want[2] and got[2].tolist() == want[3]
+        assert torch.equal(d[1].cpu(), table) and torch.equal(d[0].cpu(), lens) and d[3].item() == count
+        assert ops.read_and_clear_status("cuda") == (8 if want[6] else 0)
+    assert want[6] == short
+
+
+@pytest.mark.parametrize("batch", [1023, 1024, 1025, 3000])
+def test_gather_of_many_requests(route, batch):
+    """Up to 1024 requests the bounds are searched in shared memory, beyond them in global memory; many are empty, all start late."""
+    from uniql_b200 import ops
+    g = _gen(batch)
+    pages, page, d, kv = 64, 16, 64, 2
+    codes, scales = ops.kv4_cache(pages, kv, page, d)
+    n = pages * page
+    ops.kv4_append(_rows(g, n, kv, d, F16).cuda(), _rows(g, n, kv, d, F16).cuda(), torch.arange(n).cuda(), codes, scales)
+    table = torch.randint(0, pages, (batch, 3), generator=g).int()
+    counts = torch.randint(0, 5, (batch,), generator=g)
+    counts[torch.rand(batch, generator=g) < 0.5] = 0
+    counts[-1] = 3
+    starts = torch.randint(0, 40, (batch,), generator=g).int()
+    total = int(counts.sum()) + 9
+    got = ops.kv4_gather(codes, scales, table.cuda(), _cu(counts.tolist()).cuda(), total, d, starts=starts.cuda())
+    req = torch.repeat_interleave(torch.arange(batch), counts)
+    at = torch.cat([torch.arange(s, s + c) for s, c in zip(starts.tolist(), counts.tolist())])
+    slots = table[req, at // page].long() * page + at % page
+    every = ops.kv4_gather(codes, scales, torch.arange(pages, dtype=torch.int32)[None].cuda(), _cu([n]).cuda(), n, d)
+    for x, rows in zip(got, every):
+        assert torch.equal(x[:total - 9], rows[slots.cuda()]) and (x[total - 9:] == 0).all()
+    assert ops.read_and_clear_status("cuda") == 0
+
+
+def _striped(lens, heads, kv, d, g):
+    """Queries and a cache in which every 64 tokens raise two channels of the values, which no part of a list can be left out without
+    changing: all weights are alike within a factor of two."""
+    page = 64
+    blocks = [-(-n // page) for n in lens]
+    pages = sum(blocks)
+    order, table, at = torch.randperm(pages, generator=g).int(), torch.zeros(len(lens), max(blocks), dtype=torch.int32), 0
+    codes = torch.zeros(pages, 2, kv, page, 8, dtype=torch.int32)
+    scales = torch.zeros(pages, 2, kv, page, 2, dtype=F16)
+    for i, b in enumerate(blocks):
+        table[i, :b] = order[at:at + b]
+        at += b
+    c, s, z = ref.quantise(torch.randn(pages, kv, page, d, generator=g).half() * 0.1)
+    codes[:, 0], scales[:, 0] = ref.pack(c, 8), torch.stack((s, z), -1)
+    for i, b in enumerate(blocks):
+        for t in range(b):
+            x = torch.zeros(kv, page, d)
+            x[..., (7 * t + i) % d] = 1.0
+            x[..., (11 * t + 3 * i + 5) % d] = 1.0
+            c, s, z = ref.quantise(x)
+            codes[table[i, t].item(), 1], scales[table[i, t].item(), 1] = ref.pack(c, 8), torch.stack((s, z), -1)
+    return torch.randn(len(lens), heads, d, generator=g).half(), codes, scales, table
+
+
+@pytest.mark.parametrize("lens", [[40000], [24700] * 6, [24700] * 7, [25000] * 8, [24700] * 13, [24800] * 14, [24800] * 15, [30000, 24700, 100, 50000]])
+def test_no_part_of_a_long_list_is_lost(lens):
+    """Lists that are cut into 30 to 450 parts, more than 32 of which take the second turn of the join: each 64 tokens show in the result.
+    Bound per value: the result's rounding, weights rounded to fp16 next to codes centred by 8 steps of 1/15, scores in 32 bits."""
+    from uniql_b200 import ops
+    g = _gen(len(lens))
+    d = 64
+    q, codes, scales, table = _striped(lens, 2, 1, d, g)
+    got = ops.kv4_attention(*(t.cuda() for t in (q, codes, scales, table)), torch.tensor(lens, dtype=torch.int32).cuda()).cpu()
+    for b, n in enumerate(lens):
+        k = ref.cached(codes, scales, table[b], 0, d, n)[0]
+        v = ref.cached(codes, scales, table[b], 1, d, n)[0]
+        out, p, size, _ = ref.attend(q[b:b + 1].double(), k, v, torch.ones(1, n, dtype=torch.bool), 1 / 8)
+        # rounded weights: independent errors of at most 2^-11 of each term |c - 8| / 15 <= 8 / 15, so five deviations of their sum stay
+        # within 5 * 2^-11 * 8 / 15 * sqrt(sum p^2); their mean is zero because rounding is to nearest
+        off = 2 * (d + 16) * 2.0 ** -23 * (size[0] + 1.0)[:, None] + 2.0 ** -18
+        tol = out[0].abs() * (2.0 ** -11 + off) + 5 * 2.0 ** -11 * 8 / 15 * p[0].norm(dim=-1)[:, None] + 2.0 ** -18
+        assert ((got[b].double() - out[0]).abs() <= tol).all(), b
+        # any 64 tokens missing from the plain result would show
+        for t in range(0, n - 63, max(64, n // 64 // 40 * 64)):
+            rest = torch.ones(n, dtype=torch.bool)
+            rest[t:t + 64] = False
+            w = p[0][:, rest]
+            less = (w @ v[rest, 0]) / w.sum(-1, keepdim=True)
+            assert ((less - out[0]).abs() > 2 * tol).any(), (b, t)
