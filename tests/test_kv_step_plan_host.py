@@ -22,3 +22,12 @@ def test_cache_refuses_too_many_requests_and_cpu_lengths():
     for n in (3, 1):
         with pytest.raises(RuntimeError):
             cache.plan(torch.ones(n, dtype=torch.int32), n)
+
+
+@pytest.mark.parametrize("n", [3, -1])
+def test_decode_steps_of_requests_that_are_not_there(n):
+    """Refused before anything moves: the slice of one-token lengths would quietly be shorter than n."""
+    from uniql_b200.kv_cache import PagedKV4Cache
+    cache = PagedKV4Cache(1, 5, 1, 64, page_size=16, requests=2, max_tokens=64, device="cpu")
+    with pytest.raises(RuntimeError, match="room for 2"):
+        cache.plan_decode(n)

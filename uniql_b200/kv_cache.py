@@ -71,6 +71,8 @@ class PagedKV4Cache:
 
     def plan_decode(self, n) -> KVStep:
         """One new token for each of requests 0 .. n - 1."""
+        if not 0 <= n <= self.block_table.shape[0]:
+            raise RuntimeError(f"the cache has room for {self.block_table.shape[0]} requests")
         return self.plan(self._ones[:n], n)._replace(single=True)
 
     def append(self, layer, k, v, step) -> None:
