@@ -380,7 +380,9 @@ int uniql_w4a16_swap_plan_check(void);
  *
  * uniql_kv4_attention: one query token per request over its first lens[i] cached tokens (grouped heads: query head h reads kv head
  *   h / (heads / kv_heads)): out[i, h] = softmax(softmax_scale * q k^T) v in fp32, rounded once.  A V scale of 0 (a row that was
- *   never written) and a page outside the cache are absent tokens; without any token the result is zeros.  The work is split
+ *   never written) and a page outside the cache are absent tokens; without any token the result is zeros.  Roundings on the
+ *   way: q to fixed point, off by at most 2^-19 of its row's largest channel (a row below 2^-107 counts as zeros), and the weights
+ *   of the values to fp16; sums, maxima and parts are fp32.  The work is split
  *   over the GPU whatever the lengths are, and the parts of a request are joined in a fixed order: the same call gives the
  *   same bits.
  *   scratch  uniql_kv4_attention_scratch_bytes(...) bytes, rules as for uniql_w4a16_linear

@@ -1,17 +1,22 @@
 // Attention of one query token per request over a paged KV cache held in 4 bits.  Layout and rules: include/uniql_b200.h.
 //
 // Mathematics.  With a cached row k_t = z + s c and m = z + 8 s the score is  x_t = f (s (q . (c - 8)) + m sum(q)),  f =
-// softmax_scale log2(e).  q . (c - 8) is exact integer arithmetic on the tensor cores: four codes are the bytes of one AND, q is
-// rounded to 2^-19 of its largest channel or less and split into three signed base-128 digits, and mma.sync m16n8k32 (u8 x s8) sums
-// digit times code for each.  A packed word costs three instructions, all a half-rate pipe's, against five of that pipe and four of
-// the other one as two fp16 pairs: what bounds the arithmetic is that pipe (LOP3, PRMT, shifts: two cycles each).  (e4m3, where a
-// code is its own subnormal number, runs as conversions and fp16 products on this part.)  Scale and zero enter once per token in
-// fp32.
+// softmax_scale log2(e).  q . (c - 8) is integer arithmetic on the tensor cores: four codes are the bytes of one AND, q is a fixed-point
+// number that is off by at most 2^-19 of its largest channel, split into three signed base-128 digits, and mma.sync m16n8k32 (u8 x s8)
+// sums digit times code for each, exactly.  A packed word costs three instructions, all a half-rate pipe's, against five of that pipe
+// and four of the other one as two fp16 pairs: what bounds the arithmetic is that pipe (LOP3, PRMT, shifts: two cycles each).  (As
+// e4m3 products, where a code is its own subnormal number, the kernel was no faster.)  Scale and zero enter once per token in fp32.
 // The value side folds its scale into the exponent: with y_t = x_t + log2 s'_t, M a running bound of y and w_t = 2^(y_t - M),
 //     out = (sum w_t (c'_t - 8) + sum (w_t / s'_t) m'_t) / sum (w_t / s'_t),
-// so that w is the one operand that is rounded (fp16, 2^-12 relative above 6e-5; it is at most 2^8, see below), next to exact
-// fp16 codes, whatever the magnitude of the values.  M is raised, and the sums rescaled, only when some y exceeds it by more
+// so that of the second product w alone is rounded (fp16: by 2^-11 of itself, by 2^-25 below 6e-5; it is at most 2^8, see below), next to
+// exact fp16 codes, whatever the magnitude of the values.  M is raised, and the sums rescaled, only when some y exceeds it by more
 // than 8.
+//
+// What has fewer than 32 bits, and why: q's 20 bits in fixed point (small channels beside an outlier lose theirs; a row whose largest
+// channel is below 2^-107 counts as zeros), because the integer products take three digits; and w, because the second product would
+// cost twice as much with what fp16 leaves of it as another operand.  The sums of w are taken before it is rounded, and all sums, the
+// bound and the parts are fp32.  Error against 64 bits beside that of fp32 arithmetic, whose results are rounded alike: 1.0 to 1.2
+// times up to a few thousand tokens, 1.4 times (3.0e-4 of the result) at 131072.
 //
 // Layout of the products.  Tokens are the 16-row operand of the first product (a lane's packed words of two tokens are its
 // fragment; which channel sits at which k index is free, so long as the query fragments follow), query heads its eight
@@ -20,7 +25,8 @@
 // to the tensor cores in registers.
 //
 // Bound: HBM, (dk + dv) / 2 + 8 bytes per token and kv head, and close behind it the arithmetic: at 8 x 131072 tokens, 8 kv heads
-// (174 us at the measured copy rate), the loads alone take 180 us, the arithmetic alone 195 (as fp16 products), both 222.  Each
+// (174 us at the measured copy rate), the loads alone take 180 us, the arithmetic alone 195 (as fp16 products), both 225 in a short
+// burst and 245 to 260 back to back, where the power limit lowers the clock.  Each
 // warp keeps a ring of kStages steps of 32 tokens in flight with cp.async.
 //
 // Split: lengths are read on the device, and every CTA works out the same cut from them.  A step is 32 tokens of one request and kv

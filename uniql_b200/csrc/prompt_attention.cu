@@ -15,6 +15,10 @@
 // warp 11 looks the requests' bounds over.
 // Few units (at most one an SM) are items of their own: 256 tokens of 28 heads 8.8 us, 12.6 as pairs on half of the SMs.
 //
+// P has the input type because one product takes two operands of one type; its sum l is taken in fp32 before that.  Each term is off by
+// half a step of the type: error against 64 bits 1.2 to 1.4 times that of fp32 arithmetic, whose results are rounded alike.
+//
+// (Pairs of times below are short bursts of the kernel as it was when that step was made; they compare with each other alone.)
 // A thread stores 32 bytes of its row at a time: every store instruction touches 32 rows, which takes the load/store unit 32
 // cycles whatever their width (16 packed prompts: 497 us with 16 bytes at a time, 480 with 32).
 //
@@ -28,7 +32,8 @@
 // Bound: 128 keys of both units cost 2048 cycles of MMA, 2048 of shared memory traffic (Q and K are both read from there) and 2048
 // of exponentials (16 a clock and SM); they take 3135, the rest being the hops S -> softmax -> P -> O of a unit that the other
 // unit's work does not cover, at the 1.6 GHz that the part's power limit leaves (16384 tokens, 32 heads of 128, fp16, causal: 1.8 ms
-// in a short burst, 1.93 ms back to back = 1.14 PFLOP/s).  Tried without gain: S in two 64-key buffers a unit (Q is read twice as
+// in a short burst, 1.96 ms back to back = 1.12 PFLOP/s; 16 packed prompts of up to 2048 tokens, most behind a prefix: 535 us back to
+// back = 0.95 PFLOP/s of visible pairs).  Tried without gain: S in two 64-key buffers a unit (Q is read twice as
 // often: 2.07 ms against 1.79), P handed over in quarters (1.83 to 2.0), a quarter of the exponentials as polynomials on the FMA
 // pipe (1.75 to 1.96), waits polled without a suspend time (2.00 against 2.05 back to back).  These were measured with one CTA an item.
 // Every wait is bounded; a wait that gives up sets UNIQL_STATUS_WAIT_TIMEOUT and the kernel drains.
