@@ -358,3 +358,37 @@ def test_no_part_of_a_long_list_is_lost(lens):
             w = p[0][:, rest]
             less = (w @ v[rest, 0]) / w.sum(-1, keepdim=True)
             assert ((less - out[0]).abs() > 2 * tol).any(), (b, t)
+
+
+@pytest.mark.parametrize("bad", [0, 31, 4000, 5999])
+def test_bounds_of_thousands_of_requests_are_looked_over(bad):
+    """Most of the grid's CTAs never begin (others take their places): the look at the bounds must not be theirs."""
+    from uniql_b200 import ops
+    g = _gen(60)
+    n = 6000
+    q, k, v = (_rows(g, n, h, 64, F16).cuda() for h in (2, 1, 1))
+    cu = torch.arange(n + 1, dtype=torch.int32).cuda()
+    clean = ops.prompt_attention(q, k, v, cu, cu)
+    assert ops.read_and_clear_status("cuda") == 0
+    cu_k = cu.clone()
+    cu_k[bad] = n + 5 if bad else -1                              # one or two requests whose keys do not all exist
+    got = ops.prompt_attention(q, k, v, cu, cu_k)
+    assert ops.read_and_clear_status("cuda") == 4
+    hit = torch.zeros(n, dtype=torch.bool)
+    hit[max(bad - 1, 0):bad + 1] = True
+    assert (got[hit] == 0).all() and torch.equal(got[~hit], clean[~hit])
+
+
+def test_step_plan_without_requests_and_out_of_place(route):
+    from uniql_b200 import ops
+    from uniql_b200.kv_cache import PagedKV4Cache
+    cache = PagedKV4Cache(1, 9, 1, 64, page_size=16, requests=2, max_tokens=64)
+    step = cache.plan(torch.zeros(0, dtype=torch.int32).cuda(), 3)
+    assert step.slots.tolist() == [-1] * 3 and step.cu_keys.tolist() == [0] and step.lens.numel() == 0
+    out = cache.attend(0, *(torch.ones(3, h, 64, dtype=F16).cuda() for h in (2, 1, 1)), step)
+    assert (out == 0).all() and cache.free_count.item() == 9
+    new = torch.tensor([20, 70], dtype=torch.int32).cuda()        # the second has more tokens than the table columns
+    got = ops.kv_page_plan(cache.lens, new, cache.block_table, cache.free_pages, cache.free_count, 16, 90, whole=True)
+    assert cache.lens.tolist() == [0, 0] and cache.free_count.item() == 9
+    assert [t.tolist() for t in got[2:]] == [[0, 20, 90], [20, 0], [7], [20, 0], [0, 20, 20]]
+    assert (got[0][:20] >= 0).all() and (got[0][20:] == -1).all() and ops.read_and_clear_status("cuda") == 8

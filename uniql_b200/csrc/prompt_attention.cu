@@ -11,8 +11,7 @@
 //   P (16-bit, on the first 64 of S's columns) -- four softmax warps, one row a thread
 //   O (tensor memory) += P V, P read from tensor memory, V as an MN-major operand straight from its row-major tile
 // While the softmax of one unit runs the tensor cores work on the other:  warps 0-3 and 4-7 softmax of unit 0 and 1 (they also
-// rescale and store O), warp 8 issues the MMAs, warp 9 the TMA loads (no multicast), warp 10 hands out the items,
-// warp 11 looks the requests' bounds over.
+// rescale and store O), warp 8 issues the MMAs, warp 9 the TMA loads (no multicast), warp 10 hands out the items.
 // Few units (at most one an SM) are items of their own: 256 tokens of 28 heads 8.8 us, 12.6 as pairs on half of the SMs.
 //
 // P has the input type because one product takes two operands of one type; its sum l is taken in fp32 before that.  Each term is off by
@@ -44,8 +43,8 @@
 namespace uniql {
 
 namespace pa {
-constexpr int kMmaWarp = 8, kLoadWarp = 9, kPlanWarp = 10, kCheckWarp = 11;       // warps 0-7: softmax
-constexpr int kThreads = 384;                   // three warpgroups
+constexpr int kMmaWarp = 8, kLoadWarp = 9, kPlanWarp = 10;        // warps 0-7: softmax
+constexpr int kThreads = 384;                   // three warpgroups; the third has an idle warp
 constexpr int kSoftmaxRegs = 208, kOtherRegs = 80;      // 2 * 208 + 80 <= 3 * 168, what the block is launched with
 constexpr int kRows = 128, kKeys = 128;
 constexpr int kTmemCols = 512;                  // S0, S1, O0, O1: 128 columns each
@@ -277,7 +276,11 @@ prompt_attention_kernel(const __grid_constant__ PaParams p, const __grid_constan
       const int per = (p.batch + 31) / 32;
       const int b0 = min(lane * per, p.batch), b1 = min(b0 + per, p.batch);
       long long mine = 0;
-      for (int b = b0; b < b1; ++b) mine += pairs_of(b);
+      bool bad = false;                         // requests whose queries do not all exist, and below, of those with rows, keys
+      for (int b = b0; b < b1; ++b) {
+        mine += pairs_of(b);
+        bad |= p.cu_q[b] < 0 || p.cu_q[b + 1] < p.cu_q[b] || p.cu_q[b + 1] > p.total_q;
+      }
       long long incl = mine;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -314,7 +317,9 @@ prompt_attention_kernel(const __grid_constant__ PaParams p, const __grid_constan
             w.q0 = begin_q(b);
             w.nq = begin_q(b + 1) - w.q0;
             w.k0 = begin_k(b);
-            w.nk = sound(b) ? begin_k(b + 1) - w.k0 : 0;
+            const bool all = sound(b);
+            bad |= !all;
+            w.nk = all ? begin_k(b + 1) - w.k0 : 0;
             const int units = ((w.nq + p.tokens - 1) / p.tokens) * p.parts, u0 = p.units * (int)(n - 1 - (pair - at));
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
@@ -346,11 +351,7 @@ prompt_attention_kernel(const __grid_constant__ PaParams p, const __grid_constan
         if (timed_out) break;
         more = pa_next(tc_smem_addr(&s_next[k & 1]), x);
       }
-    }
-    if (warp == kCheckWarp) {                   // nobody waits for it: the bounds of all requests, over all CTAs
-      bool all = true;
-      for (long long b = blockIdx.x * 32ll + lane; b < p.batch; b += gridDim.x * 32ll) all &= sound((int)b);
-      if (!all && p.status_word) atomicOr(p.status_word, UNIQL_STATUS_BAD_INDEX);
+      if (bad && p.status_word) atomicOr(p.status_word, UNIQL_STATUS_BAD_INDEX);
     }
     if (warp == kLoadWarp) {
       // ------------------------------------------------------------------ loads: Q, then K 0, V 0, K 1, V 1, ... of every item
