@@ -31,8 +31,8 @@
 // Bound: 128 keys of both units cost 2048 cycles of MMA, 2048 of shared memory traffic (Q and K are both read from there) and 2048
 // of exponentials (16 a clock and SM); they take 3135, the rest being the hops S -> softmax -> P -> O of a unit that the other
 // unit's work does not cover, at the 1.6 GHz that the part's power limit leaves (16384 tokens, 32 heads of 128, fp16, causal: 1.8 ms
-// in a short burst, 1.96 ms back to back = 1.12 PFLOP/s; 16 packed prompts of up to 2048 tokens, most behind a prefix: 535 us back to
-// back = 0.95 PFLOP/s of visible pairs).  Tried without gain: S in two 64-key buffers a unit (Q is read twice as
+// in a short burst, 1.98 ms back to back = 1.11 PFLOP/s; 16 packed prompts of up to 2048 tokens, all behind a prefix: 541 us back to
+// back = 0.94 PFLOP/s of visible pairs).  Tried without gain: S in two 64-key buffers a unit (Q is read twice as
 // often: 2.07 ms against 1.79), P handed over in quarters (1.83 to 2.0), a quarter of the exponentials as polynomials on the FMA
 // pipe (1.75 to 1.96), waits polled without a suspend time (2.00 against 2.05 back to back).  These were measured with one CTA an item.
 // Every wait is bounded; a wait that gives up sets UNIQL_STATUS_WAIT_TIMEOUT and the kernel drains.
